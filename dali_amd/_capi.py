@@ -17,7 +17,7 @@ class DaliAmdError(RuntimeError):
 
 
 # ------------------------------------------------------------------ enums
-UINT8, FLOAT16, FLOAT, INT8, INT16, UINT16, INT32, UINT32 = 0, 1, 2, 3, 4, 5, 6, 7
+UINT8, FLOAT16, FLOAT, INT8, INT16, UINT16, INT32, UINT32, BFLOAT16, INT64 = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
 LAYOUT_HWC, LAYOUT_CHW = 0, 1
 INTERP_NN, INTERP_LINEAR, INTERP_TRIANGULAR, INTERP_CUBIC, INTERP_LANCZOS3, INTERP_GAUSSIAN = 0, 1, 2, 3, 4, 5
 JPEG_GRAY, JPEG_YCC, JPEG_RGB = 0, 1, 2
@@ -147,6 +147,54 @@ class PointwiseDesc(C.Structure):
                 ("wg_start", C.c_int32)]
 
 
+RECURRENCE_DECAY, RECURRENCE_GATE = 0, 1
+BLOCK_NORM_MAX_CHANNELS = 16384
+
+
+class SequenceRows(C.Structure):
+    _fields_ = [("offsets", C.c_void_p), ("lengths", C.c_void_p), ("rows", C.c_int64), ("steps", C.c_int64),
+                ("sequences", C.c_int32), ("index_dtype", C.c_int32)]
+
+
+class RecurrenceArgs(C.Structure):
+    _fields_ = [("seq", SequenceRows), ("x", C.c_void_p), ("decay", C.c_void_p), ("initial", C.c_void_p), ("y", C.c_void_p),
+                ("final_state", C.c_void_p), ("saved", C.c_void_p), ("dy", C.c_void_p), ("dfinal", C.c_void_p),
+                ("dx", C.c_void_p), ("ddecay", C.c_void_p), ("dinitial", C.c_void_p), ("x_row", C.c_int64),
+                ("x_seq", C.c_int64), ("decay_row", C.c_int64), ("decay_seq", C.c_int64), ("dy_row", C.c_int64),
+                ("dy_seq", C.c_int64), ("channels", C.c_int32), ("dtype", C.c_int32), ("decay_dtype", C.c_int32),
+                ("form", C.c_int32), ("per_channel", C.c_int32), ("reserved", C.c_int32)]
+
+
+class RecurrencePlan(C.Structure):
+    _fields_ = [("saved_bytes", C.c_size_t), ("forward_workspace_bytes", C.c_size_t), ("backward_workspace_bytes", C.c_size_t)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("gate", C.c_void_p), ("residual", C.c_void_p), ("post_weight", C.c_void_p),
+                ("scale", C.c_void_p), ("pre_weight", C.c_void_p), ("hidden", C.c_void_p), ("normed", C.c_void_p),
+                ("rstd_post", C.c_void_p), ("rstd_pre", C.c_void_p), ("dhidden", C.c_void_p), ("dnormed", C.c_void_p),
+                ("dx", C.c_void_p), ("dgate", C.c_void_p), ("dresidual", C.c_void_p), ("dpost_weight", C.c_void_p),
+                ("dscale", C.c_void_p), ("dpre_weight", C.c_void_p), ("rows", C.c_int64), ("x_row", C.c_int64),
+                ("gate_row", C.c_int64), ("residual_row", C.c_int64), ("dhidden_row", C.c_int64),
+                ("dnormed_row", C.c_int64), ("channels", C.c_int32), ("dtype", C.c_int32), ("residual_dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32)]
+
+
+class BlockNormPlan(C.Structure):
+    _fields_ = [("backward_workspace_bytes", C.c_size_t)]
+
+
+class EmbeddingArgs(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("table", C.c_void_p), ("out", C.c_void_p), ("dout", C.c_void_p), ("dtable", C.c_void_p),
+                ("tokens", C.c_int64), ("vocab", C.c_int64), ("padding", C.c_int64), ("table_row", C.c_int64),
+                ("dout_row", C.c_int64), ("channels", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("index_dtype", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class EmbeddingPlan(C.Structure):
+    _fields_ = [("backward_workspace_bytes", C.c_size_t)]
+
+
 # ------------------------------------------------------------------ structs (host)
 class JpegInfo(C.Structure):
     _fields_ = [("width", C.c_int32), ("height", C.c_int32), ("num_components", C.c_int32),
@@ -196,6 +244,9 @@ _KERNEL_SYMBOLS = [
     "daliamdAudioResampleLobes", "daliamdAudioResampleWindow", "daliamdAudioResampleSetup", "daliamdAudioResampleRun",
     "daliamdConvertNormSetup", "daliamdConvertNormRun",
     "daliamdNormalizeSetup", "daliamdNormalizeRun",
+    "daliamdRecurrenceSetup", "daliamdRecurrenceRun", "daliamdRecurrenceBackwardRun",
+    "daliamdBlockNormSetup", "daliamdBlockNormRun", "daliamdBlockNormBackwardRun",
+    "daliamdEmbeddingSetup", "daliamdEmbeddingRun", "daliamdEmbeddingBackwardRun",
 ]
 
 _HOST_SYMBOLS = [

@@ -1,0 +1,86 @@
+// Shared by the sequence operators (recurrence, block norm, embedding): element types, rows of sequences, the logistic
+// function.  Internal; not part of the C ABI.
+#ifndef DALI_AMD_CSRC_SEQUENCE_COMMON_H_
+#define DALI_AMD_CSRC_SEQUENCE_COMMON_H_
+
+#include "common.h"
+
+namespace daliamd {
+
+struct Bf16 { uint16_t bits; };
+typedef _Float16 F16;
+
+__device__ __forceinline__ float BitsToFloat(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(F16 v) { return (float)v; }
+__device__ __forceinline__ float ToFloat(Bf16 v) { return BitsToFloat((uint32_t)v.bits << 16); }
+
+template <typename T> __device__ __forceinline__ T FromFloat(float v);
+template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
+template <> __device__ __forceinline__ F16 FromFloat<F16>(float v) { return (F16)v; }
+template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
+#if defined(__AMDGCN__)
+  return Bf16{__builtin_bit_cast(uint16_t, (__bf16)v)};   // one instruction on gfx950: to nearest, ties to even
+#else
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return Bf16{(uint16_t)((u >> 16) | 0x40u)};
+  return Bf16{(uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};
+#endif
+}
+
+__device__ __forceinline__ float LoadElement(const void *p, int64_t i, int dtype) {
+  return dtype == DALIAMD_FLOAT ? static_cast<const float *>(p)[i]
+       : dtype == DALIAMD_FLOAT16 ? ToFloat(static_cast<const F16 *>(p)[i]) : ToFloat(static_cast<const Bf16 *>(p)[i]);
+}
+__device__ __forceinline__ void StoreElement(void *p, int64_t i, int dtype, float v) {
+  if (dtype == DALIAMD_FLOAT) static_cast<float *>(p)[i] = v;
+  else if (dtype == DALIAMD_FLOAT16) static_cast<F16 *>(p)[i] = FromFloat<F16>(v);
+  else static_cast<Bf16 *>(p)[i] = FromFloat<Bf16>(v);
+}
+
+inline bool IsSequenceType(int dtype) { return dtype == DALIAMD_FLOAT || dtype == DALIAMD_FLOAT16 || dtype == DALIAMD_BFLOAT16; }
+inline int ElementSize(int dtype) { return dtype == DALIAMD_FLOAT ? 4 : 2; }
+
+__device__ __forceinline__ int64_t LoadIndex(const void *p, int64_t i, int dtype) {
+  return dtype == DALIAMD_INT64 ? static_cast<const int64_t *>(p)[i] : (int64_t) static_cast<const int32_t *>(p)[i];
+}
+
+// the rows [begin, end) of sequence s, whatever the device holds in offsets / lengths
+__device__ __forceinline__ void SequenceRange(const daliamdSequenceRows &q, int s, int64_t *begin, int64_t *end) {
+  if (q.offsets) {
+    const int64_t b = min(max(LoadIndex(q.offsets, s, q.index_dtype), (int64_t)0), q.rows);
+    *begin = b;
+    *end = max(b, min(LoadIndex(q.offsets, s + 1, q.index_dtype), q.rows));
+  } else {
+    *begin = (int64_t)s * q.steps;
+    *end = *begin + (q.lengths ? min(max(LoadIndex(q.lengths, s, q.index_dtype), (int64_t)0), q.steps) : q.steps);
+  }
+}
+
+// the sequence that `row` belongs to, or -1: with ascending offsets the last one that begins at or before it
+__device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int64_t row, int64_t *begin, int64_t *end) {
+  int s;
+  if (q.offsets) {
+    int lo = 0, hi = q.sequences - 1;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (LoadIndex(q.offsets, mid, q.index_dtype) <= row) lo = mid; else hi = mid - 1;
+    }
+    s = lo;
+  } else {
+    s = (int)((uint32_t)row / (uint32_t)q.steps);
+  }
+  SequenceRange(q, s, begin, end);
+  return *begin <= row && row < *end ? s : -1;
+}
+
+__device__ __forceinline__ float Exp(float v) { return expf(v); }
+// f = 1 / (1 + exp(-g)) and k = 1 - f, both to the last bits: k is small where a gate holds, and it is what h moves by
+__device__ __forceinline__ void Logistic(float g, float *f, float *k) {
+  const float t = Exp(-fabsf(g)), big = 1.0f / (1.0f + t), small = t * big;
+  *f = g < 0 ? small : big;
+  *k = g < 0 ? big : small;
+}
+
+}  // namespace daliamd
+#endif  // DALI_AMD_CSRC_SEQUENCE_COMMON_H_

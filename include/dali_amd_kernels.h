@@ -124,7 +124,7 @@ DALIAMD_API daliamdResult_t daliamdMemcpy2DD2DAsync(void *dst, size_t dst_pitch,
 /* Element types of kernel outputs (subset of DALIDataType, include/dali/core/dali_data_type.h) */
 typedef enum {
   DALIAMD_UINT8 = 0, DALIAMD_FLOAT16 = 1, DALIAMD_FLOAT = 2, DALIAMD_INT8 = 3, DALIAMD_INT16 = 4, DALIAMD_UINT16 = 5,
-  DALIAMD_INT32 = 6, DALIAMD_UINT32 = 7
+  DALIAMD_INT32 = 6, DALIAMD_UINT32 = 7, DALIAMD_BFLOAT16 = 8, DALIAMD_INT64 = 9
 } daliamdDType_t;
 typedef enum { DALIAMD_LAYOUT_HWC = 0, DALIAMD_LAYOUT_CHW = 1 } daliamdLayout_t;
 
@@ -747,6 +747,113 @@ DALIAMD_API daliamdResult_t daliamdNormalizeRun(daliamdStream_t stream, const da
                                                 int stat_workgroups, int apply_workgroups, int64_t max_bins,
                                                 int calc_mean, int calc_stddev, int ddof, float epsilon, float scale,
                                                 float shift);
+
+/* ----------------------------------------------------------------------------------------------
+ * Sequence operators: what follows the loader on the device, over batches of sequences of different lengths (frames of
+ * mel features, token ids).  Rows are the steps of all sequences, one behind the other, `channels` values each (adjacent
+ * in memory).  The reference has no counterpart; types: FLOAT, FLOAT16, BFLOAT16, arithmetic in 32 bits or more.
+ *
+ * Unlike the per-sample kernels above these take ONE argument struct by value: a batch is one tensor, not a table of
+ * buffers.  Setup checks the arguments and says how large the workspaces have to be (pure host code); Run checks them
+ * again against what it is given, enqueues, and neither allocates nor waits.
+ *
+ * daliamdSequenceRows: which rows belong to which sequence.
+ *   dense   offsets == NULL: `sequences` blocks of `steps` rows, sequence_rows == sequences * steps.  With `lengths`
+ *           (device, [sequences]) only the first lengths[s] steps of block s are rows of the sequence;
+ *   packed  offsets (device, [sequences + 1], ascending): sequence s has the rows [offsets[s], offsets[s + 1]) of `rows`.
+ * Both are read on the device: values outside [0, rows] (or [0, steps]) are clamped, no row outside the tensors is ever
+ * touched.  Rows of no sequence get zeros in the outputs (gradients too); their inputs are not used.
+ * -------------------------------------------------------------------------------------------- */
+typedef struct {
+  const void *offsets, *lengths;  /* device, index_dtype; at most one of the two                        */
+  int64_t rows;                   /* dense: sequences * steps                                           */
+  int64_t steps;                  /* dense only                                                         */
+  int32_t sequences, index_dtype; /* INT32 or INT64                                                     */
+} daliamdSequenceRows;
+
+/* Linear recurrence along each sequence, per channel, from h_0 = initial (0 if NULL):
+ *   DECAY  h_t = a_t h_{t-1} + x_t                           a = decay
+ *   GATE   h_t = f_t h_{t-1} + (1 - f_t) x_t                 f = 1 / (1 + exp(-decay))
+ * y_t = h_t, final_state = h of the last step (h_0 for a sequence of no steps).
+ * decay: [rows][channels] in x's type or FLOAT, or [channels] with per_channel (same for every step).
+ * Backward: from dy and dfinal (NULL: zero) the gradients of x, decay (per_channel: summed over all rows) and initial.
+ * `saved` is written by a forward pass that a backward pass follows (states at the starts of the kernels' row tiles;
+ * plan.saved_bytes) and read by the latter with the same x, decay and initial. */
+typedef enum { DALIAMD_RECURRENCE_DECAY = 0, DALIAMD_RECURRENCE_GATE = 1 } daliamdRecurrenceForm_t;
+typedef struct {
+  daliamdSequenceRows seq;
+  const void *x, *decay;
+  const float *initial;           /* [sequences][channels] or NULL                                      */
+  void *y;                        /* dtype, dense [rows][channels]                                      */
+  float *final_state;             /* [sequences][channels] or NULL; may be the buffer `initial`         */
+  float *saved;                   /* plan.saved_bytes or NULL (no backward pass follows)                */
+  const void *dy;                 /* backward from here on: dtype                                       */
+  const float *dfinal;            /* [sequences][channels] or NULL                                      */
+  void *dx, *ddecay;              /* x's / decay's type, dense                                          */
+  float *dinitial;                /* [sequences][channels] or NULL                                      */
+  /* distances in elements between rows, and (dense) between the first rows of sequences; adjacent channels are adjacent */
+  int64_t x_row, x_seq, decay_row, decay_seq, dy_row, dy_seq;
+  int32_t channels, dtype, decay_dtype, form, per_channel, reserved;
+} daliamdRecurrenceArgs;
+typedef struct {
+  size_t saved_bytes, forward_workspace_bytes, backward_workspace_bytes;
+} daliamdRecurrencePlan;
+DALIAMD_API daliamdResult_t daliamdRecurrenceSetup(const daliamdRecurrenceArgs *args, daliamdRecurrencePlan *plan);
+DALIAMD_API daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurrenceArgs *args, void *workspace,
+                                                 size_t workspace_bytes);
+DALIAMD_API daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const daliamdRecurrenceArgs *args,
+                                                         void *workspace, size_t workspace_bytes);
+
+/* What stands between two blocks of a layer, one pass over the rows; every part may be left out (NULL):
+ *   u = x rstd(x) post_weight          v = u silu(gate)          h = residual + scale v          n = h rstd(h) pre_weight
+ * rstd(z) = 1 / sqrt(mean(z^2) + eps) over a row's channels, silu(g) = g / (1 + exp(-g)).  hidden = h has the residual's
+ * type (x's without one), normed = n is computed from h before its rounding and has x's type; without pre_weight there is
+ * no n.  rstd_post / rstd_pre ([rows], FLOAT) are written if not NULL; the backward pass needs those of the norms in use.
+ * Backward: dhidden / dnormed (NULL: zero) -> dx, dgate, dresidual and the weights' gradients, sums over the rows in a fixed
+ * order.  post_weight, scale and pre_weight: [channels], x's type or FLOAT (weight_dtype), dense. */
+typedef struct {
+  const void *x, *gate, *residual, *post_weight, *scale, *pre_weight;
+  void *hidden, *normed;
+  float *rstd_post, *rstd_pre;
+  const void *dhidden, *dnormed;
+  void *dx, *dgate, *dresidual, *dpost_weight, *dscale, *dpre_weight;
+  int64_t rows;
+  int64_t x_row, gate_row, residual_row, dhidden_row, dnormed_row; /* elements between rows; outputs are dense */
+  int32_t channels, dtype, residual_dtype, weight_dtype;
+  float eps;
+  int32_t reserved;
+} daliamdBlockNormArgs;
+typedef struct {
+  size_t backward_workspace_bytes;
+} daliamdBlockNormPlan;
+enum { DALIAMD_BLOCK_NORM_MAX_CHANNELS = 16384 };
+DALIAMD_API daliamdResult_t daliamdBlockNormSetup(const daliamdBlockNormArgs *args, daliamdBlockNormPlan *plan);
+DALIAMD_API daliamdResult_t daliamdBlockNormRun(daliamdStream_t stream, const daliamdBlockNormArgs *args);
+DALIAMD_API daliamdResult_t daliamdBlockNormBackwardRun(daliamdStream_t stream, const daliamdBlockNormArgs *args, void *workspace,
+                                                        size_t workspace_bytes);
+
+/* out_i = scale * table[ids_i] (zeros for an id outside [0, vocab)), rounded once.
+ * Backward: dtable_v = scale * sum over { i : ids_i = v } of dout_i, added up in the order of i, for every row v of the
+ * table (zeros where no token is v, and for v == padding); the tokens are sorted in the workspace. */
+typedef struct {
+  const void *ids;                /* device, [tokens], index_dtype                                      */
+  const void *table;              /* [vocab][channels], rows table_row elements apart                   */
+  void *out;                      /* out_dtype, dense [tokens][channels]                                */
+  const void *dout;               /* backward: out_dtype, rows dout_row elements apart                  */
+  void *dtable;                   /* backward: dtype, dense [vocab][channels]                           */
+  int64_t tokens, vocab, padding; /* padding < 0: none                                                  */
+  int64_t table_row, dout_row;
+  int32_t channels, dtype, out_dtype, index_dtype;
+  float scale;
+  int32_t reserved;
+} daliamdEmbeddingArgs;
+typedef struct {
+  size_t backward_workspace_bytes;
+} daliamdEmbeddingPlan;
+DALIAMD_API daliamdResult_t daliamdEmbeddingSetup(const daliamdEmbeddingArgs *args, daliamdEmbeddingPlan *plan);
+DALIAMD_API daliamdResult_t daliamdEmbeddingRun(daliamdStream_t stream, const daliamdEmbeddingArgs *args);
+DALIAMD_API daliamdResult_t daliamdEmbeddingBackwardRun(daliamdStream_t stream, const daliamdEmbeddingArgs *args, void *workspace,
+                                                        size_t workspace_bytes);
 
 #ifdef __cplusplus
 }
