@@ -9,136 +9,277 @@
 
 namespace daliamd {
 
-constexpr int kNormRowThreads = 256;
+// A row's channels stay in the registers of TPR threads, NV pieces of V = 16 bytes of x each: one pass over memory, whatever
+// the number of sums.  TPR <= 64: 256 / TPR rows per workgroup, sums by shuffles inside a wave; above: one row per workgroup
+// step, sums by shuffles and one exchange through LDS.  Workgroups go through the rows with a stride; the backward pass keeps
+// its sums over rows (three weights) in registers meanwhile and leaves one partial sum per workgroup, which ColumnSumKernel
+// adds up in a fixed order.
+template <int TPR> constexpr int NormThreads() { return TPR > 256 ? TPR : 256; }
 
-// the sum over a workgroup, in every thread
-__device__ __forceinline__ float WorkgroupSum(float v, float *shared) {
+// the sum over the TPR threads of a row, in each of them; `slot` alternates between calls: one barrier per sum, because a wave
+// that writes a slot again has passed the barrier behind the last reads of it
+template <int TPR> __device__ __forceinline__ float RowSum(float v, float (*shared)[TPR > 64 ? TPR / 64 : 1], int slot) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = 0;
-  for (int w = 0; w < kNormRowThreads / 64; w++) t += shared[w];
-  return t;
-}
-
-struct NormElement { float x, u, v, h, silu, dsilu; };
-
-// the forward formulas of one channel
-__device__ __forceinline__ NormElement Forward(const daliamdBlockNormArgs &p, int64_t row, int c, float rstd) {
-  NormElement e;
-  e.x = LoadElement(p.x, row * p.x_row + c, p.dtype);
-  e.u = p.post_weight ? e.x * rstd * LoadElement(p.post_weight, c, p.weight_dtype) : e.x;
-  e.silu = 1.0f, e.dsilu = 0.0f;
-  if (p.gate) {
-    const float g = LoadElement(p.gate, row * p.gate_row + c, p.dtype);
-    float f, k;
-    Logistic(g, &f, &k);
-    e.silu = g * f;
-    e.dsilu = f * (1.0f + g * k);
+  for (int off = (TPR > 64 ? 64 : TPR) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) shared[slot][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < TPR / 64; w++) v += shared[slot][w];
   }
-  e.v = e.u * e.silu;
-  e.h = p.scale ? e.v * LoadElement(p.scale, c, p.weight_dtype) : e.v;
-  if (p.residual) e.h += LoadElement(p.residual, row * p.residual_row + c, p.residual_dtype);
-  return e;
+  return v;
 }
 
-__global__ __launch_bounds__(kNormRowThreads) void BlockNormKernel(daliamdBlockNormArgs p) {
-  __shared__ float shared[kNormRowThreads / 64];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  float rstd = 1.0f;
-  if (p.post_weight) {
-    float sum = 0;
-    for (int c = tid; c < p.channels; c += kNormRowThreads) {
-      const float x = LoadElement(p.x, row * p.x_row + c, p.dtype);
-      sum += x * x;
+template <typename XT, int V> __device__ __forceinline__ void LoadWeights(float *w, const void *p, int dtype, const ChannelMap &m, int i) {
+  if (dtype == DALIAMD_FLOAT) {
+    Group<float, V> g;
+    LoadChannels(g, static_cast<const float *>(p), m, i);
+#pragma unroll
+    for (int j = 0; j < V; j++) w[j] = g[j];
+  } else {
+    Group<XT, V> g;
+    LoadChannels(g, static_cast<const XT *>(p), m, i);
+#pragma unroll
+    for (int j = 0; j < V; j++) w[j] = g[j];
+  }
+}
+
+template <typename XT, typename RT, int TPR, int NV>
+__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlockNormArgs p, int wide) {
+  constexpr int V = 16 / sizeof(XT), kRows = NormThreads<TPR>() / TPR;
+  __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
+  const ChannelMap m{p.channels, TPR, (int)threadIdx.x % TPR, wide != 0};
+  const float inv = 1.0f / p.channels;
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
+    const int64_t row = base + threadIdx.x / TPR;
+    const bool live = kRows == 1 || row < p.rows;
+    const int64_t at = live ? row : base;   // (rows of a wave that do not exist: the first one's again, not written)
+    Group<XT, V> x[NV], g[NV];
+    Group<RT, V> r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      LoadChannels(x[i], static_cast<const XT *>(p.x) + at * p.x_row, m, i);
+      if (p.gate) LoadChannels(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row, m, i);
+      if (p.residual) LoadChannels(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row, m, i);
     }
-    rstd = 1.0f / sqrtf(WorkgroupSum(sum, shared) / p.channels + p.eps);
-    if (p.rstd_post && tid == 0) p.rstd_post[row] = rstd;
+    float rstd = 1.0f;
+    if (p.post_weight) {
+      float sum = 0;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) sum = fmaf(x[i][j], x[i][j], sum);
+      rstd = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 0) * inv + p.eps);
+      if (p.rstd_post && m.lane == 0 && live) p.rstd_post[row] = rstd;
+    }
+    float h[NV][V], sum = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float post[V], scale[V];
+      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
+      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float v = x[i][j];
+        if (p.post_weight) v = v * rstd * post[j];
+        if (p.gate) {
+          float f, k;
+          Logistic(g[i][j], &f, &k);
+          v *= g[i][j] * f;
+        }
+        if (p.scale) v *= scale[j];
+        if (p.residual) v += r[i][j];
+        h[i][j] = v;
+        sum = fmaf(v, v, sum);
+      }
+      if (live) StoreChannels<RT, V>(static_cast<RT *>(p.hidden) + row * p.channels, m, i, h[i]);
+    }
+    if (p.pre_weight) {
+      const float rstd2 = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 1) * inv + p.eps);
+      if (p.rstd_pre && m.lane == 0 && live) p.rstd_pre[row] = rstd2;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        float pre[V];
+        LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+#pragma unroll
+        for (int j = 0; j < V; j++) pre[j] = h[i][j] * rstd2 * pre[j];
+        if (live) StoreChannels<XT, V>(static_cast<XT *>(p.normed) + row * p.channels, m, i, pre);
+      }
+    }
+    if (TPR > 64 && (!p.post_weight || !p.pre_weight)) __syncthreads();   // one sum per row: the slot is written again
   }
+}
+
+// partial: [gridDim.x][3][channels], sums of the workgroup's rows for post_weight, scale and pre_weight
+template <typename XT, typename RT, int TPR, int NV>
+__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, int wide, float *partial) {
+  constexpr int V = 16 / sizeof(XT), kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
+  __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
+  const ChannelMap m{p.channels, TPR, (int)threadIdx.x % TPR, wide != 0};
+  const float inv = 1.0f / p.channels;
+  const bool second = p.pre_weight && p.dnormed;
+  float apost[NV][V] = {}, ascale[NV][V] = {}, apre[NV][V] = {};
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
+    const int64_t row = base + threadIdx.x / TPR;
+    const bool live = kRows == 1 || row < p.rows;
+    const int64_t at = live ? row : base;
+    Group<XT, V> x[NV], g[NV], dn[NV];
+    Group<RT, V> r[NV], dh[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      LoadChannels(x[i], static_cast<const XT *>(p.x) + at * p.x_row, m, i);
+      if (p.gate) LoadChannels(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row, m, i);
+      if (second) {
+        LoadChannels(dn[i], static_cast<const XT *>(p.dnormed) + at * p.dnormed_row, m, i);
+        if (p.residual) LoadChannels(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row, m, i);
+      }
+      if (p.dhidden) LoadChannels(dh[i], static_cast<const RT *>(p.dhidden) + at * p.dhidden_row, m, i);
+    }
+    const float rstd = p.post_weight ? p.rstd_post[at] : 1.0f, rstd2 = second ? p.rstd_pre[at] : 1.0f;
+    // v, and with the second norm h^ and the mean of dn w_pre h^
+    float v[NV][V], hat[NV][V], mean2 = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float post[V], scale[V], pre[V];
+      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
+      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
+      if (second) LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float e = x[i][j];
+        if (p.post_weight) e = e * rstd * post[j];
+        if (p.gate) {
+          float f, k;
+          Logistic(g[i][j], &f, &k);
+          e *= g[i][j] * f;
+        }
+        v[i][j] = e;
+        if (second) {
+          if (p.scale) e *= scale[j];
+          if (p.residual) e += r[i][j];
+          e *= rstd2;
+          hat[i][j] = e;
+          mean2 = fmaf(dn[i][j] * pre[j], e, mean2);
+        }
+      }
+    }
+    if (second) mean2 = RowSum<TPR>(mean2, shared, 0) * inv;
+    float d[NV][V], mean1 = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float post[V], scale[V], pre[V], dgate[V];
+      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
+      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
+      if (second) LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float e = p.dhidden ? dh[i][j] : 0.0f;
+        if (second) {
+          e += rstd2 * (dn[i][j] * pre[j] - hat[i][j] * mean2);
+          if (live) apre[i][j] = fmaf(dn[i][j], hat[i][j], apre[i][j]);
+        }
+        d[i][j] = e;
+        if (live) ascale[i][j] = fmaf(e, v[i][j], ascale[i][j]);
+      }
+      if (p.residual && live) StoreChannels<RT, V>(static_cast<RT *>(p.dresidual) + row * p.channels, m, i, d[i]);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float e = d[i][j];
+        if (p.scale) e *= scale[j];
+        const float hat1 = x[i][j] * rstd;
+        if (p.gate) {
+          float f, k;
+          const float gg = g[i][j];
+          Logistic(gg, &f, &k);
+          dgate[j] = e * (p.post_weight ? hat1 * post[j] : hat1) * (f * fmaf(gg, k, 1.0f));
+          e *= gg * f;
+        }
+        if (p.post_weight) {
+          if (live) apost[i][j] = fmaf(e, hat1, apost[i][j]);
+          e *= post[j];
+          mean1 = fmaf(e, hat1, mean1);
+        }
+        d[i][j] = e;
+      }
+      if (p.gate && live) StoreChannels<XT, V>(static_cast<XT *>(p.dgate) + row * p.channels, m, i, dgate);
+    }
+    if (p.post_weight) {
+      mean1 = RowSum<TPR>(mean1, shared, 1) * inv;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) d[i][j] = rstd * (d[i][j] - x[i][j] * rstd * mean1);
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) StoreChannels<XT, V>(static_cast<XT *>(p.dx) + row * p.channels, m, i, d[i]);
+    }
+    if (TPR > 64 && (!p.post_weight || !second)) __syncthreads();
+  }
+  if (!partial) return;
+  float *out = partial + (int64_t)blockIdx.x * 3 * p.channels;
+  if (kRows == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      if (p.post_weight) StoreChannels<float, V>(out, m, i, apost[i]);
+      if (p.scale) StoreChannels<float, V>(out + p.channels, m, i, ascale[i]);
+      if (p.pre_weight) StoreChannels<float, V>(out + 2 * p.channels, m, i, apre[i]);
+    }
+  } else {
+    // the threads with the same channels in all rows of the workgroup: the first row's adds them up
+    __shared__ float rows[3][kRows > 1 ? kThreads : 1];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float post[V], scale[V], pre[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        __syncthreads();
+        rows[0][threadIdx.x] = apost[i][j];
+        rows[1][threadIdx.x] = ascale[i][j];
+        rows[2][threadIdx.x] = apre[i][j];
+        __syncthreads();
+        post[j] = scale[j] = pre[j] = 0;
+        if (threadIdx.x < TPR)
+          for (int k = 0; k < kRows; k++) {
+            post[j] += rows[0][k * TPR + threadIdx.x];
+            scale[j] += rows[1][k * TPR + threadIdx.x];
+            pre[j] += rows[2][k * TPR + threadIdx.x];
+          }
+      }
+      if (threadIdx.x < TPR) {
+        if (p.post_weight) StoreChannels<float, V>(out, m, i, post);
+        if (p.scale) StoreChannels<float, V>(out + p.channels, m, i, scale);
+        if (p.pre_weight) StoreChannels<float, V>(out + 2 * p.channels, m, i, pre);
+      }
+    }
+  }
+}
+
+// the sum of each column of `partial`, in a fixed order: kParts threads take every kParts-th row, then one adds them up
+constexpr int kSumColumns = 64, kSumParts = 16;
+__global__ __launch_bounds__(kSumColumns * kSumParts) void BlockNormWeightsKernel(daliamdBlockNormArgs p, const float *partial, int count) {
+  __shared__ float part[kSumParts][kSumColumns];
+  const int column = threadIdx.x % kSumColumns, k = threadIdx.x / kSumColumns;
+  const int c = blockIdx.x * kSumColumns + column, which = blockIdx.y;
+  void *out = which == 0 ? p.dpost_weight : which == 1 ? p.dscale : p.dpre_weight;
+  if (!(which == 0 ? p.post_weight : which == 1 ? p.scale : p.pre_weight)) return;
   float sum = 0;
-  for (int c = tid; c < p.channels; c += kNormRowThreads) {
-    const float h = Forward(p, row, c, rstd).h;
-    sum += h * h;
-    StoreElement(p.hidden, row * p.channels + c, p.residual ? p.residual_dtype : p.dtype, h);
+  if (c < p.channels) {
+#pragma unroll 8
+    for (int n = k; n < count; n += kSumParts) sum += partial[((int64_t)n * 3 + which) * p.channels + c];
   }
-  if (!p.pre_weight) return;
-  const float rstd2 = 1.0f / sqrtf(WorkgroupSum(sum, shared) / p.channels + p.eps);
-  if (p.rstd_pre && tid == 0) p.rstd_pre[row] = rstd2;
-  for (int c = tid; c < p.channels; c += kNormRowThreads)
-    StoreElement(p.normed, row * p.channels + c, p.dtype, Forward(p, row, c, rstd).h * rstd2 * LoadElement(p.pre_weight, c, p.weight_dtype));
-}
-
-// the gradient of h at one channel, with the mean of the norm behind it
-__device__ __forceinline__ float HiddenGradient(const daliamdBlockNormArgs &p, int64_t row, int c, float h, float rstd2, float mean) {
-  float d = p.dhidden ? LoadElement(p.dhidden, row * p.dhidden_row + c, p.residual ? p.residual_dtype : p.dtype) : 0.0f;
-  if (p.pre_weight && p.dnormed)
-    d += rstd2 * (LoadElement(p.dnormed, row * p.dnormed_row + c, p.dtype) * LoadElement(p.pre_weight, c, p.weight_dtype) - h * rstd2 * mean);
-  return d;
-}
-
-__global__ __launch_bounds__(kNormRowThreads) void BlockNormBackwardKernel(daliamdBlockNormArgs p) {
-  __shared__ float shared[kNormRowThreads / 64];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const float rstd = p.post_weight ? p.rstd_post[row] : 1.0f, rstd2 = p.pre_weight ? p.rstd_pre[row] : 1.0f;
-  float mean = 0;
-  if (p.pre_weight && p.dnormed) {
-    for (int c = tid; c < p.channels; c += kNormRowThreads)
-      mean += LoadElement(p.dnormed, row * p.dnormed_row + c, p.dtype) * LoadElement(p.pre_weight, c, p.weight_dtype) * Forward(p, row, c, rstd).h * rstd2;
-    mean = WorkgroupSum(mean, shared) / p.channels;
-  }
-  float mean1 = 0;
-  for (int c = tid; c < p.channels; c += kNormRowThreads) {
-    const NormElement e = Forward(p, row, c, rstd);
-    const float dh = HiddenGradient(p, row, c, e.h, rstd2, mean);
-    if (p.residual) StoreElement(p.dresidual, row * p.channels + c, p.residual_dtype, dh);
-    const float dv = p.scale ? dh * LoadElement(p.scale, c, p.weight_dtype) : dh, du = dv * e.silu;
-    if (p.gate) StoreElement(p.dgate, row * p.channels + c, p.dtype, dv * e.u * e.dsilu);
-    if (p.post_weight) mean1 += du * LoadElement(p.post_weight, c, p.weight_dtype) * e.x * rstd;
-    else StoreElement(p.dx, row * p.channels + c, p.dtype, du);
-  }
-  if (!p.post_weight) return;
-  mean1 = WorkgroupSum(mean1, shared) / p.channels;
-  for (int c = tid; c < p.channels; c += kNormRowThreads) {
-    const NormElement e = Forward(p, row, c, rstd);
-    const float dh = HiddenGradient(p, row, c, e.h, rstd2, mean);
-    const float du = (p.scale ? dh * LoadElement(p.scale, c, p.weight_dtype) : dh) * e.silu;
-    StoreElement(p.dx, row * p.channels + c, p.dtype, rstd * (du * LoadElement(p.post_weight, c, p.weight_dtype) - e.x * rstd * mean1));
+  part[k][column] = sum;
+  __syncthreads();
+  if (k == 0 && c < p.channels) {
+    for (int n = 1; n < kSumParts; n++) sum += part[n][column];
+    StoreElement(out, c, p.weight_dtype, sum);
   }
 }
 
-// the weights' gradients: one thread per channel goes through all rows
-__global__ __launch_bounds__(kNormRowThreads) void BlockNormWeightsKernel(daliamdBlockNormArgs p, const float *means) {
-  const int c = blockIdx.x * kNormRowThreads + threadIdx.x;
-  if (c >= p.channels) return;
-  double post = 0, scale = 0, pre = 0;
-  for (int64_t row = 0; row < p.rows; row++) {
-    const float rstd = p.post_weight ? p.rstd_post[row] : 1.0f, rstd2 = p.pre_weight ? p.rstd_pre[row] : 1.0f;
-    const NormElement e = Forward(p, row, c, rstd);
-    const float dh = HiddenGradient(p, row, c, e.h, rstd2, means[row]);
-    if (p.pre_weight && p.dnormed) pre += LoadElement(p.dnormed, row * p.dnormed_row + c, p.dtype) * (e.h * rstd2);
-    scale += dh * e.v;
-    post += (p.scale ? dh * LoadElement(p.scale, c, p.weight_dtype) : dh) * e.silu * e.x * rstd;
-  }
-  if (p.post_weight) StoreElement(p.dpost_weight, c, p.weight_dtype, (float)post);
-  if (p.scale) StoreElement(p.dscale, c, p.weight_dtype, (float)scale);
-  if (p.pre_weight) StoreElement(p.dpre_weight, c, p.weight_dtype, (float)pre);
-}
-
-__global__ __launch_bounds__(kNormRowThreads) void BlockNormMeansKernel(daliamdBlockNormArgs p, float *means) {
-  __shared__ float shared[kNormRowThreads / 64];
-  const int64_t row = blockIdx.x;
-  const float rstd = p.post_weight ? p.rstd_post[row] : 1.0f, rstd2 = p.pre_weight ? p.rstd_pre[row] : 1.0f;
-  float mean = 0;
-  if (p.pre_weight && p.dnormed)
-    for (int c = threadIdx.x; c < p.channels; c += kNormRowThreads)
-      mean += LoadElement(p.dnormed, row * p.dnormed_row + c, p.dtype) * LoadElement(p.pre_weight, c, p.weight_dtype) * Forward(p, row, c, rstd).h * rstd2;
-  mean = WorkgroupSum(mean, shared) / p.channels;
-  if (threadIdx.x == 0) means[row] = mean;
-}
+// workgroups of the backward pass, at most: enough to fill the card, few enough that their partial sums are a small part of
+// what it moves
+static int64_t BackwardWorkgroups(int64_t rows) { return rows < 512 ? rows : 512; }
 
 static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdBlockNormPlan *plan) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNorm: NULL argument");
@@ -152,8 +293,59 @@ static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdB
   DALIAMD_REQUIRE(!(a.post_weight || a.scale || a.pre_weight) || a.weight_dtype == a.dtype || a.weight_dtype == DALIAMD_FLOAT, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdBlockNorm: the weights must have x's type or be FLOAT");
   DALIAMD_REQUIRE(a.eps >= 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNorm: eps must not be negative");
-  plan->backward_workspace_bytes = sizeof(float) * (size_t)a.rows;
+  plan->backward_workspace_bytes = sizeof(float) * 3 * (size_t)BackwardWorkgroups(a.rows) * a.channels;
   return DALIAMD_SUCCESS;
+}
+
+// every tensor in use can be read and written 16 bytes at a time: then a thread has adjacent channels
+static bool Wide(const daliamdBlockNormArgs &a, bool backward) {
+  const int e = ElementSize(a.dtype), r = a.residual ? ElementSize(a.residual_dtype) : e;
+  const int w = a.post_weight || a.scale || a.pre_weight ? ElementSize(a.weight_dtype) : e;
+  if (a.channels % (16 / e)) return false;
+  bool ok = RowsAligned(a.x, a.x_row, e) && RowsAligned(a.gate, a.gate ? a.gate_row : 0, e) && RowsAligned(a.residual, a.residual ? a.residual_row : 0, r) &&
+            RowsAligned(a.post_weight, 0, w) && RowsAligned(a.scale, 0, w) && RowsAligned(a.pre_weight, 0, w);
+  if (backward)
+    ok = ok && RowsAligned(a.dhidden, a.dhidden ? a.dhidden_row : 0, r) && RowsAligned(a.dnormed, a.dnormed ? a.dnormed_row : 0, e) &&
+         RowsAligned(a.dx, 0, e) && RowsAligned(a.dgate, 0, e) && RowsAligned(a.dresidual, 0, r);
+  else
+    ok = ok && RowsAligned(a.hidden, 0, r) && RowsAligned(a.normed, 0, e);
+  return ok;
+}
+
+template <typename XT, typename RT, int TPR, int NV> struct NormLaunch {
+  static constexpr int kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
+  static void Forward(hipStream_t s, const daliamdBlockNormArgs &a) {
+    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    KernelTimer timer("BlockNormKernel", s);
+    hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV>), dim3((unsigned)groups), dim3(kThreads), 0, s, a, (int)Wide(a, false));
+  }
+  static void Backward(hipStream_t s, const daliamdBlockNormArgs &a, float *partial, int *count) {
+    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    *count = (int)(groups < BackwardWorkgroups(a.rows) ? groups : BackwardWorkgroups(a.rows));
+    KernelTimer timer("BlockNormBackwardKernel", s);
+    hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV>), dim3((unsigned)*count), dim3(kThreads), 0, s, a, (int)Wide(a, true), partial);
+  }
+};
+
+// the number of threads per row and pieces per thread: the fewest that hold the row
+template <typename XT, typename RT, typename F> static void WithShape(int channels, F f) {
+  const int pieces = (channels + 16 / (int)sizeof(XT) - 1) / (16 / (int)sizeof(XT));
+  if (pieces <= 8) f(NormLaunch<XT, RT, 8, 1>());
+  else if (pieces <= 16) f(NormLaunch<XT, RT, 16, 1>());
+  else if (pieces <= 32) f(NormLaunch<XT, RT, 32, 1>());
+  else if (pieces <= 64) f(NormLaunch<XT, RT, 64, 1>());
+  else if (pieces <= 128) f(NormLaunch<XT, RT, 64, 2>());
+  else if (pieces <= 256) f(NormLaunch<XT, RT, 256, 1>());
+  else if (pieces <= 512) f(NormLaunch<XT, RT, 256, 2>());
+  else if (pieces <= 1024) f(NormLaunch<XT, RT, 1024, 1>());
+  else if (pieces <= 2048) f(NormLaunch<XT, RT, 1024, 2>());
+  else f(NormLaunch<XT, RT, 1024, 4>());
+}
+template <typename F> static void WithTypes(const daliamdBlockNormArgs &a, F f) {
+  const bool wide_residual = a.residual && a.residual_dtype == DALIAMD_FLOAT;
+  if (a.dtype == DALIAMD_FLOAT) WithShape<float, float>(a.channels, f);
+  else if (a.dtype == DALIAMD_FLOAT16) wide_residual ? WithShape<F16, float>(a.channels, f) : WithShape<F16, F16>(a.channels, f);
+  else wide_residual ? WithShape<Bf16, float>(a.channels, f) : WithShape<Bf16, Bf16>(a.channels, f);
 }
 
 }  // namespace daliamd
@@ -173,10 +365,7 @@ daliamdResult_t daliamdBlockNormRun(daliamdStream_t stream, const daliamdBlockNo
   DALIAMD_REQUIRE(args->x && args->hidden && (!args->pre_weight || args->normed), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdBlockNormRun: NULL tensor");
   hipStream_t s = (hipStream_t)stream;
-  {
-    KernelTimer timer("BlockNormKernel", s);
-    hipLaunchKernelGGL(BlockNormKernel, dim3((unsigned)args->rows), dim3(kNormRowThreads), 0, s, *args);
-  }
+  WithTypes(*args, [&](auto launch) { launch.Forward(s, *args); });
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
 }
@@ -193,14 +382,14 @@ daliamdResult_t daliamdBlockNormBackwardRun(daliamdStream_t stream, const daliam
   DALIAMD_REQUIRE(workspace_bytes >= plan.backward_workspace_bytes && (workspace || !plan.backward_workspace_bytes),
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNormBackwardRun: the workspace is too small");
   hipStream_t s = (hipStream_t)stream;
-  float *means = static_cast<float *>(workspace);
-  if (a.rows) {
-    KernelTimer timer("BlockNormBackwardKernel", s);
-    hipLaunchKernelGGL(BlockNormBackwardKernel, dim3((unsigned)a.rows), dim3(kNormRowThreads), 0, s, a);
-  }
-  if (a.post_weight || a.scale || a.pre_weight) {
-    if (a.rows) hipLaunchKernelGGL(BlockNormMeansKernel, dim3((unsigned)a.rows), dim3(kNormRowThreads), 0, s, a, means);
-    hipLaunchKernelGGL(BlockNormWeightsKernel, dim3((a.channels + kNormRowThreads - 1) / kNormRowThreads), dim3(kNormRowThreads), 0, s, a, means);
+  const bool weights = a.post_weight || a.scale || a.pre_weight;
+  float *partial = weights ? static_cast<float *>(workspace) : nullptr;
+  int count = 0;
+  if (a.rows) WithTypes(a, [&](auto launch) { launch.Backward(s, a, partial, &count); });
+  if (weights) {
+    KernelTimer timer("BlockNormWeightsKernel", s);
+    hipLaunchKernelGGL(BlockNormWeightsKernel, dim3((a.channels + kSumColumns - 1) / kSumColumns, 3), dim3(kSumColumns * kSumParts), 0, s, a,
+                       partial, count);
   }
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;

@@ -28,6 +28,60 @@ template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
 #endif
 }
 
+// V adjacent elements in registers, as they are in memory; read and written 16 bytes at a time where that is possible
+template <typename T, int V> struct alignas(16) Group {
+  T v[V];
+  __device__ __forceinline__ float operator[](int j) const { return ToFloat(v[j]); }
+};
+template <typename T, int V> __device__ __forceinline__ void LoadWide(Group<T, V> &g, const T *p) {
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(&g)[k] = reinterpret_cast<const uint4 *>(p)[k];
+}
+template <typename T, int V> __device__ __forceinline__ void StoreWide(T *p, const float *f) {
+  Group<T, V> g;
+#pragma unroll
+  for (int j = 0; j < V; j++) g.v[j] = FromFloat<T>(f[j]);
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(&g)[k];
+}
+
+// Which channels a thread of a row has, in `n` pieces of V: adjacent ones where every row of every tensor can be read 16 bytes
+// at a time (`wide`), else every `threads`-th, so that a wave's loads of single elements are adjacent.
+struct ChannelMap {
+  int channels, threads, lane;
+  bool wide;
+  template <int V> __device__ __forceinline__ int First(int i) const { return wide ? (i * threads + lane) * V : i * V * threads + lane; }
+  __device__ __forceinline__ int Step() const { return wide ? 1 : threads; }
+};
+template <typename T, int V> __device__ __forceinline__ void LoadChannels(Group<T, V> &g, const T *row, const ChannelMap &m, int i) {
+  const int c = m.First<V>(i);
+  if (m.wide) {
+    if (c < m.channels) {
+      LoadWide(g, row + c);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(&g)[k] = make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j++) g.v[j] = c + j * m.threads < m.channels ? row[c + j * m.threads] : FromFloat<T>(0.0f);
+  }
+}
+template <typename T, int V> __device__ __forceinline__ void StoreChannels(T *row, const ChannelMap &m, int i, const float *f) {
+  const int c = m.First<V>(i);
+  if (m.wide) {
+    if (c < m.channels) StoreWide<T, V>(row + c, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (c + j * m.threads < m.channels) row[c + j * m.threads] = FromFloat<T>(f[j]);
+  }
+}
+// whether rows of `elem`-byte elements, `stride` elements apart, all start at multiples of 16 bytes
+inline bool RowsAligned(const void *p, int64_t stride, int elem) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride * elem)) & 15) == 0;
+}
+
 __device__ __forceinline__ float LoadElement(const void *p, int64_t i, int dtype) {
   return dtype == DALIAMD_FLOAT ? static_cast<const float *>(p)[i]
        : dtype == DALIAMD_FLOAT16 ? ToFloat(static_cast<const F16 *>(p)[i]) : ToFloat(static_cast<const Bf16 *>(p)[i]);
