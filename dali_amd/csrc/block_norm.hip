@@ -5,6 +5,7 @@
 //   dr = dh     dv = dh s                                      ds      = sum over rows of dh v
 //   dg = dv u silu'(g)     du = dv silu(g)                     dw_post = sum over rows of du x^
 //   dx = rstd(x) (du w_post - x^ <du w_post x^>)
+#include <algorithm>
 #include "sequence_common.h"
 
 namespace daliamd {
@@ -315,7 +316,7 @@ static bool Wide(const daliamdBlockNormArgs &a, bool backward) {
 template <typename XT, typename RT, int TPR, int NV> struct NormLaunch {
   static constexpr int kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
   static void Forward(hipStream_t s, const daliamdBlockNormArgs &a) {
-    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    const int64_t groups = std::min<int64_t>((a.rows + kRows - 1) / kRows, 1 << 20);
     KernelTimer timer("BlockNormKernel", s);
     hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV>), dim3((unsigned)groups), dim3(kThreads), 0, s, a, (int)Wide(a, false));
   }

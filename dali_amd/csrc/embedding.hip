@@ -3,26 +3,428 @@
 
 namespace daliamd {
 
-constexpr int kEmbThreads = 256;
+// ---- lookup ------------------------------------------------------------------------------------------------------------
+// TPR threads per row, 8 channels per thread and step; kTokens rows per thread, whose loads are all in flight at once.
+constexpr int kEmbThreads = 256, kEmbV = 8;
 
-__global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingArgs p) {
-  const int64_t token = blockIdx.x;
-  const int64_t id = LoadIndex(p.ids, token, p.index_dtype);
-  const bool in_table = id >= 0 && id < p.vocab;
-  for (int c = threadIdx.x; c < p.channels; c += kEmbThreads)
-    StoreElement(p.out, token * p.channels + c, p.out_dtype, in_table ? LoadElement(p.table, id * p.table_row + c, p.dtype) * p.scale : 0.0f);
+template <typename TT, typename OT, int kTokens>
+__global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingArgs p, int tpr, int wide) {
+  const ChannelMap m{p.channels, tpr, (int)threadIdx.x % tpr, wide != 0};
+  const int64_t first = ((int64_t)blockIdx.x * (kEmbThreads / tpr) + threadIdx.x / tpr) * kTokens;
+  int64_t row[kTokens];
+#pragma unroll
+  for (int k = 0; k < kTokens; k++) {
+    const int64_t id = first + k < p.tokens ? LoadIndex(p.ids, first + k, p.index_dtype) : -1;
+    row[k] = id >= 0 && id < p.vocab ? id : -1;
+  }
+  for (int i = 0; i * tpr * kEmbV < p.channels; i++) {
+    Group<TT, kEmbV> g[kTokens];
+#pragma unroll
+    for (int k = 0; k < kTokens; k++) LoadChannels(g[k], static_cast<const TT *>(p.table) + max(row[k], (int64_t)0) * p.table_row, m, i);
+#pragma unroll
+    for (int k = 0; k < kTokens; k++) {
+      float v[kEmbV];
+#pragma unroll
+      for (int j = 0; j < kEmbV; j++) v[j] = row[k] >= 0 ? g[k][j] * p.scale : 0.0f;
+      if (first + k < p.tokens) StoreChannels<OT, kEmbV>(static_cast<OT *>(p.out) + (first + k) * p.channels, m, i, v);
+    }
+  }
 }
 
-// one workgroup per row of the table looks through all tokens
-__global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEmbeddingArgs p) {
-  const int64_t id = blockIdx.x;
-  for (int c = threadIdx.x; c < p.channels; c += kEmbThreads) {
-    float sum = 0;
-    if (id != p.padding)
-      for (int64_t t = 0; t < p.tokens; t++)
-        if (LoadIndex(p.ids, t, p.index_dtype) == id) sum += LoadElement(p.dout, t * p.dout_row + c, p.out_dtype);
-    StoreElement(p.dtable, id * p.channels + c, p.dtype, sum * p.scale);
+// ---- the tokens, sorted ------------------------------------------------------------------------------------------------
+// A stable sort of the tokens by id, least significant digit first (so that equal ids stay in the order of the tokens, and the
+// sums below have a fixed order).  A token that takes no part (padding, ids outside the table) has the key `vocab`, behind all
+// others.  Per digit of up to 9 bits: SortCountKernel counts the digits of each tile of tokens; SortScatterKernel adds up the
+// counts in front of its own (all digits below, and this digit in the tiles before: a few hundred numbers per digit, read by
+// every workgroup instead of a launch of their own) and moves its tile's tokens.  Up to kSmallTokens: everything in one workgroup.
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kTileTokens = 2048, kMaxTiles = 512;
+constexpr int kSmallTokens = 4096, kSmallThreads = 1024, kSmallRounds = kSmallTokens / kSmallThreads;
+
+struct EmbSort {
+  int64_t tokens, tile;         // tile: tokens per workgroup, a multiple of kSortThreads
+  int tiles, passes, bits;      // bits per digit
+  uint32_t *key[2], *index[2], *count;
+};
+
+__device__ __forceinline__ uint32_t TokenKey(const daliamdEmbeddingArgs &p, int64_t t) {
+  const int64_t id = LoadIndex(p.ids, t, p.index_dtype);
+  return (uint32_t)(id >= 0 && id < p.vocab && id != p.padding ? id : p.vocab);
+}
+
+// the lanes of the wave whose digit is this lane's (those with `valid`)
+__device__ __forceinline__ uint64_t SameDigit(uint32_t digit, int bits, bool valid) {
+  uint64_t mask = __ballot(valid);
+  for (int b = 0; b < bits; b++) {
+    const uint64_t set = __ballot((digit >> b) & 1);
+    mask &= (digit >> b) & 1 ? set : ~set;
   }
+  return mask;
+}
+
+// One round of 64 tokens of a wave in their order: the place of each behind those with its digit so far; next[digit] counts.
+__device__ __forceinline__ uint32_t TakePlace(uint32_t *next, uint32_t digit, int bits, bool valid) {
+  const uint64_t mask = SameDigit(digit, bits, valid);
+  const int lane = threadIdx.x & 63;
+  const uint32_t before = (uint32_t)__popcll(mask & (((uint64_t)1 << lane) - 1));
+  uint32_t place = 0;
+  if (valid) place = next[digit] + before;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (valid && before == 0) next[digit] += (uint32_t)__popcll(mask);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return place;
+}
+
+__global__ __launch_bounds__(kSortThreads) void SortCountKernel(daliamdEmbeddingArgs p, EmbSort s, int pass) {
+  __shared__ uint32_t count[kDigits];
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
+  __syncthreads();
+  const int64_t begin = blockIdx.x * s.tile, end = min(begin + s.tile, s.tokens);
+  const int shift = pass * s.bits;
+  const uint32_t digits = (1u << s.bits) - 1;
+  for (int64_t t = begin + threadIdx.x; t < end; t += kSortThreads) {
+    const uint32_t key = pass ? s.key[pass & 1][t] : TokenKey(p, t);
+    atomicAdd(&count[(key >> shift) & digits], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) s.count[(int64_t)blockIdx.x * kDigits + d] = count[d];
+}
+
+// exclusive prefix sums of one number per thread over kSortThreads == kDigits threads
+__device__ __forceinline__ uint32_t PrefixOfDigits(uint32_t v, uint32_t *wave_total) {
+  uint32_t incl = v;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t u = (uint32_t)__shfl_up((int)incl, off, 64);
+    if (lane >= off) incl += u;
+  }
+  if (lane == 63) wave_total[wave] = incl;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; w++) before += wave_total[w];
+  return before + incl - v;
+}
+
+__global__ __launch_bounds__(kSortThreads) void SortScatterKernel(daliamdEmbeddingArgs p, EmbSort s, int pass) {
+  static_assert(kSortThreads == kDigits, "a thread per digit");
+  __shared__ uint32_t next[kSortWaves][kDigits], wave_total[kSortWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  for (int w = 0; w < kSortWaves; w++) next[w][tid] = 0;
+  // this digit in the tiles before, and in all of them
+  uint32_t before = 0, all = 0;
+#pragma unroll 8
+  for (int t = 0; t < s.tiles; t++) {
+    const uint32_t n = s.count[(int64_t)t * kDigits + tid];
+    all += n;
+    if (t < (int)blockIdx.x) before += n;
+  }
+  __syncthreads();
+  // the tokens of a wave: one stretch of the tile
+  const int64_t begin = blockIdx.x * s.tile + wave * (s.tile / kSortWaves), end = min(begin + s.tile / kSortWaves, s.tokens);
+  const int shift = pass * s.bits;
+  const uint32_t digits = (1u << s.bits) - 1;
+  for (int64_t t = begin + lane; t < end; t += 64) {
+    const uint32_t key = pass ? s.key[pass & 1][t] : TokenKey(p, t);
+    atomicAdd(&next[wave][(key >> shift) & digits], 1u);
+  }
+  uint32_t place = PrefixOfDigits(all, wave_total) + before;
+  __syncthreads();
+  for (int w = 0; w < kSortWaves; w++) {
+    const uint32_t n = next[w][tid];
+    next[w][tid] = place;
+    place += n;
+  }
+  __syncthreads();
+  for (int64_t t = begin; t < end; t += 64) {
+    const bool valid = t + lane < end;
+    const uint32_t key = !valid ? 0 : pass ? s.key[pass & 1][t + lane] : TokenKey(p, t + lane);
+    const uint32_t index = !valid ? 0 : pass ? s.index[pass & 1][t + lane] : (uint32_t)(t + lane);
+    const uint32_t to = TakePlace(next[wave], (key >> shift) & digits, s.bits, valid);
+    if (valid) {
+      s.key[(pass + 1) & 1][to] = key;
+      s.index[(pass + 1) & 1][to] = index;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kSmallThreads) void SortSmallKernel(daliamdEmbeddingArgs p, EmbSort s) {
+  constexpr int kWaves = kSmallThreads / 64;
+  __shared__ uint32_t key[kSmallTokens], next[kWaves][kDigits], wave_total[kWaves];
+  __shared__ uint16_t index[kSmallTokens];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, tokens = (int)s.tokens;
+  uint32_t k[kSmallRounds], to[kSmallRounds];
+  uint16_t at[kSmallRounds];
+  for (int pass = 0; pass < s.passes; pass++) {
+    const int shift = pass * s.bits;
+    const uint32_t digits = (1u << s.bits) - 1;
+    for (int d = tid; d < kWaves * kDigits; d += kSmallThreads) next[d / kDigits][d % kDigits] = 0;
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; r++) {
+      const int t = (wave * kSmallRounds + r) * 64 + lane;
+      if (t >= tokens) continue;
+      k[r] = pass ? key[t] : TokenKey(p, t);
+      at[r] = pass ? index[t] : (uint16_t)t;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; r++)
+      if ((wave * kSmallRounds + r) * 64 + lane < tokens) atomicAdd(&next[wave][(k[r] >> shift) & digits], 1u);
+    __syncthreads();
+    uint32_t all = 0;
+    if (tid < kDigits)
+      for (int w = 0; w < kWaves; w++) all += next[w][tid];
+    uint32_t place = PrefixOfDigits(all, wave_total);
+    __syncthreads();
+    if (tid < kDigits)
+      for (int w = 0; w < kWaves; w++) {
+        const uint32_t n = next[w][tid];
+        next[w][tid] = place;
+        place += n;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; r++) {
+      const bool valid = (wave * kSmallRounds + r) * 64 + lane < tokens;
+      to[r] = TakePlace(next[wave], valid ? (k[r] >> shift) & digits : 0, s.bits, valid);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; r++)
+      if ((wave * kSmallRounds + r) * 64 + lane < tokens) key[to[r]] = k[r], index[to[r]] = at[r];
+    __syncthreads();
+  }
+  for (int t = tid; t < tokens; t += kSmallThreads) {
+    s.key[s.passes & 1][t] = key[t];
+    s.index[s.passes & 1][t] = index[t];
+  }
+}
+
+// ---- sums of the sorted tokens' gradients --------------------------------------------------------------------------------
+// The sorted tokens are cut into chunks of kChunk, whatever their ids: a token that fills half a batch is as much work per
+// workgroup as rare ones.  A chunk adds up each run of equal ids in it.  A run that lies within a chunk is a row of the result; of
+// one that goes on, each chunk leaves its part, and EmbeddingJoinKernel adds those of one run in their order.  Rows without a
+// token are filled with zeros by further workgroups of the same launch.
+constexpr int kChunk = 32, kFillRows = 64;
+
+struct EmbSums {
+  const uint32_t *key, *index;
+  float *part;                  // [chunks][2][channels]: of the run that came from the chunk before, of the one that goes on behind
+  int chunks, chunk_groups, tpr, wide;
+};
+
+// the first place whose key is not below `key`
+__device__ __forceinline__ int64_t LowerBound(const uint32_t *keys, int64_t n, uint32_t key) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+template <typename TT, typename OT>
+__global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEmbeddingArgs p, EmbSums s) {
+  const int64_t n = p.tokens;
+  if ((int)blockIdx.x >= s.chunk_groups) {   // rows without a token
+    __shared__ uint64_t empty;
+    const int64_t row = (int64_t)((int)blockIdx.x - s.chunk_groups) * kFillRows;
+    if (threadIdx.x < kFillRows) {
+      const int64_t v = row + threadIdx.x;
+      bool none = false;
+      if (v < p.vocab) {
+        const int64_t at = LowerBound(s.key, n, (uint32_t)v);
+        none = at >= n || s.key[at] != (uint32_t)v;
+      }
+      const uint64_t mask = __ballot(none);
+      if (threadIdx.x == 0) empty = mask;
+    }
+    __syncthreads();
+    const ChannelMap m{p.channels, kEmbThreads, (int)threadIdx.x, s.wide != 0};
+    const float zero[kEmbV] = {};
+    for (uint64_t mask = empty; mask; mask &= mask - 1) {
+      TT *out = static_cast<TT *>(p.dtable) + (row + __ffsll((unsigned long long)mask) - 1) * p.channels;
+      for (int i = 0; i * kEmbThreads * kEmbV < p.channels; i++) StoreChannels<TT, kEmbV>(out, m, i, zero);
+    }
+    return;
+  }
+  const ChannelMap m{p.channels, s.tpr, (int)threadIdx.x % s.tpr, s.wide != 0};
+  const int64_t chunk = (int64_t)blockIdx.x * (kEmbThreads / s.tpr) + threadIdx.x / s.tpr;
+  const int64_t begin = chunk * kChunk, end = min(begin + kChunk, n);
+  if (begin >= end) return;
+  const uint32_t vocab = (uint32_t)p.vocab;
+  const bool from_before = begin > 0 && s.key[begin - 1] == s.key[begin];
+  const bool goes_on = end < n && s.key[end] == s.key[end - 1];
+  constexpr int kAhead = 8;   // rows in flight
+  for (int i = 0; i * s.tpr * kEmbV < p.channels; i++) {
+    float sum[kEmbV] = {};
+    uint32_t run = s.key[begin];
+    bool first = true;        // the chunk's first run
+    for (int64_t t0 = begin; t0 < end && s.key[t0] < vocab; t0 += kAhead) {
+      Group<OT, kEmbV> g[kAhead];
+      uint32_t key[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        key[a] = t0 + a < end ? s.key[t0 + a] : vocab;
+        if (key[a] < vocab) LoadChannels(g[a], static_cast<const OT *>(p.dout) + (int64_t)s.index[t0 + a] * p.dout_row, m, i);
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        if (key[a] != run && run < vocab) {   // a run ends, not the chunk's last
+          if (first && from_before) {
+            StoreChannels<float, kEmbV>(s.part + chunk * 2 * p.channels, m, i, sum);
+          } else if (t0 + a < end || !goes_on) {
+#pragma unroll
+            for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
+            StoreChannels<TT, kEmbV>(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, m, i, sum);
+          } else {
+            StoreChannels<float, kEmbV>(s.part + (chunk * 2 + 1) * p.channels, m, i, sum);
+          }
+          first = false;
+#pragma unroll
+          for (int j = 0; j < kEmbV; j++) sum[j] = 0;
+        }
+        run = key[a];
+        if (key[a] < vocab) {
+#pragma unroll
+          for (int j = 0; j < kEmbV; j++) sum[j] += g[a][j];
+        }
+      }
+    }
+    if (run < vocab) {        // the chunk's last token was the last of a group of kAhead
+      if (first && from_before) {
+        StoreChannels<float, kEmbV>(s.part + chunk * 2 * p.channels, m, i, sum);
+      } else if (goes_on) {
+        StoreChannels<float, kEmbV>(s.part + (chunk * 2 + 1) * p.channels, m, i, sum);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
+        StoreChannels<TT, kEmbV>(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, m, i, sum);
+      }
+    }
+  }
+}
+
+// A run over several chunks: kJoinParts threads for 4 channels, each adding up a stretch of its parts.  Most workgroups find
+// nothing to do or two or three parts: small ones, so that a frequent token's long run is the only one that takes time.
+constexpr int kJoinLanes = 64, kJoinParts = 4, kJoinColumns = kJoinLanes * 4;
+__global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(daliamdEmbeddingArgs p, EmbSums s) {
+  __shared__ float part[kJoinParts][kJoinColumns];
+  const int64_t chunk = blockIdx.x, begin = chunk * kChunk, end = begin + kChunk;
+  if (end >= p.tokens || s.key[end] != s.key[end - 1]) return;                  // nothing goes on behind this chunk
+  const uint32_t key = s.key[end - 1];
+  if (key >= (uint32_t)p.vocab) return;
+  if (begin > 0 && s.key[begin - 1] == key) return;                             // it began in a chunk before
+  const int64_t last = (LowerBound(s.key, p.tokens, key + 1) - 1) / kChunk;     // the chunk that the run ends in
+  const int lane = threadIdx.x % kJoinLanes, k = threadIdx.x / kJoinLanes;
+  const int64_t count = last - chunk, each = (count + kJoinParts - 1) / kJoinParts;
+  const int64_t from = chunk + 1 + k * each, to = min(from + each, last + 1);
+  for (int c0 = blockIdx.y * kJoinColumns; c0 < p.channels; c0 += gridDim.y * kJoinColumns) {
+    const ChannelMap m{p.channels - c0, kJoinLanes, lane, (p.channels & 3) == 0};
+    float sum[4] = {};
+    Group<float, 4> g;
+    if (k == 0) {
+      LoadChannels(g, s.part + (chunk * 2 + 1) * p.channels + c0, m, 0);
+      for (int j = 0; j < 4; j++) sum[j] = g[j];
+    }
+#pragma unroll 8
+    for (int64_t n = from; n < to; n++) {
+      LoadChannels(g, s.part + n * 2 * p.channels + c0, m, 0);
+      for (int j = 0; j < 4; j++) sum[j] += g[j];
+    }
+    __syncthreads();
+    for (int j = 0; j < 4; j++) part[k][lane * 4 + j] = sum[j];
+    __syncthreads();
+    if (k == 0)
+      for (int j = 0; j < 4; j++) {
+        const int c = m.First<4>(0) + j * m.Step();
+        for (int n = 1; n < kJoinParts; n++) sum[j] += part[n][lane * 4 + j];
+        if (c < m.channels) StoreElement(p.dtable, (int64_t)key * p.channels + c0 + c, p.dtype, sum[j] * p.scale);
+      }
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------
+struct EmbLayout {
+  EmbSort sort;
+  EmbSums sums;
+  size_t bytes;
+};
+
+// how the backward pass uses its workspace
+static EmbLayout LayOut(const daliamdEmbeddingArgs &a, void *workspace) {
+  EmbLayout l = {};
+  EmbSort &s = l.sort;
+  s.tokens = a.tokens;
+  int bits = 1;
+  while (bits < 31 && (a.vocab >> bits)) bits++;          // keys 0 .. vocab
+  s.passes = (bits + kDigitBits - 1) / kDigitBits;
+  s.bits = (bits + s.passes - 1) / s.passes;
+  s.tile = kTileTokens;
+  if (a.tokens > (int64_t)kTileTokens * kMaxTiles)
+    s.tile = ((a.tokens + kMaxTiles - 1) / kMaxTiles + kSortThreads - 1) / kSortThreads * kSortThreads;
+  s.tiles = (int)((a.tokens + s.tile - 1) / s.tile);
+  EmbSums &u = l.sums;
+  u.chunks = (int)((a.tokens + kChunk - 1) / kChunk);
+  u.tpr = 8;
+  while (u.tpr < kEmbThreads && u.tpr * kEmbV < a.channels) u.tpr *= 2;
+  u.chunk_groups = (u.chunks + kEmbThreads / u.tpr - 1) / (kEmbThreads / u.tpr);
+  uint8_t *at = static_cast<uint8_t *>(workspace);
+  auto take = [&](size_t bytes) {
+    uint8_t *p = at + l.bytes;
+    l.bytes += (bytes + 255) & ~(size_t)255;
+    return p;
+  };
+  for (int k = 0; k < 2; k++) {
+    s.key[k] = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t) * (size_t)a.tokens));
+    s.index[k] = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t) * (size_t)a.tokens));
+  }
+  s.count = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t) * kDigits * (size_t)s.tiles));
+  u.part = reinterpret_cast<float *>(take(sizeof(float) * 2 * (size_t)u.chunks * a.channels));
+  u.key = s.key[s.passes & 1];
+  u.index = s.index[s.passes & 1];
+  return l;
+}
+
+static bool WideEmbedding(const daliamdEmbeddingArgs &a, bool backward) {
+  const int e = ElementSize(a.dtype), o = ElementSize(a.out_dtype);
+  if (a.channels % kEmbV) return false;
+  if (backward) return RowsAligned(a.dout, a.dout_row, o) && RowsAligned(a.dtable, 0, e);
+  return RowsAligned(a.table, a.table_row, e) && RowsAligned(a.out, 0, o);
+}
+
+template <typename TT, typename OT> struct EmbLaunch {
+  static void Forward(hipStream_t s, const daliamdEmbeddingArgs &a) {
+    int tpr = 8;
+    while (tpr < kEmbThreads && tpr * kEmbV < a.channels) tpr *= 2;
+    const int64_t per_group = kEmbThreads / tpr;
+    const int wide = WideEmbedding(a, false);
+    KernelTimer timer("EmbeddingKernel", s);
+    // four rows per thread where that still leaves workgroups for every compute unit
+    if (a.tokens >= 4 * per_group * 1024)
+      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 4>), dim3((unsigned)((a.tokens + 4 * per_group - 1) / (4 * per_group))), dim3(kEmbThreads), 0, s, a, tpr, wide);
+    else
+      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 1>), dim3((unsigned)((a.tokens + per_group - 1) / per_group)), dim3(kEmbThreads), 0, s, a, tpr, wide);
+  }
+  static void Backward(hipStream_t s, const daliamdEmbeddingArgs &a, const EmbSums &sums) {
+    const int64_t fill = (a.vocab + kFillRows - 1) / kFillRows;
+    KernelTimer timer("EmbeddingBackwardKernel", s);
+    hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT>), dim3((unsigned)(sums.chunk_groups + fill)), dim3(kEmbThreads), 0, s, a, sums);
+  }
+};
+template <typename F> static void WithTypes(const daliamdEmbeddingArgs &a, F f) {
+  auto out = [&](auto table) {
+    using TT = decltype(table);
+    if (a.out_dtype == DALIAMD_FLOAT) f(EmbLaunch<TT, float>());
+    else if (a.out_dtype == DALIAMD_FLOAT16) f(EmbLaunch<TT, F16>());
+    else f(EmbLaunch<TT, Bf16>());
+  };
+  if (a.dtype == DALIAMD_FLOAT) out(float());
+  else if (a.dtype == DALIAMD_FLOAT16) out(F16());
+  else out(Bf16());
 }
 
 static daliamdResult_t CheckEmbedding(const daliamdEmbeddingArgs *args, daliamdEmbeddingPlan *plan) {
@@ -35,7 +437,7 @@ static daliamdResult_t CheckEmbedding(const daliamdEmbeddingArgs *args, daliamdE
                   "daliamdEmbedding: table and output must be FLOAT, FLOAT16 or BFLOAT16");
   DALIAMD_REQUIRE(a.index_dtype == DALIAMD_INT32 || a.index_dtype == DALIAMD_INT64, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdEmbedding: ids must be INT32 or INT64");
-  plan->backward_workspace_bytes = 0;
+  plan->backward_workspace_bytes = LayOut(a, nullptr).bytes;
   return DALIAMD_SUCCESS;
 }
 
@@ -55,10 +457,7 @@ daliamdResult_t daliamdEmbeddingRun(daliamdStream_t stream, const daliamdEmbeddi
   if (!args->tokens) return DALIAMD_SUCCESS;
   DALIAMD_REQUIRE(args->ids && args->table && args->out, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdEmbeddingRun: NULL tensor");
   hipStream_t s = (hipStream_t)stream;
-  {
-    KernelTimer timer("EmbeddingKernel", s);
-    hipLaunchKernelGGL(EmbeddingKernel, dim3((unsigned)args->tokens), dim3(kEmbThreads), 0, s, *args);
-  }
+  WithTypes(*args, [&](auto launch) { launch.Forward(s, *args); });
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
 }
@@ -72,9 +471,26 @@ daliamdResult_t daliamdEmbeddingBackwardRun(daliamdStream_t stream, const daliam
   DALIAMD_REQUIRE(workspace_bytes >= plan.backward_workspace_bytes && (workspace || !plan.backward_workspace_bytes),
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdEmbeddingBackwardRun: the workspace is too small");
   hipStream_t s = (hipStream_t)stream;
-  {
-    KernelTimer timer("EmbeddingBackwardKernel", s);
-    hipLaunchKernelGGL(EmbeddingBackwardKernel, dim3((unsigned)args->vocab), dim3(kEmbThreads), 0, s, *args);
+  const daliamdEmbeddingArgs &a = *args;
+  const EmbLayout l = LayOut(a, workspace);
+  EmbSums sums = l.sums;
+  sums.wide = WideEmbedding(a, true);
+  if (a.tokens && a.tokens <= kSmallTokens) {
+    KernelTimer timer("EmbeddingSortKernel", s);
+    hipLaunchKernelGGL(SortSmallKernel, dim3(1), dim3(kSmallThreads), 0, s, a, l.sort);
+  } else if (a.tokens) {
+    for (int pass = 0; pass < l.sort.passes; pass++) {
+      KernelTimer timer("EmbeddingSortKernel", s);
+      hipLaunchKernelGGL(SortCountKernel, dim3(l.sort.tiles), dim3(kSortThreads), 0, s, a, l.sort, pass);
+      hipLaunchKernelGGL(SortScatterKernel, dim3(l.sort.tiles), dim3(kSortThreads), 0, s, a, l.sort, pass);
+    }
+  }
+  WithTypes(a, [&](auto launch) { launch.Backward(s, a, sums); });
+  if (sums.chunks > 1) {
+    KernelTimer timer("EmbeddingJoinKernel", s);
+    const int tiles = (a.channels + kJoinColumns - 1) / kJoinColumns;
+    hipLaunchKernelGGL(EmbeddingJoinKernel, dim3((unsigned)sums.chunks - 1, (unsigned)(tiles < 65535 ? tiles : 65535)),
+                       dim3(kJoinLanes * kJoinParts), 0, s, a, sums);
   }
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
