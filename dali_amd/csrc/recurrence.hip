@@ -1,88 +1,33 @@
-// Linear recurrence along sequences, h_t = a_t h_{t-1} + b_t per channel, and its backward pass.
-#include "sequence_common.h"
+// C entries of the linear recurrence: checks, chunks and workspaces.  recurrence.h says how the kernels work.
+#include <algorithm>
+#include "recurrence.h"
 
 namespace daliamd {
 
-constexpr int kRecThreads = 256;
-
-struct RecArgs : daliamdRecurrenceArgs {
-  float *workspace;   // backward: per-channel gradients [sequences][channels]
-};
-
-__device__ __forceinline__ int64_t RowAt(const daliamdSequenceRows &q, int64_t row, int64_t row_stride, int64_t seq_stride) {
-  if (q.offsets) return row * row_stride;
-  const int64_t s = (uint32_t)row / (uint32_t)q.steps;
-  return s * seq_stride + (row - s * q.steps) * row_stride;
-}
-
-// a_t and the factor of x_t
-__device__ __forceinline__ void Coefficients(const RecArgs &p, int64_t row, int c, float *a, float *k) {
-  const float g = LoadElement(p.decay, p.per_channel ? c : RowAt(p.seq, row, p.decay_row, p.decay_seq) + c, p.decay_dtype);
-  if (p.form == DALIAMD_RECURRENCE_GATE) Logistic(g, a, k);
-  else *a = g, *k = 1.0f;
-}
-
-__global__ __launch_bounds__(kRecThreads) void RecurrenceForwardKernel(RecArgs p) {
-  const int c = blockIdx.x * kRecThreads + threadIdx.x, s = blockIdx.y;
-  if (c >= p.channels) return;
-  int64_t begin, end;
-  SequenceRange(p.seq, s, &begin, &end);
-  double h = p.initial ? p.initial[(int64_t)s * p.channels + c] : 0.0f;
-  for (int64_t row = begin; row < end; row++) {
-    float a, k;
-    Coefficients(p, row, c, &a, &k);
-    const double x = LoadElement(p.x, RowAt(p.seq, row, p.x_row, p.x_seq) + c, p.dtype);
-    if (p.saved) p.saved[row * p.channels + c] = (float)h;
-    h = p.form == DALIAMD_RECURRENCE_GATE ? h + (double)k * (x - h) : (double)a * h + x;
-    StoreElement(p.y, row * p.channels + c, p.dtype, (float)h);
+// per-channel gradients: the chunks' sums, in their order
+constexpr int kRecSumColumns = 16, kRecSumParts = 16;
+__global__ __launch_bounds__(kRecSumColumns * kRecSumParts) void RecurrenceChannelSumKernel(RecKernelArgs p) {
+  __shared__ float part[kRecSumParts][kRecSumColumns];
+  const int column = threadIdx.x % kRecSumColumns, k = threadIdx.x / kRecSumColumns, c = blockIdx.x * kRecSumColumns + column;
+  float sum = 0;
+  if (c < p.a.channels) {
+#pragma unroll 8
+    for (int n = k; n < p.chunks; n += kRecSumParts) sum += p.partial[(int64_t)n * p.a.channels + c];
   }
-  if (p.final_state) p.final_state[(int64_t)s * p.channels + c] = (float)h;
-}
-
-__global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecArgs p) {
-  const int c = blockIdx.x * kRecThreads + threadIdx.x, s = blockIdx.y;
-  if (c >= p.channels) return;
-  int64_t begin, end;
-  SequenceRange(p.seq, s, &begin, &end);
-  double carry = p.dfinal ? p.dfinal[(int64_t)s * p.channels + c] : 0.0f, sum = 0;
-  for (int64_t row = end - 1; row >= begin; row--) {
-    float a, k;
-    Coefficients(p, row, c, &a, &k);
-    const double lambda = carry + (p.dy ? LoadElement(p.dy, RowAt(p.seq, row, p.dy_row, p.dy_seq) + c, p.dtype) : 0.0f);
-    const double before = p.saved[row * p.channels + c];
-    double dx = lambda, da = lambda * before;
-    if (p.form == DALIAMD_RECURRENCE_GATE) {
-      dx *= k;
-      da = lambda * (before - LoadElement(p.x, RowAt(p.seq, row, p.x_row, p.x_seq) + c, p.dtype)) * ((double)a * k);
-    }
-    StoreElement(p.dx, row * p.channels + c, p.dtype, (float)dx);
-    if (p.per_channel) sum += da;
-    else StoreElement(p.ddecay, row * p.channels + c, p.decay_dtype, (float)da);
-    carry = p.form == DALIAMD_RECURRENCE_GATE ? lambda - k * lambda : a * lambda;
-  }
-  if (p.dinitial) p.dinitial[(int64_t)s * p.channels + c] = (float)carry;
-  if (p.per_channel) p.workspace[(int64_t)s * p.channels + c] = (float)sum;
-}
-
-// zeros where no sequence is
-__global__ __launch_bounds__(kRecThreads) void RecurrenceDeadRowsKernel(RecArgs p, int backward) {
-  const int64_t row = blockIdx.x;
-  int64_t begin, end;
-  if (FindSequence(p.seq, row, &begin, &end) >= 0) return;
-  for (int c = threadIdx.x; c < p.channels; c += kRecThreads) {
-    StoreElement(backward ? p.dx : p.y, row * p.channels + c, p.dtype, 0.0f);
-    if (backward && !p.per_channel) StoreElement(p.ddecay, row * p.channels + c, p.decay_dtype, 0.0f);
+  part[k][column] = sum;
+  __syncthreads();
+  if (k == 0 && c < p.a.channels) {
+    for (int n = 1; n < kRecSumParts; n++) sum += part[n][column];
+    StoreElement(p.a.ddecay, c, p.a.decay_dtype, sum);
   }
 }
 
-__global__ __launch_bounds__(kRecThreads) void RecurrenceChannelSumKernel(RecArgs p) {
-  const int c = blockIdx.x * kRecThreads + threadIdx.x;
-  if (c >= p.channels) return;
-  double sum = 0;
-  for (int s = 0; s < p.seq.sequences; s++) sum += p.workspace[(int64_t)s * p.channels + c];
-  StoreElement(p.ddecay, c, p.decay_dtype, (float)sum);
+// the initial states, where the call writes the final ones over them
+__global__ __launch_bounds__(kRecThreads) void RecurrenceCopyStateKernel(float *to, const float *from, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kRecThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kRecThreads) to[i] = from[i];
 }
 
+// ---- launches ------------------------------------------------------------------------------------------------------------
 static daliamdResult_t CheckRows(const daliamdSequenceRows &q, const char *what) {
   DALIAMD_REQUIRE(q.rows >= 0 && q.rows < ((int64_t)1 << 31) && q.sequences >= 0, DALIAMD_ERROR_OUT_OF_RANGE,
                   "%s: rows and sequences must be in [0, 2^31)", what);
@@ -95,7 +40,7 @@ static daliamdResult_t CheckRows(const daliamdSequenceRows &q, const char *what)
   return DALIAMD_SUCCESS;
 }
 
-static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args, daliamdRecurrencePlan *plan) {
+static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrence: NULL argument");
   const daliamdRecurrenceArgs &a = *args;
   if (daliamdResult_t r = CheckRows(a.seq, "daliamdRecurrence")) return r;
@@ -105,10 +50,71 @@ static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args, daliam
                   "daliamdRecurrence: decay must have x's type or be FLOAT");
   DALIAMD_REQUIRE(a.form == DALIAMD_RECURRENCE_DECAY || a.form == DALIAMD_RECURRENCE_GATE, DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrence: unknown form %d", a.form);
-  plan->saved_bytes = sizeof(float) * (size_t)a.seq.rows * a.channels;
-  plan->forward_workspace_bytes = 0;
-  plan->backward_workspace_bytes = a.per_channel ? sizeof(float) * (size_t)a.seq.sequences * a.channels : 0;
   return DALIAMD_SUCCESS;
+}
+
+constexpr int kRecEnough = 192, kRecTarget = 512;   // workgroups: enough without chunks; wanted with them
+
+// Chunks and workspaces: a function of sizes and types alone, so that the backward pass finds what the forward pass saved.
+struct RecLayout {
+  RecKernelArgs k;
+  float *initial_copy;
+  size_t saved_bytes, forward_bytes, backward_bytes;
+};
+// a few steps per sequence and nothing to save: one thread goes through a sequence's steps
+static bool FewSteps(const daliamdRecurrenceArgs &a) {
+  return !a.seq.offsets && a.seq.steps > 0 && a.seq.steps <= kRecFewSteps && !a.saved;
+}
+static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
+  RecLayout l = {};
+  RecKernelArgs &k = l.k;
+  k.a = a;
+  const daliamdSequenceRows &q = a.seq;
+  const int e = ElementSize(a.dtype), d = ElementSize(a.decay_dtype), ch = kRecLanes * (16 / e);
+  k.channel_tiles = (a.channels + ch - 1) / ch;
+  if (!q.offsets && q.steps > 0 && q.steps < kRecTile) {
+    k.chunk_rows = kRecTile / q.steps * q.steps;                     // whole sequences
+  } else if (!q.offsets && (int64_t)q.sequences * k.channel_tiles >= kRecEnough) {
+    k.chunk_rows = q.steps;
+  } else {
+    const int64_t wanted = std::max(1, kRecTarget / k.channel_tiles), tiles = (q.rows + kRecTile - 1) / kRecTile;
+    k.chunk_rows = std::max<int64_t>(1, (tiles + wanted - 1) / wanted) * kRecTile;
+    k.joined = q.rows > k.chunk_rows;
+  }
+  k.chunk_rows = std::max<int64_t>(k.chunk_rows, 1);
+  k.chunks = (int)std::max<int64_t>(1, (q.rows + k.chunk_rows - 1) / k.chunk_rows);
+  k.tiles = (int)((k.chunk_rows + kRecTile - 1) / kRecTile);
+  auto wide = [](const void *p, int64_t row, int64_t seq, int elem) { return RowsAligned(p, row, elem) && (seq * elem & 15) == 0; };
+  k.x_wide = wide(a.x, a.x_row, a.x_seq, e);
+  k.decay_wide = wide(a.decay, a.decay_row, a.decay_seq, d);
+  k.dy_wide = wide(a.dy, a.dy_row, a.dy_seq, e);
+  l.saved_bytes = sizeof(float) * (size_t)k.chunks * k.tiles * a.channels;
+  uint8_t *at = static_cast<uint8_t *>(workspace);
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t *p = at + used;
+    used += (bytes + 255) & ~(size_t)255;
+    return p;
+  };
+  if (k.joined) {
+    k.chunk_a = reinterpret_cast<double *>(take(sizeof(double) * (size_t)k.chunks * a.channels));
+    k.chunk_s = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.chunks * a.channels));
+    k.chunk_r = reinterpret_cast<int *>(take(sizeof(int) * (size_t)k.chunks * k.channel_tiles));
+  }
+  const size_t states = sizeof(float) * (size_t)q.sequences * a.channels;
+  const uint8_t *initial = reinterpret_cast<const uint8_t *>(a.initial), *final_state = reinterpret_cast<const uint8_t *>(a.final_state);
+  k.few_steps = FewSteps(a);
+  l.forward_bytes = used;
+  // tiles read initial states while others write final ones
+  if (initial && final_state && !k.few_steps && initial < final_state + states && final_state < initial + states) {
+    const size_t before = used;
+    l.initial_copy = reinterpret_cast<float *>(take(states));
+    l.forward_bytes = used;
+    used = before;
+  }
+  if (a.per_channel) k.partial = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.chunks * a.channels));
+  l.backward_bytes = used;
+  return l;
 }
 
 }  // namespace daliamd
@@ -116,28 +122,37 @@ static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args, daliam
 extern "C" {
 
 daliamdResult_t daliamdRecurrenceSetup(const daliamdRecurrenceArgs *args, daliamdRecurrencePlan *plan) {
+  using namespace daliamd;
   DALIAMD_REQUIRE(plan, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceSetup: NULL argument");
-  return daliamd::CheckRecurrence(args, plan);
+  if (daliamdResult_t r = CheckRecurrence(args)) return r;
+  const RecLayout l = LayOut(*args, nullptr);
+  plan->saved_bytes = l.saved_bytes;
+  plan->forward_workspace_bytes = l.forward_bytes;
+  plan->backward_workspace_bytes = l.backward_bytes;
+  return DALIAMD_SUCCESS;
 }
 
 daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurrenceArgs *args, void *workspace, size_t workspace_bytes) {
   using namespace daliamd;
-  daliamdRecurrencePlan plan;
-  if (daliamdResult_t r = CheckRecurrence(args, &plan)) return r;
+  if (daliamdResult_t r = CheckRecurrence(args)) return r;
   const daliamdSequenceRows &q = args->seq;
+  RecLayout l = LayOut(*args, workspace);
   DALIAMD_REQUIRE(q.rows == 0 || (args->x && args->decay && args->y), DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceRun: NULL tensor");
-  DALIAMD_REQUIRE(workspace_bytes >= plan.forward_workspace_bytes && (workspace || !plan.forward_workspace_bytes),
-                  DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceRun: the workspace is too small");
+  DALIAMD_REQUIRE(workspace_bytes >= l.forward_bytes && (workspace || !l.forward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
+                  "daliamdRecurrenceRun: the workspace is too small");
   if (!q.sequences) return DALIAMD_SUCCESS;
+  l.k.out_wide = RowsAligned(args->y, args->channels, ElementSize(args->dtype));
   hipStream_t s = (hipStream_t)stream;
-  RecArgs p;
-  static_cast<daliamdRecurrenceArgs &>(p) = *args;
-  p.workspace = nullptr;
-  {
-    KernelTimer timer("RecurrenceForwardKernel", s);
-    hipLaunchKernelGGL(RecurrenceForwardKernel, dim3((p.channels + kRecThreads - 1) / kRecThreads, q.sequences), dim3(kRecThreads), 0, s, p);
+  if (l.initial_copy) {
+    const int64_t n = (int64_t)q.sequences * args->channels;
+    KernelTimer timer("RecurrenceCopyStateKernel", s);
+    hipLaunchKernelGGL(RecurrenceCopyStateKernel, dim3((unsigned)std::min<int64_t>((n + kRecThreads - 1) / kRecThreads, 4096)), dim3(kRecThreads), 0, s,
+                       l.initial_copy, args->initial, n);
+    l.k.a.initial = l.initial_copy;
   }
-  if ((q.offsets || q.lengths) && q.rows) hipLaunchKernelGGL(RecurrenceDeadRowsKernel, dim3((unsigned)q.rows), dim3(kRecThreads), 0, s, p, 0);
+  if (args->dtype == DALIAMD_FLOAT) LaunchRecurrence<float>(s, l.k);
+  else if (args->dtype == DALIAMD_FLOAT16) LaunchRecurrence<F16>(s, l.k);
+  else LaunchRecurrence<Bf16>(s, l.k);
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
 }
@@ -145,24 +160,23 @@ daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurr
 daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const daliamdRecurrenceArgs *args, void *workspace,
                                              size_t workspace_bytes) {
   using namespace daliamd;
-  daliamdRecurrencePlan plan;
-  if (daliamdResult_t r = CheckRecurrence(args, &plan)) return r;
+  if (daliamdResult_t r = CheckRecurrence(args)) return r;
   const daliamdSequenceRows &q = args->seq;
-  DALIAMD_REQUIRE((args->ddecay || (q.rows == 0 && !args->per_channel)) && (q.rows == 0 || (args->x && args->decay && args->dx && args->saved)), DALIAMD_ERROR_INVALID_ARGUMENT,
-                  "daliamdRecurrenceBackwardRun: NULL tensor");
-  DALIAMD_REQUIRE(workspace_bytes >= plan.backward_workspace_bytes && (workspace || !plan.backward_workspace_bytes),
-                  DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: the workspace is too small");
+  RecLayout l = LayOut(*args, workspace);
+  DALIAMD_REQUIRE((args->ddecay || (q.rows == 0 && !args->per_channel)) && (q.rows == 0 || (args->x && args->decay && args->dx && args->saved)),
+                  DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: NULL tensor");
+  DALIAMD_REQUIRE(workspace_bytes >= l.backward_bytes && (workspace || !l.backward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
+                  "daliamdRecurrenceBackwardRun: the workspace is too small");
   hipStream_t s = (hipStream_t)stream;
-  RecArgs p;
-  static_cast<daliamdRecurrenceArgs &>(p) = *args;
-  p.workspace = static_cast<float *>(workspace);
-  const unsigned ctiles = (p.channels + kRecThreads - 1) / kRecThreads;
-  if (q.sequences) {
-    KernelTimer timer("RecurrenceBackwardKernel", s);
-    hipLaunchKernelGGL(RecurrenceBackwardKernel, dim3(ctiles, q.sequences), dim3(kRecThreads), 0, s, p);
+  l.k.out_wide = RowsAligned(args->dx, args->channels, ElementSize(args->dtype));
+  l.k.decay_out_wide = RowsAligned(args->ddecay, args->channels, ElementSize(args->decay_dtype));
+  if (args->dtype == DALIAMD_FLOAT) LaunchRecurrenceBackward<float>(s, l.k);
+  else if (args->dtype == DALIAMD_FLOAT16) LaunchRecurrenceBackward<F16>(s, l.k);
+  else LaunchRecurrenceBackward<Bf16>(s, l.k);
+  if (args->per_channel) {
+    KernelTimer timer("RecurrenceChannelSumKernel", s);
+    hipLaunchKernelGGL(RecurrenceChannelSumKernel, dim3((args->channels + kRecSumColumns - 1) / kRecSumColumns), dim3(kRecSumColumns * kRecSumParts), 0, s, l.k);
   }
-  if (p.per_channel) hipLaunchKernelGGL(RecurrenceChannelSumKernel, dim3(ctiles), dim3(kRecThreads), 0, s, p);
-  if ((q.offsets || q.lengths) && q.rows) hipLaunchKernelGGL(RecurrenceDeadRowsKernel, dim3((unsigned)q.rows), dim3(kRecThreads), 0, s, p, 1);
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
 }

@@ -105,14 +105,15 @@ def _recurrence_args(x, decay, initial, offsets, lengths, form):
 
 def _recurrence_forward(x, decay, initial, offsets, lengths, form, final, save):
     a = _recurrence_args(x, decay, initial, offsets, lengths, form)
+    if final is None:
+        final = torch.empty((a.seq.sequences, a.channels), dtype=torch.float32, device=x.device)
+    a.final_state = final.data_ptr()
     plan = capi.RecurrencePlan()
     capi.check(capi.kernels().daliamdRecurrenceSetup(C.byref(a), C.byref(plan)))
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if final is None:
-        final = torch.empty((a.seq.sequences, a.channels), dtype=torch.float32, device=x.device)
     saved = torch.empty(plan.saved_bytes // 4, dtype=torch.float32, device=x.device) if save else None
     ws = _workspace(plan.forward_workspace_bytes, x.device)
-    a.y, a.final_state, a.saved = y.data_ptr(), final.data_ptr(), _ptr(saved)
+    a.y, a.saved = y.data_ptr(), _ptr(saved)
     _call("daliamdRecurrenceRun", x.device, C.byref(a), C.c_void_p(_ptr(ws)), C.c_size_t(plan.forward_workspace_bytes))
     return y, final, saved
 

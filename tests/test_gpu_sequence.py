@@ -233,6 +233,20 @@ def test_recurrence_state_in_place_step_by_step(dtype):
     R.check("state", half, ref["state"], F, ref["state_slack"])
 
 
+@pytest.mark.parametrize("lens", [[40, 1, 300, 0, 7, 90], [2000, 3, 700]])
+def test_recurrence_state_in_place_packed(lens):
+    """The final states are written over the initial ones, of sequences that share a tile of rows and that span several."""
+    offsets = torch.from_numpy(np.cumsum([0] + lens)).int().cuda()
+    x, g = rand(42, sum(lens), 64, dtype=BF), decays(43, "gate", sum(lens), 64, dtype=BF)
+    state = rand(44, len(lens), 64)
+    spans = R.ranges(0, len(lens), offsets=offsets.cpu().tolist())
+    ref = R.recurrence(R.f64(x), R.f64(g), "gate", spans, R.f64(state))
+    y, s = sequence.linear_recurrence(x, g, form="gate", initial_state=state, offsets=offsets, final_state=state)
+    assert s is state
+    R.check("y", y, ref["y"], BF, ref["y_slack"])
+    R.check("state", state, ref["state"], F, ref["state_slack"])
+
+
 def test_recurrence_offsets_out_of_range_are_clamped():
     """Nothing outside the tensors is read or written, whatever the offsets say: rows behind stay as they were."""
     big = rand(36, 64 + 300, 40)
