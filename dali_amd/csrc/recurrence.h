@@ -4,22 +4,28 @@
 //   DECAY: dx = L, ddecay = L h_{t-1}      GATE: dx = (1 - f) L, ddecay = L (h_{t-1} - x_t) f (1 - f)
 //
 // A stretch of steps maps the state in front of it to the one behind it: h -> A h + S, A the product of its a_t, S what it makes
-// of 0; two stretches one after the other are (A1 A2, A2 S1 + S2).  A workgroup has 128 bytes of channels (8 lanes x 16 bytes) and
-// goes through the rows in tiles of 256: 32 stretches of 8 steps, one per thread and 16 bytes, held in registers between the two
+// of 0; two stretches one after the other are (A1 A2, A2 S1 + S2).  A workgroup has 128 bytes of channels (8 lanes x 16 bytes) of a
+// tile of 256 rows: 32 stretches of 8 steps, one per thread and 16 bytes, held in registers between the two
 // times they are needed - for (A, S) of the stretch, and, once the state in front of it is known, for the steps themselves.  The
-// states in front come from a scan over the 32 stretches (shuffles inside a wave, the four waves through LDS) and the state behind
-// the tile before, which stays in registers.  So memory is read once, in whole lines, however long the dependent chain is.
+// states in front come from a scan over the 32 stretches (shuffles inside a wave, the four waves through LDS) and the state in
+// front of the tile.  So memory is read once, in whole lines, however long the dependent chain is.
 //
 // Rows are one axis over all sequences; a sequence that begins inside a stretch is a step that forgets (R: whatever is in front
 // does not count).  Tiles inside one sequence (`interior`) take a path without these tests.
 //
+// The state in front of a tile is what the tile before leaves behind, which another workgroup has: a chain.  A workgroup says
+// what is known as soon as it is known - the product (A, S) of its tile, or the state behind it where that needs nothing from in
+// front (a sequence begins in the tile) - and then goes back along the chain, four tiles at a time, adding up products until it
+// meets a state.  Every 8th tile says no product, but the state behind it, once it has found the one in front: no tile
+// looks further back than that, and which numbers make up a state does not depend on who was first, so neither do its bits.  Tiles are given out by a counter in the order of the chain, so a
+// workgroup only ever waits for workgroups that have begun before it and wait for none behind them: every wait ends.  Each number
+// is said in one 64-bit word together with a mark that it is there, so a number and its mark cannot be seen apart and no fence is
+// needed (a release to the whole card would write back the L2 of an XCD); the words are cleared by a launch in front.
+// With whole sequences in each tile (dense, at most 256 steps) there is no chain.
+//
 // 1 - f is computed and applied as such (h += (1 - f)(x - h)), and products of decays are held in 64 bits: with a gate of 0.9999
 // the rounding of f to 32 bits is an error of 3e-8 in each of ten thousand steps that still count, and with constant gates all
 // of one sign.
-//
-// Where sequences times channel groups are too few workgroups to fill the card, or the host does not know where sequences begin,
-// the rows are cut into chunks of whole tiles: RecurrenceChunkKernel finds (A, S, R) of each, and the kernels then start from the
-// scan over the chunks in front.  That reads the inputs twice.
 //
 // The backward pass runs through the tiles from the last to the first.  It does not use y: the states are computed again in 32
 // bits from the one in front of each tile, which the forward pass saves (1/256 of the rows), in the same tile as the L_t: x, decay
@@ -40,16 +46,17 @@ constexpr int kRecTile = kRecWaves * kRecPieces * kRecSteps;
 
 struct RecKernelArgs {
   daliamdRecurrenceArgs a;
-  int64_t chunk_rows;
-  int chunks, tiles, channel_tiles;   // tiles: per chunk
+  int64_t tile_rows;                  // kRecTile, or a little less: whole sequences
+  int tiles, channel_tiles;
   bool few_steps;                     // a thread goes through a sequence's steps
-  bool joined;                        // chunks are parts of sequences: their products below are there
+  bool chained;                       // a tile may need the state behind the one before
   bool x_wide, decay_wide, dy_wide, out_wide, decay_out_wide;
-  double *chunk_a;                    // [chunks][channels]
-  float *chunk_s;                     // [chunks][channels]
-  int *chunk_r;                       // [chunks][channel_tiles]
-  float *partial;                     // per-channel gradients [chunks][channels]
+  uint32_t *ticket;                   // the chain: cleared before each launch, with the words behind it
+  uint64_t *words;                    // [tiles][kRecWords][channel_tiles * channels of a tile]
+  float *partial;                     // per-channel gradients [tiles][channels]
 };
+constexpr int kRecGroup = 8;          // tiles from one that says its state to the next
+constexpr int kRecWords = 4;          // the state behind the tile; S; A in two halves
 
 // one source file per type of x
 template <typename XT> void LaunchRecurrence(hipStream_t s, const RecKernelArgs &p);

@@ -1,10 +1,10 @@
-// C entries of the linear recurrence: checks, chunks and workspaces.  recurrence.h says how the kernels work.
+// C entries of the linear recurrence: checks, tiles and workspaces.  recurrence.h says how the kernels work.
 #include <algorithm>
 #include "recurrence.h"
 
 namespace daliamd {
 
-// per-channel gradients: the chunks' sums, in their order
+// per-channel gradients: the tiles' sums, in a fixed order
 constexpr int kRecSumColumns = 16, kRecSumParts = 16;
 __global__ __launch_bounds__(kRecSumColumns * kRecSumParts) void RecurrenceChannelSumKernel(RecKernelArgs p) {
   __shared__ float part[kRecSumParts][kRecSumColumns];
@@ -12,7 +12,7 @@ __global__ __launch_bounds__(kRecSumColumns * kRecSumParts) void RecurrenceChann
   float sum = 0;
   if (c < p.a.channels) {
 #pragma unroll 8
-    for (int n = k; n < p.chunks; n += kRecSumParts) sum += p.partial[(int64_t)n * p.a.channels + c];
+    for (int n = k; n < p.tiles; n += kRecSumParts) sum += p.partial[(int64_t)n * p.a.channels + c];
   }
   part[k][column] = sum;
   __syncthreads();
@@ -20,6 +20,10 @@ __global__ __launch_bounds__(kRecSumColumns * kRecSumParts) void RecurrenceChann
     for (int n = 1; n < kRecSumParts; n++) sum += part[n][column];
     StoreElement(p.a.ddecay, c, p.a.decay_dtype, sum);
   }
+}
+
+__global__ __launch_bounds__(kRecThreads) void RecurrenceClearKernel(uint4 *words, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kRecThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kRecThreads) words[i] = make_uint4(0, 0, 0, 0);
 }
 
 // the initial states, where the call writes the final ones over them
@@ -53,13 +57,11 @@ static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
   return DALIAMD_SUCCESS;
 }
 
-constexpr int kRecEnough = 192, kRecTarget = 512;   // workgroups: enough without chunks; wanted with them
-
-// Chunks and workspaces: a function of sizes and types alone, so that the backward pass finds what the forward pass saved.
+// Tiles and workspaces: a function of sizes and types alone, so that the backward pass finds what the forward pass saved.
 struct RecLayout {
   RecKernelArgs k;
   float *initial_copy;
-  size_t saved_bytes, forward_bytes, backward_bytes;
+  size_t chain_bytes, saved_bytes, forward_bytes, backward_bytes;
 };
 // a few steps per sequence and nothing to save: one thread goes through a sequence's steps
 static bool FewSteps(const daliamdRecurrenceArgs &a) {
@@ -72,23 +74,15 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   const daliamdSequenceRows &q = a.seq;
   const int e = ElementSize(a.dtype), d = ElementSize(a.decay_dtype), ch = kRecLanes * (16 / e);
   k.channel_tiles = (a.channels + ch - 1) / ch;
-  if (!q.offsets && q.steps > 0 && q.steps < kRecTile) {
-    k.chunk_rows = kRecTile / q.steps * q.steps;                     // whole sequences
-  } else if (!q.offsets && (int64_t)q.sequences * k.channel_tiles >= kRecEnough) {
-    k.chunk_rows = q.steps;
-  } else {
-    const int64_t wanted = std::max(1, kRecTarget / k.channel_tiles), tiles = (q.rows + kRecTile - 1) / kRecTile;
-    k.chunk_rows = std::max<int64_t>(1, (tiles + wanted - 1) / wanted) * kRecTile;
-    k.joined = q.rows > k.chunk_rows;
-  }
-  k.chunk_rows = std::max<int64_t>(k.chunk_rows, 1);
-  k.chunks = (int)std::max<int64_t>(1, (q.rows + k.chunk_rows - 1) / k.chunk_rows);
-  k.tiles = (int)((k.chunk_rows + kRecTile - 1) / kRecTile);
+  const bool whole = !q.offsets && q.steps > 0 && q.steps <= kRecTile;   // whole sequences in each tile
+  k.tile_rows = whole ? kRecTile / q.steps * q.steps : kRecTile;
+  k.tiles = (int)std::max<int64_t>(1, (q.rows + k.tile_rows - 1) / k.tile_rows);
+  k.chained = !whole && k.tiles > 1;
   auto wide = [](const void *p, int64_t row, int64_t seq, int elem) { return RowsAligned(p, row, elem) && (seq * elem & 15) == 0; };
   k.x_wide = wide(a.x, a.x_row, a.x_seq, e);
   k.decay_wide = wide(a.decay, a.decay_row, a.decay_seq, d);
   k.dy_wide = wide(a.dy, a.dy_row, a.dy_seq, e);
-  l.saved_bytes = sizeof(float) * (size_t)k.chunks * k.tiles * a.channels;
+  l.saved_bytes = sizeof(float) * (size_t)k.tiles * a.channels;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   size_t used = 0;
   auto take = [&](size_t bytes) {
@@ -96,10 +90,10 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
     used += (bytes + 255) & ~(size_t)255;
     return p;
   };
-  if (k.joined) {
-    k.chunk_a = reinterpret_cast<double *>(take(sizeof(double) * (size_t)k.chunks * a.channels));
-    k.chunk_s = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.chunks * a.channels));
-    k.chunk_r = reinterpret_cast<int *>(take(sizeof(int) * (size_t)k.chunks * k.channel_tiles));
+  if (k.chained) {
+    k.ticket = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t)));
+    k.words = reinterpret_cast<uint64_t *>(take(sizeof(uint64_t) * kRecWords * (size_t)k.tiles * k.channel_tiles * ch));
+    l.chain_bytes = used;
   }
   const size_t states = sizeof(float) * (size_t)q.sequences * a.channels;
   const uint8_t *initial = reinterpret_cast<const uint8_t *>(a.initial), *final_state = reinterpret_cast<const uint8_t *>(a.final_state);
@@ -112,9 +106,17 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
     l.forward_bytes = used;
     used = before;
   }
-  if (a.per_channel) k.partial = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.chunks * a.channels));
+  if (a.per_channel) k.partial = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.tiles * a.channels));
   l.backward_bytes = used;
   return l;
+}
+
+static void ClearChain(hipStream_t s, const RecLayout &l) {
+  if (!l.chain_bytes || l.k.few_steps) return;
+  const int64_t n = l.chain_bytes / sizeof(uint4);
+  KernelTimer timer("RecurrenceClearKernel", s);
+  hipLaunchKernelGGL(RecurrenceClearKernel, dim3((unsigned)std::min<int64_t>((n + kRecThreads - 1) / kRecThreads, 1024)), dim3(kRecThreads), 0, s,
+                     reinterpret_cast<uint4 *>(l.k.ticket), n);
 }
 
 }  // namespace daliamd
@@ -150,6 +152,7 @@ daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurr
                        l.initial_copy, args->initial, n);
     l.k.a.initial = l.initial_copy;
   }
+  ClearChain(s, l);
   if (args->dtype == DALIAMD_FLOAT) LaunchRecurrence<float>(s, l.k);
   else if (args->dtype == DALIAMD_FLOAT16) LaunchRecurrence<F16>(s, l.k);
   else LaunchRecurrence<Bf16>(s, l.k);
@@ -170,6 +173,8 @@ daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const dalia
   hipStream_t s = (hipStream_t)stream;
   l.k.out_wide = RowsAligned(args->dx, args->channels, ElementSize(args->dtype));
   l.k.decay_out_wide = RowsAligned(args->ddecay, args->channels, ElementSize(args->decay_dtype));
+  l.k.few_steps = false;
+  ClearChain(s, l);
   if (args->dtype == DALIAMD_FLOAT) LaunchRecurrenceBackward<float>(s, l.k);
   else if (args->dtype == DALIAMD_FLOAT16) LaunchRecurrenceBackward<F16>(s, l.k);
   else LaunchRecurrenceBackward<Bf16>(s, l.k);

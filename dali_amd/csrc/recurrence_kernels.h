@@ -41,20 +41,26 @@ template <typename T, int V> __device__ __forceinline__ void StoreStep(T *p, con
   }
 }
 
-// what the stretches of a tile leave behind, per wave; two of them, used in turn: one barrier per scan
+// what the stretches of a tile leave behind, per wave
 template <int CH> struct RecShared {
-  double a[2][kRecWaves][CH];
-  float s[2][kRecWaves][CH];
-  int r[2][kRecWaves];
+  double a[kRecWaves][CH];
+  float s[kRecWaves][CH];
+  int r[kRecWaves];
+  float front[CH];              // the state in front of the tile
+};
+
+// A stretch's place in its wave's scan: what is in front of it inside the wave.
+template <int V> struct RecFront {
+  double a[V];
+  float s[V];
+  bool r;
 };
 
 // A thread's place and the scans of its workgroup.
 template <typename XT> struct RecLane {
   static constexpr int V = RecV<XT>(), CH = RecChannels<XT>();
   int wave, piece, lane_c, channel, n;   // n: its channels that exist
-  int turn = 0;
-  RecShared<CH> &shared;
-  __device__ __forceinline__ RecLane(RecShared<CH> &sh, int channels, int channel_tile) : shared(sh) {
+  __device__ __forceinline__ RecLane(int channels, int channel_tile) {
     const int tid = threadIdx.x;
     wave = tid >> 6;
     piece = (tid & 63) / kRecLanes;
@@ -64,11 +70,10 @@ template <typename XT> struct RecLane {
   }
   __device__ __forceinline__ int Stretch() const { return wave * kRecPieces + piece; }
 
-  // Scan over the stretches of the workgroup, in the order of time or (REV) against it.  a, s, r: of this thread's stretch; h: the
-  // state in front of all of them -> the one behind; start: the state in front of this thread's.  MAY_RESET false: no r is set.
-  // total_a / total_r: the product over the workgroup.
+  // Scan over the stretches of a wave, in the order of time or (REV) against it; a, s, r: of this thread's stretch.  The wave's
+  // own product goes to `shared`.  MAY_RESET false: no r is set.
   template <bool REV, bool MAY_RESET>
-  __device__ __forceinline__ void Scan(double (&a)[V], float (&s)[V], bool r, double (&h)[V], float (&start)[V], double *total_a, bool *total_r) {
+  __device__ __forceinline__ RecFront<V> ScanWave(RecShared<CH> &shared, double (&a)[V], float (&s)[V], bool r) const {
     const int order = REV ? kRecPieces - 1 - piece : piece;
     bool any = r;
 #pragma unroll
@@ -86,44 +91,144 @@ template <typename XT> struct RecLane {
       }
       if (MAY_RESET && have) any |= before;
     }
-    turn ^= 1;
     if (order == kRecPieces - 1) {
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        shared.a[turn][wave][lane_c + j] = a[j];
-        shared.s[turn][wave][lane_c + j] = s[j];
+        shared.a[wave][lane_c + j] = a[j];
+        shared.s[wave][lane_c + j] = s[j];
       }
-      if (MAY_RESET && lane_c == 0) shared.r[turn][wave] = any;
+      if (lane_c == 0) shared.r[wave] = any;
     }
-    // what is in front of the stretch inside its wave
-    const bool front = order > 0;
-    const bool any_front = MAY_RESET && (REV ? __shfl_down((int)any, kRecLanes, 64) : __shfl_up((int)any, kRecLanes, 64)) != 0;
+    RecFront<V> front;
+    const bool have = order > 0;
+    front.r = MAY_RESET && (REV ? __shfl_down((int)any, kRecLanes, 64) : __shfl_up((int)any, kRecLanes, 64)) != 0 && have;
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const double a1 = REV ? __shfl_down(a[j], kRecLanes, 64) : __shfl_up(a[j], kRecLanes, 64);
       const float s1 = REV ? __shfl_down(s[j], kRecLanes, 64) : __shfl_up(s[j], kRecLanes, 64);
-      a[j] = front ? a1 : 1.0;
-      s[j] = front ? s1 : 0.0f;
+      front.a[j] = have ? a1 : 1.0;
+      front.s[j] = have ? s1 : 0.0f;
     }
-    __syncthreads();
-    double in_front[V];
+    return front;
+  }
+
+  // The state in front of this thread's stretch, from the one in front of the tile.
+  template <bool REV, bool MAY_RESET>
+  __device__ __forceinline__ void Start(const RecShared<CH> &shared, const RecFront<V> &front, const float (&in)[V], float (&start)[V]) const {
+    double h[V];
 #pragma unroll
-    for (int k = 0; k < kRecWaves; k++) {
+    for (int j = 0; j < V; j++) h[j] = in[j];
+#pragma unroll
+    for (int k = 0; k < kRecWaves - 1; k++) {
       const int w = REV ? kRecWaves - 1 - k : k;
-      const bool forget = MAY_RESET && shared.r[turn][w] != 0;
-      if (MAY_RESET && total_r) *total_r |= forget;
+      if (REV ? w <= wave : w >= wave) break;
+      const bool forget = MAY_RESET && shared.r[w] != 0;
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        if (w == wave) in_front[j] = h[j];
-        const double wa = shared.a[turn][w][lane_c + j], ws = shared.s[turn][w][lane_c + j];
-        h[j] = forget ? ws : fma(wa, h[j], ws);
-        if (total_a) total_a[j] *= wa;
-      }
+      for (int j = 0; j < V; j++) h[j] = forget ? (double)shared.s[w][lane_c + j] : fma(shared.a[w][lane_c + j], h[j], (double)shared.s[w][lane_c + j]);
     }
 #pragma unroll
-    for (int j = 0; j < V; j++) start[j] = front && any_front ? s[j] : (float)fma(a[j], in_front[j], (double)s[j]);
+    for (int j = 0; j < V; j++) start[j] = front.r ? front.s[j] : (float)fma(front.a[j], h[j], (double)front.s[j]);
   }
 };
+
+// ---- the chain -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void Say(uint64_t *word, uint32_t value) {
+  __hip_atomic_store(word, ((uint64_t)1 << 32) | value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t Hear(const uint64_t *word) { return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ bool Said(uint64_t word) { return (word >> 32) != 0; }
+__device__ __forceinline__ float Value(uint64_t word) { return BitsToFloat((uint32_t)word); }
+
+// For one channel of the workgroup's tile: finds the state in front of the tile and says what is behind it.  a, s, r: of the
+// whole tile; `known`: nothing in front counts but `state`.  Returns the state in front.
+template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int64_t channel, double a, float s, bool r, bool known, float state) {
+  uint64_t *mine = p.words + (int64_t)tile * kRecWords * width + channel;
+  const bool joint = (REV ? p.tiles - 1 - tile : tile) % kRecGroup == kRecGroup - 1;
+  if (r || known) {
+    Say(mine, __builtin_bit_cast(uint32_t, r ? s : (float)fma(a, (double)state, (double)s)));
+    if (known) return state;
+  } else if (!joint) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, a);
+    Say(mine + width, __builtin_bit_cast(uint32_t, s));
+    Say(mine + 2 * width, (uint32_t)(bits >> 32));
+    Say(mine + 3 * width, (uint32_t)bits);
+  }
+  // the product of the tiles between the one looked at and this one
+  double pa = 1.0;
+  float ps = 0.0f;
+  constexpr int kAhead = 4;
+  const int64_t step = (REV ? 1 : -1) * kRecWords * width;
+  const int last = REV ? p.tiles - 1 : 0;
+  const uint64_t *at = mine + step;
+  int left = REV ? last - tile : tile;       // tiles in front of this one
+  for (bool found = false; !found && left > 0;) {
+    uint64_t w[kAhead][kRecWords];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+#pragma unroll
+      for (int i = 0; i < kRecWords; i++) w[k][i] = k < left ? Hear(at + k * step + i * width) : 0;
+    int moved = 0;
+    bool go = true;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      if (!go) continue;
+      if (Said(w[k][0])) {
+        ps = (float)fma(pa, (double)Value(w[k][0]), (double)ps);
+        found = true;
+        go = false;
+      } else if (Said(w[k][1]) && Said(w[k][2]) && Said(w[k][3])) {
+        ps = (float)fma(pa, (double)Value(w[k][1]), (double)ps);
+        pa *= __builtin_bit_cast(double, (uint64_t)(uint32_t)w[k][2] << 32 | (uint32_t)w[k][3]);
+        moved++;
+      } else {
+        go = false;
+      }
+    }
+    at += moved * step;
+    left -= moved;
+    if (!found && moved == 0) __builtin_amdgcn_s_sleep(1);
+  }
+  if (joint && !r) Say(mine, __builtin_bit_cast(uint32_t, (float)fma(a, (double)ps, (double)s)));
+  return ps;
+}
+
+// The state in front of the tile into shared.front: by the first threads, one per channel.  initial: of `sequence` where that
+// begins with the tile (REV: ends with it); `needs`: the row in front belongs to the same sequence.
+template <bool REV, typename XT>
+__device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecChannels<XT>()> &shared, int tile, int channel_tile, bool needs,
+                                          const float *initial, int sequence) {
+  constexpr int CH = RecChannels<XT>();
+  if (threadIdx.x >= CH) return;
+  const int channel = channel_tile * CH + threadIdx.x;
+  double a = 1.0;
+  float s = 0.0f;
+  bool r = false;
+#pragma unroll
+  for (int k = 0; k < kRecWaves; k++) {
+    const int w = REV ? kRecWaves - 1 - k : k;
+    const double wa = shared.a[w][threadIdx.x];
+    const float ws = shared.s[w][threadIdx.x];
+    const bool forget = shared.r[w] != 0;
+    s = forget ? ws : (float)fma(wa, (double)s, (double)ws);
+    a *= wa;
+    r |= forget;
+  }
+  const float state = initial && sequence >= 0 && channel < p.a.channels ? initial[(int64_t)sequence * p.a.channels + channel] : 0.0f;
+  shared.front[threadIdx.x] = p.chained ? Chain<REV>(p, tile, (int64_t)p.channel_tiles * CH, channel, a, s, r, !needs, state) : state;
+}
+
+// the workgroup's tile: in the order of the chain
+template <bool REV> __device__ __forceinline__ void TakeTile(const RecKernelArgs &p, int *slot, int *tile, int *channel_tile) {
+  int64_t id = blockIdx.x;
+  if (p.chained) {
+    if (threadIdx.x == 0) *slot = (int)atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    id = *slot;
+  }
+  *channel_tile = (int)(id % p.channel_tiles);
+  *tile = (int)(id / p.channel_tiles);
+  if (REV) *tile = p.tiles - 1 - *tile;
+}
 
 // Where sequences begin and end in a thread's stretch: bit k belongs to its k-th step.
 struct RecEvents { uint32_t live, first, last; };
@@ -166,9 +271,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecDecay 
   __device__ __forceinline__ float Coefficient(const Group<GT, V> &g, int j) const {
     if (PER_CHANNEL) return k_fixed[j];
     if (FORM == DALIAMD_RECURRENCE_DECAY) return g[j];
-    float f, k;
-    Logistic(g[j], &f, &k);
-    return k;
+    return OneMinusLogistic<sizeof(GT) == 4>(g[j]);
   }
   __device__ __forceinline__ double Product(float coefficient, int j) const {
     if (PER_CHANNEL) return a_fixed[j];
@@ -216,11 +319,11 @@ template <int V> __device__ __forceinline__ void StoreState(float *state, const 
 }
 
 // Sequences of no steps: their state is the initial one, their initial state's gradient that of the state.
-template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &p, int chunk, int stretch, int channel, int n, const float *from, float *to) {
+template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &p, int tile, int stretch, int channel, int n, const float *from, float *to) {
   const daliamdSequenceRows &q = p.a.seq;
   if (!to || !(q.offsets || q.lengths || q.steps == 0)) return;
   constexpr int kStretches = kRecWaves * kRecPieces;
-  for (int64_t s = (int64_t)chunk * kStretches + stretch; s < q.sequences; s += (int64_t)p.chunks * kStretches) {
+  for (int64_t s = (int64_t)tile * kStretches + stretch; s < q.sequences; s += (int64_t)p.tiles * kStretches) {
     int64_t begin, end;
     SequenceRange(q, (int)s, &begin, &end);
     if (begin < end) continue;
@@ -230,36 +333,25 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
   }
 }
 
-// The state in front of a chunk (REV: behind it) from the products of those before it.
-template <bool REV, typename XT> __device__ __forceinline__ void JoinChunks(RecLane<XT> &lane, const RecKernelArgs &p, int chunk, int channel_tile, double (&h)[RecLane<XT>::V]) {
-  constexpr int V = RecLane<XT>::V;
-  const int count = REV ? p.chunks - 1 - chunk : chunk;
-  if (!p.joined || count == 0) return;
-  constexpr int kStretches = kRecWaves * kRecPieces;
-  const int each = (count + kStretches - 1) / kStretches, base = REV ? chunk + 1 : 0;
-  const int from = base + lane.Stretch() * each, to = min(from + each, base + count);
-  double a[V];
-  float s[V], start[V];
-  bool r = false;
-#pragma unroll
-  for (int j = 0; j < V; j++) a[j] = 1.0, s[j] = 0.0f;
-#pragma unroll 4
-  for (int k = from; k < to; k++) {
-    const int c = REV ? to - 1 - (k - from) : k;
-    const bool forget = p.chunk_r[(int64_t)c * p.channel_tiles + channel_tile] != 0;
-    r |= forget;
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-      if (j >= lane.n) continue;
-      const int64_t at = (int64_t)c * p.a.channels + lane.channel + j;
-      const double ca = p.chunk_a[at];
-      const float cs = p.chunk_s[at];
-      s[j] = forget ? cs : (float)fma(ca, (double)s[j], (double)cs);
-      a[j] *= ca;
-    }
+// What a workgroup knows of its rows: those of one sequence alone, or not.
+struct RecPlace {
+  int64_t row, limit, begin, end;
+  int sequence;
+  bool interior;
+  __device__ __forceinline__ RecPlace(const RecKernelArgs &p, int tile) {
+    row = tile * p.tile_rows;
+    limit = min(row + p.tile_rows, p.a.seq.rows);
+    sequence = row < limit ? FindSequence(p.a.seq, row, &begin, &end) : -1;
+    interior = sequence >= 0 && row + kRecTile <= min(end, limit);
   }
-  lane.template Scan<REV, true>(a, s, r, h, start, nullptr, nullptr);
-}
+  // the sequence of the last row, and whether it goes on behind
+  __device__ __forceinline__ bool GoesOn(const RecKernelArgs &p) const {
+    if (interior) return row + kRecTile < end;
+    if (row >= limit) return false;
+    int64_t b, e;
+    return FindSequence(p.a.seq, limit - 1, &b, &e) >= 0 && limit < e;
+  }
+};
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForward {
   static constexpr int V = RecV<XT>();
@@ -291,15 +383,25 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
   }
 
   template <bool EVENTS>
-  __device__ static __forceinline__ void Process(const RecKernelArgs &p, RecLane<XT> &lane, const Decay &decay, const Tile &t, int64_t row, int64_t limit,
-                                                 int sequence, bool ends, double (&h)[V]) {
+  __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> &shared, const Decay &decay,
+                                                 const Tile &t, const RecPlace &place, int tile, int channel_tile) {
+    const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = FindEvents(p.a.seq, row, limit);
     float c[kRecSteps][V], s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
-    lane.template Scan<false, EVENTS>(a, s, r, h, state, nullptr, nullptr);
+    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
+    __syncthreads();
+    const bool starts = place.sequence < 0 || place.row == place.begin;
+    FindFront<false, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
+    __syncthreads();
     if (lane.n == 0) return;
+    float in[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) in[j] = shared.front[lane.lane_c + j];
+    if (p.a.saved && lane.Stretch() == 0) StoreState<V>(p.a.saved, in, tile, p.a.channels, lane.channel, lane.n);
+    lane.template Start<false, EVENTS>(shared, front, in, state);
     XT *y = static_cast<XT *>(p.a.y) + row * p.a.channels + lane.channel;
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
@@ -316,7 +418,8 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
       StoreStep<XT, V>(y + (int64_t)k * p.a.channels, state, p.out_wide, lane.n);
       if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
     }
-    if (!EVENTS && ends && lane.Stretch() == kRecWaves * kRecPieces - 1) StoreState<V>(p.a.final_state, state, sequence, p.a.channels, lane.channel, lane.n);
+    if (!EVENTS && place.row + kRecTile == place.end && lane.Stretch() == kRecWaves * kRecPieces - 1)
+      StoreState<V>(p.a.final_state, state, place.sequence, p.a.channels, lane.channel, lane.n);
   }
 };
 
@@ -325,39 +428,17 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceForwardKernel(RecKernel
   typedef RecForward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared;
-  const int channel_tile = blockIdx.x % p.channel_tiles, chunk = blockIdx.x / p.channel_tiles;
-  RecLane<XT> lane(shared, p.a.channels, channel_tile);
+  __shared__ int slot;
+  int tile, channel_tile;
+  TakeTile<false>(p, &slot, &tile, &channel_tile);
+  const RecLane<XT> lane(p.a.channels, channel_tile);
+  const RecPlace place(p, tile);
+  typename Op::Tile t;
+  LoadTile<XT, GT, PER_CHANNEL, true>(t, p, place.row + (int64_t)lane.Stretch() * kRecSteps, place.limit, lane.channel, lane.n);
   const typename Op::Decay decay(p.a, lane.channel, lane.n);
-  double h[V] = {};
-  JoinChunks<false>(lane, p, chunk, channel_tile, h);
-  const int64_t first = chunk * p.chunk_rows, limit = min(first + p.chunk_rows, p.a.seq.rows);
-  int64_t begin = 0, end = 0;
-  int sequence = -1;
-  typename Op::Tile now, next;
-  const int64_t offset = (int64_t)lane.Stretch() * kRecSteps;
-  LoadTile<XT, GT, PER_CHANNEL, true>(next, p, first + offset, limit, lane.channel, lane.n);
-  int tile = 0;
-  for (int64_t row = first; row < limit; row += kRecTile, tile++) {
-    now = next;
-    LoadTile<XT, GT, PER_CHANNEL, true>(next, p, row + kRecTile + offset, limit, lane.channel, lane.n);
-    if (row < begin || row >= end) sequence = FindSequence(p.a.seq, row, &begin, &end);
-    const bool interior = sequence >= 0 && row + kRecTile <= end && row + kRecTile <= limit;
-    if (interior && row == begin) {
-      float state[V];
-      LoadState<V>(state, p.a.initial, sequence, p.a.channels, lane.channel, lane.n);
-#pragma unroll
-      for (int j = 0; j < V; j++) h[j] = state[j];
-    }
-    if (p.a.saved && lane.Stretch() == 0) {
-      float state[V];
-#pragma unroll
-      for (int j = 0; j < V; j++) state[j] = (float)h[j];
-      StoreState<V>(p.a.saved, state, (int64_t)chunk * p.tiles + tile, p.a.channels, lane.channel, lane.n);
-    }
-    if (interior) Op::template Process<false>(p, lane, decay, now, row + offset, limit, sequence, row + kRecTile == end, h);
-    else Op::template Process<true>(p, lane, decay, now, row + offset, limit, 0, false, h);
-  }
-  PassEmpty<V>(p, chunk, lane.Stretch(), lane.channel, lane.n, p.a.initial, p.a.final_state);
+  if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, place, tile, channel_tile);
+  else Op::template Process<true>(p, lane, shared, decay, t, place, tile, channel_tile);
+  PassEmpty<V>(p, tile, lane.Stretch(), lane.channel, lane.n, p.a.initial, p.a.final_state);
 }
 
 // (A, S, R) of a thread's stretch against time; dy NULL: zeros
@@ -400,75 +481,35 @@ template <typename XT> __device__ __forceinline__ void LoadGradient(Group<XT, Re
   }
 }
 
-// the product of each chunk, in the order of time or (REV) against it
-template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool REV>
-__global__ __launch_bounds__(kRecThreads) void RecurrenceChunkKernel(RecKernelArgs p) {
-  typedef RecForward<XT, GT, FORM, PER_CHANNEL> Op;
-  constexpr int V = RecV<XT>();
-  __shared__ RecShared<RecChannels<XT>()> shared;
-  const int channel_tile = blockIdx.x % p.channel_tiles, chunk = blockIdx.x / p.channel_tiles;
-  RecLane<XT> lane(shared, p.a.channels, channel_tile);
-  const typename Op::Decay decay(p.a, lane.channel, lane.n);
-  const int64_t first = chunk * p.chunk_rows, limit = min(first + p.chunk_rows, p.a.seq.rows);
-  double h[V] = {}, total[V];
-  bool any = false;
-#pragma unroll
-  for (int j = 0; j < V; j++) total[j] = 1.0;
-  int64_t begin = 0, end = 0;
-  for (int tile = 0; tile < p.tiles; tile++) {
-    const int64_t row = first + (int64_t)(REV ? p.tiles - 1 - tile : tile) * kRecTile;
-    if (row >= limit) continue;
-    const int64_t at = row + (int64_t)lane.Stretch() * kRecSteps;
-    typename Op::Tile t;
-    Group<XT, V> dy[kRecSteps];
-    LoadTile<XT, GT, PER_CHANNEL, !REV>(t, p, at, limit, lane.channel, lane.n);
-    if (REV) LoadGradient(dy, p, at, limit, lane.channel, lane.n);
-    const RecEvents e = FindEvents(p.a.seq, at, limit);
-    float c[kRecSteps][V], s[V], start[V];
-    double a[V];
-    bool r;
-    if (REV) {
-#pragma unroll
-      for (int k = 0; k < kRecSteps; k++)
-#pragma unroll
-        for (int j = 0; j < V; j++) c[k][j] = decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
-      r = ComposeBack<XT, GT, FORM, PER_CHANNEL, true>(p, decay, dy, c, e, at, lane.channel, lane.n, a, s);
-    } else {
-      r = Op::template Compose<true>(p, decay, t, e, at, lane.channel, lane.n, c, a, s);
-    }
-    lane.template Scan<REV, true>(a, s, r, h, start, total, &any);
-  }
-  if (lane.Stretch() == 0) {
-#pragma unroll
-    for (int j = 0; j < V; j++)
-      if (j < lane.n) {
-        const int64_t at = (int64_t)chunk * p.a.channels + lane.channel + j;
-        p.chunk_a[at] = total[j];
-        p.chunk_s[at] = (float)h[j];
-      }
-    if (threadIdx.x == 0) p.chunk_r[(int64_t)chunk * p.channel_tiles + channel_tile] = any;
-  }
-}
-
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackward {
   static constexpr int V = RecV<XT>();
   typedef RecForward<XT, GT, FORM, PER_CHANNEL> Forward;
   typedef typename Forward::Decay Decay;
   typedef typename Forward::Tile Tile;
 
-  // in_front: the state in front of the tile; m: M behind it -> M of its first step
   template <bool EVENTS>
-  __device__ static __forceinline__ void Process(const RecKernelArgs &p, RecLane<XT> &lane, const Decay &decay, const Tile &t, const Group<XT, V> (&dy)[kRecSteps],
-                                                 int64_t row, int64_t limit, int sequence, bool begins, double (&in_front)[V], double (&m)[V], float (&sum)[V]) {
+  __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> (&shared)[2], const Decay &decay,
+                                                 const Tile &t, const Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, int tile, int channel_tile,
+                                                 const float (&saved)[V], float (&sum)[V]) {
+    const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = FindEvents(p.a.seq, row, limit);
     float c[kRecSteps][V], s[V], state[V], back[V];
     double a[V];
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
-    lane.template Scan<false, EVENTS>(a, s, r, in_front, state, nullptr, nullptr);
+    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
     r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, c, e, row, lane.channel, lane.n, a, s);
-    lane.template Scan<true, EVENTS>(a, s, r, m, back, nullptr, nullptr);
+    const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
+    __syncthreads();
+    const bool needs = place.GoesOn(p);
+    FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
+    __syncthreads();
     if (lane.n == 0) return;
+    float in[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) in[j] = shared[1].front[lane.lane_c + j];
+    lane.template Start<false, EVENTS>(shared[0], front, saved, state);
+    lane.template Start<true, EVENTS>(shared[1], behind, in, back);
     int64_t begin, end;
     float before[kRecSteps][V];
 #pragma unroll
@@ -507,7 +548,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
       StoreStep<XT, V>(static_cast<XT *>(p.a.dx) + at, dx, p.out_wide, lane.n);
       if (!PER_CHANNEL) StoreStep<GT, V>(static_cast<GT *>(p.a.ddecay) + at, dg, p.decay_out_wide, lane.n);
     }
-    if (!EVENTS && begins && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, sequence, p.a.channels, lane.channel, lane.n);
+    if (!EVENTS && place.row == place.begin && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, place.sequence, p.a.channels, lane.channel, lane.n);
   }
 };
 
@@ -515,40 +556,23 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
 __global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecKernelArgs p) {
   typedef RecBackward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
-  __shared__ RecShared<RecChannels<XT>()> shared;
-  const int channel_tile = blockIdx.x % p.channel_tiles, chunk = blockIdx.x / p.channel_tiles;
-  RecLane<XT> lane(shared, p.a.channels, channel_tile);
+  __shared__ RecShared<RecChannels<XT>()> shared[2];
+  __shared__ int slot;
+  int tile, channel_tile;
+  TakeTile<true>(p, &slot, &tile, &channel_tile);
+  const RecLane<XT> lane(p.a.channels, channel_tile);
+  const RecPlace place(p, tile);
+  const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps;
+  typename Op::Tile t;
+  Group<XT, V> dy[kRecSteps];
+  float saved[V], sum[V] = {};
+  LoadTile<XT, GT, PER_CHANNEL, true>(t, p, row, place.limit, lane.channel, lane.n);
+  LoadGradient(dy, p, row, place.limit, lane.channel, lane.n);
+  LoadState<V>(saved, p.a.saved, tile, p.a.channels, lane.channel, lane.n);
   const typename Op::Decay decay(p.a, lane.channel, lane.n);
-  double m[V] = {};
-  JoinChunks<true>(lane, p, chunk, channel_tile, m);
-  const int64_t first = chunk * p.chunk_rows, limit = min(first + p.chunk_rows, p.a.seq.rows);
-  const int64_t offset = (int64_t)lane.Stretch() * kRecSteps;
-  float sum[V] = {};
-  int64_t begin = 0, end = 0;
-  int sequence = -1;
-  for (int tile = first < limit ? (int)((limit - first + kRecTile - 1) / kRecTile) - 1 : -1; tile >= 0; tile--) {
-    const int64_t row = first + (int64_t)tile * kRecTile;
-    typename Op::Tile t;
-    Group<XT, V> dy[kRecSteps];
-    float saved[V];
-    LoadTile<XT, GT, PER_CHANNEL, true>(t, p, row + offset, limit, lane.channel, lane.n);
-    LoadGradient(dy, p, row + offset, limit, lane.channel, lane.n);
-    LoadState<V>(saved, p.a.saved, (int64_t)chunk * p.tiles + tile, p.a.channels, lane.channel, lane.n);
-    if (row < begin || row >= end) sequence = FindSequence(p.a.seq, row, &begin, &end);
-    const bool interior = sequence >= 0 && row + kRecTile <= end && row + kRecTile <= limit;
-    if (interior && row + kRecTile == end) {
-      float state[V];
-      LoadState<V>(state, p.a.dfinal, sequence, p.a.channels, lane.channel, lane.n);
-#pragma unroll
-      for (int j = 0; j < V; j++) m[j] = state[j];
-    }
-    double in_front[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) in_front[j] = saved[j];
-    if (interior) Op::template Process<false>(p, lane, decay, t, dy, row + offset, limit, sequence, row == begin, in_front, m, sum);
-    else Op::template Process<true>(p, lane, decay, t, dy, row + offset, limit, 0, false, in_front, m, sum);
-  }
-  PassEmpty<V>(p, chunk, lane.Stretch(), lane.channel, lane.n, p.a.dfinal, p.a.dinitial);
+  if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
+  else Op::template Process<true>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
+  PassEmpty<V>(p, tile, lane.Stretch(), lane.channel, lane.n, p.a.dfinal, p.a.dinitial);
   if (PER_CHANNEL) {
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -558,15 +582,15 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecKerne
     __syncthreads();
     if (lane.piece == 0) {
 #pragma unroll
-      for (int j = 0; j < V; j++) shared.s[0][lane.wave][lane.lane_c + j] = sum[j];
+      for (int j = 0; j < V; j++) shared[0].s[lane.wave][lane.lane_c + j] = sum[j];
     }
     __syncthreads();
     if (lane.Stretch() == 0) {
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float total = 0;
-        for (int w = 0; w < kRecWaves; w++) total += shared.s[0][w][lane.lane_c + j];
-        if (j < lane.n) p.partial[(int64_t)chunk * p.a.channels + lane.channel + j] = total;
+        for (int w = 0; w < kRecWaves; w++) total += shared[0].s[w][lane.lane_c + j];
+        if (j < lane.n) p.partial[(int64_t)tile * p.a.channels + lane.channel + j] = total;
       }
     }
   }
@@ -615,20 +639,12 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecLaunch
       hipLaunchKernelGGL((RecurrenceStepKernel<XT, GT, FORM, PER_CHANNEL>), dim3((unsigned)((threads + kRecThreads - 1) / kRecThreads)), dim3(kRecThreads), 0, s, p);
       return;
     }
-    const dim3 grid((unsigned)p.chunks * p.channel_tiles);
-    if (p.joined) {
-      KernelTimer timer("RecurrenceChunkKernel", s);
-      hipLaunchKernelGGL((RecurrenceChunkKernel<XT, GT, FORM, PER_CHANNEL, false>), grid, dim3(kRecThreads), 0, s, p);
-    }
+    const dim3 grid((unsigned)p.tiles * p.channel_tiles);
     KernelTimer timer("RecurrenceForwardKernel", s);
     hipLaunchKernelGGL((RecurrenceForwardKernel<XT, GT, FORM, PER_CHANNEL>), grid, dim3(kRecThreads), 0, s, p);
   }
   static void Backward(hipStream_t s, const RecKernelArgs &p) {
-    const dim3 grid((unsigned)p.chunks * p.channel_tiles);
-    if (p.joined) {
-      KernelTimer timer("RecurrenceChunkKernel", s);
-      hipLaunchKernelGGL((RecurrenceChunkKernel<XT, GT, FORM, PER_CHANNEL, true>), grid, dim3(kRecThreads), 0, s, p);
-    }
+    const dim3 grid((unsigned)p.tiles * p.channel_tiles);
     KernelTimer timer("RecurrenceBackwardKernel", s);
     hipLaunchKernelGGL((RecurrenceBackwardKernel<XT, GT, FORM, PER_CHANNEL>), grid, dim3(kRecThreads), 0, s, p);
   }

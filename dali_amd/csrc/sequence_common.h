@@ -136,5 +136,22 @@ __device__ __forceinline__ void Logistic(float g, float *f, float *k) {
   *k = g < 0 ? big : small;
 }
 
+// 1 - f alone, in the instructions that the hardware has for it.  The product with log2(e) is off by 2^-24 of itself, which is
+// |g| 2^-24 of the result: EXACT puts that back.
+template <bool EXACT> __device__ __forceinline__ float OneMinusLogistic(float g) {
+  constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+#if defined(__AMDGCN__)
+  const float p = g * kLog2e;
+  float t = __builtin_amdgcn_exp2f(p);
+  if (EXACT) {
+    const float more = t * (fmaf(g, kLog2e, -p) * kLn2);
+    t += t < __builtin_inff() ? more : 0.0f;
+  }
+  return __builtin_amdgcn_rcpf(1.0f + t);
+#else
+  return (float)(1.0 / (1.0 + exp((double)g)));
+#endif
+}
+
 }  // namespace daliamd
 #endif  // DALI_AMD_CSRC_SEQUENCE_COMMON_H_

@@ -323,6 +323,11 @@ static inline unsigned long long atomicCAS(unsigned long long *p, unsigned long 
   return hipemu_atomic_cas(p, cmp, v);
 }
 
+// relaxed / ordered accesses of a scope: the model's memory is coherent
+#define __HIP_MEMORY_SCOPE_AGENT 4
+#define __hip_atomic_store(p, v, order, scope) __atomic_store_n((hipemu_a64 *)(p), (uint64_t)(v), __ATOMIC_SEQ_CST)
+#define __hip_atomic_load(p, order, scope) __atomic_load_n((const hipemu_a64 *)(p), __ATOMIC_SEQ_CST)
+
 // ------------------------------------------------------------------------------------------------ host API
 static inline const char *hipGetErrorString(hipError_t e) {
   switch (e) {
