@@ -4,10 +4,10 @@
 //   DECAY: dx = L, ddecay = L h_{t-1}      GATE: dx = (1 - f) L, ddecay = L (h_{t-1} - x_t) f (1 - f)
 //
 // A stretch of steps maps the state in front of it to the one behind it: h -> A h + S, A the product of its a_t, S what it makes
-// of 0; two stretches one after the other are (A1 A2, A2 S1 + S2).  A workgroup has 128 bytes of channels (8 lanes x 16 bytes) of a
-// tile of 256 rows: 32 stretches of 8 steps, one per thread and 16 bytes, held in registers between the two
+// of 0; two stretches one after the other are (A1 A2, A2 S1 + S2).  A workgroup has 128 bytes of channels (16 lanes x 8 bytes) of a
+// tile of 256 rows: 32 stretches of 8 steps, one per thread and 8 bytes, held in registers between the two
 // times they are needed - for (A, S) of the stretch, and, once the state in front of it is known, for the steps themselves.  The
-// states in front come from a scan over the 32 stretches (shuffles inside a wave, the four waves through LDS) and the state in
+// states in front come from a scan over the 32 stretches (shuffles inside a wave, the eight waves through LDS) and the state in
 // front of the tile.  So memory is read once, in whole lines, however long the dependent chain is.
 //
 // Rows are one axis over all sequences; a sequence that begins inside a stretch is a step that forgets (R: whatever is in front
@@ -37,8 +37,8 @@
 
 namespace daliamd {
 
-constexpr int kRecThreads = 256, kRecWaves = kRecThreads / 64;
-constexpr int kRecLanes = 8;                          // lanes over channels
+constexpr int kRecThreads = 512, kRecWaves = kRecThreads / 64;
+constexpr int kRecLanes = 16, kRecBytes = 8;          // lanes over channels, bytes of x in each
 constexpr int kRecPieces = 64 / kRecLanes;            // stretches per wave
 constexpr int kRecSteps = 8;                          // steps per stretch
 constexpr int kRecFewSteps = 4;                       // up to so many, a thread goes through a sequence's steps
@@ -46,13 +46,14 @@ constexpr int kRecTile = kRecWaves * kRecPieces * kRecSteps;
 
 struct RecKernelArgs {
   daliamdRecurrenceArgs a;
-  int64_t tile_rows;                  // kRecTile, or a little less: whole sequences
+  int tile_rows;                      // kRecTile, or a little less: whole sequences
   int tiles, channel_tiles;
   bool few_steps;                     // a thread goes through a sequence's steps
   bool chained;                       // a tile may need the state behind the one before
   bool x_wide, decay_wide, dy_wide, out_wide, decay_out_wide;
+  bool x_plain, decay_plain, dy_plain; // ... and rows one distance apart, those of a tile within 32 bits
   uint32_t *ticket;                   // the chain: cleared before each launch, with the words behind it
-  uint64_t *words;                    // [tiles][kRecWords][channel_tiles * channels of a tile]
+  uint64_t *words;                    // [tiles][channel_tiles * channels of a tile][kRecWords]
   float *partial;                     // per-channel gradients [tiles][channels]
 };
 constexpr int kRecGroup = 8;          // tiles from one that says its state to the next

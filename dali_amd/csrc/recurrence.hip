@@ -33,8 +33,8 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceCopyStateKernel(float *
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
 static daliamdResult_t CheckRows(const daliamdSequenceRows &q, const char *what) {
-  DALIAMD_REQUIRE(q.rows >= 0 && q.rows < ((int64_t)1 << 31) && q.sequences >= 0, DALIAMD_ERROR_OUT_OF_RANGE,
-                  "%s: rows and sequences must be in [0, 2^31)", what);
+  DALIAMD_REQUIRE(q.rows >= 0 && q.rows <= DALIAMD_SEQUENCE_MAX_ROWS && q.sequences >= 0, DALIAMD_ERROR_OUT_OF_RANGE,
+                  "%s: rows must be in [0, %d], sequences not negative", what, (int)DALIAMD_SEQUENCE_MAX_ROWS);
   DALIAMD_REQUIRE(!(q.offsets && q.lengths), DALIAMD_ERROR_INVALID_ARGUMENT, "%s: offsets and lengths exclude each other", what);
   DALIAMD_REQUIRE(!(q.offsets || q.lengths) || q.index_dtype == DALIAMD_INT32 || q.index_dtype == DALIAMD_INT64, DALIAMD_ERROR_UNSUPPORTED,
                   "%s: offsets and lengths must be INT32 or INT64", what);
@@ -44,11 +44,14 @@ static daliamdResult_t CheckRows(const daliamdSequenceRows &q, const char *what)
   return DALIAMD_SUCCESS;
 }
 
+// (a tile's rows of an output stay within 32 bits)
+constexpr int kRecMaxChannels = 1 << 20;
+
 static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrence: NULL argument");
   const daliamdRecurrenceArgs &a = *args;
   if (daliamdResult_t r = CheckRows(a.seq, "daliamdRecurrence")) return r;
-  DALIAMD_REQUIRE(a.channels >= 1 && a.channels <= (1 << 24), DALIAMD_ERROR_OUT_OF_RANGE, "daliamdRecurrence: channels must be in [1, 2^24]");
+  DALIAMD_REQUIRE(a.channels >= 1 && a.channels <= kRecMaxChannels, DALIAMD_ERROR_OUT_OF_RANGE, "daliamdRecurrence: channels must be in [1, %d]", kRecMaxChannels);
   DALIAMD_REQUIRE(IsSequenceType(a.dtype), DALIAMD_ERROR_UNSUPPORTED, "daliamdRecurrence: x must be FLOAT, FLOAT16 or BFLOAT16");
   DALIAMD_REQUIRE(a.decay_dtype == a.dtype || a.decay_dtype == DALIAMD_FLOAT, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdRecurrence: decay must have x's type or be FLOAT");
@@ -72,16 +75,27 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   RecKernelArgs &k = l.k;
   k.a = a;
   const daliamdSequenceRows &q = a.seq;
-  const int e = ElementSize(a.dtype), d = ElementSize(a.decay_dtype), ch = kRecLanes * (16 / e);
+  const int e = ElementSize(a.dtype), d = ElementSize(a.decay_dtype), ch = kRecLanes * (kRecBytes / e);
   k.channel_tiles = (a.channels + ch - 1) / ch;
   const bool whole = !q.offsets && q.steps > 0 && q.steps <= kRecTile;   // whole sequences in each tile
-  k.tile_rows = whole ? kRecTile / q.steps * q.steps : kRecTile;
+  k.tile_rows = whole ? kRecTile / (int)q.steps * (int)q.steps : kRecTile;
   k.tiles = (int)std::max<int64_t>(1, (q.rows + k.tile_rows - 1) / k.tile_rows);
   k.chained = !whole && k.tiles > 1;
-  auto wide = [](const void *p, int64_t row, int64_t seq, int elem) { return RowsAligned(p, row, elem) && (seq * elem & 15) == 0; };
+  // (channels by 8 bytes of x: a thread then has all of its channels or none)
+  const bool whole_groups = a.channels % (kRecBytes / e) == 0;
+  auto wide = [&](const void *p, int64_t row, int64_t seq, int elem) {
+    const int bytes = kRecBytes / e * elem;
+    return whole_groups && RowsAligned(p, row, elem, bytes) && RowsAligned(nullptr, seq, elem, bytes);
+  };
   k.x_wide = wide(a.x, a.x_row, a.x_seq, e);
   k.decay_wide = wide(a.decay, a.decay_row, a.decay_seq, d);
   k.dy_wide = wide(a.dy, a.dy_row, a.dy_seq, e);
+  auto plain = [&](bool wide, int64_t row, int64_t seq, int elem) {
+    return wide && (q.offsets || q.sequences <= 1 || seq == q.steps * row) && row >= 0 && row <= ((int64_t)1 << 31) / (kRecTile * elem) - kRecTile;
+  };
+  k.x_plain = plain(k.x_wide, a.x_row, a.x_seq, e);
+  k.decay_plain = plain(k.decay_wide, a.decay_row, a.decay_seq, d);
+  k.dy_plain = plain(k.dy_wide, a.dy_row, a.dy_seq, e);
   l.saved_bytes = sizeof(float) * (size_t)k.tiles * a.channels;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   size_t used = 0;
@@ -109,6 +123,11 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   if (a.per_channel) k.partial = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.tiles * a.channels));
   l.backward_bytes = used;
   return l;
+}
+
+static bool OutWide(const daliamdRecurrenceArgs &a, const void *p, int dtype) {
+  const int v = kRecBytes / ElementSize(a.dtype), elem = ElementSize(dtype);
+  return a.channels % v == 0 && RowsAligned(p, a.channels, elem, v * elem);
 }
 
 static void ClearChain(hipStream_t s, const RecLayout &l) {
@@ -143,7 +162,7 @@ daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurr
   DALIAMD_REQUIRE(workspace_bytes >= l.forward_bytes && (workspace || !l.forward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceRun: the workspace is too small");
   if (!q.sequences) return DALIAMD_SUCCESS;
-  l.k.out_wide = RowsAligned(args->y, args->channels, ElementSize(args->dtype));
+  l.k.out_wide = OutWide(*args, args->y, args->dtype);
   hipStream_t s = (hipStream_t)stream;
   if (l.initial_copy) {
     const int64_t n = (int64_t)q.sequences * args->channels;
@@ -171,8 +190,8 @@ daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const dalia
   DALIAMD_REQUIRE(workspace_bytes >= l.backward_bytes && (workspace || !l.backward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceBackwardRun: the workspace is too small");
   hipStream_t s = (hipStream_t)stream;
-  l.k.out_wide = RowsAligned(args->dx, args->channels, ElementSize(args->dtype));
-  l.k.decay_out_wide = RowsAligned(args->ddecay, args->channels, ElementSize(args->decay_dtype));
+  l.k.out_wide = OutWide(*args, args->dx, args->dtype);
+  l.k.decay_out_wide = OutWide(*args, args->ddecay, args->decay_dtype);
   l.k.few_steps = false;
   ClearChain(s, l);
   if (args->dtype == DALIAMD_FLOAT) LaunchRecurrenceBackward<float>(s, l.k);

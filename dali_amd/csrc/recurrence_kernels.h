@@ -6,33 +6,57 @@
 
 namespace daliamd {
 
-template <typename XT> constexpr int RecV() { return 16 / (int)sizeof(XT); }
+template <typename XT> constexpr int RecV() { return kRecBytes / (int)sizeof(XT); }
 template <typename XT> constexpr int RecChannels() { return kRecLanes * RecV<XT>(); }
 
-// the rows of a thread's stretch in a tensor: blocks of `steps` rows seq apart (dense), or one block
-struct RowCursor {
-  int64_t s, t, steps;
-  __device__ __forceinline__ RowCursor(const daliamdSequenceRows &q, int64_t row) {
-    if (q.offsets) {
-      s = 0, t = row, steps = q.rows;
-    } else {
-      s = (uint32_t)row / (uint32_t)q.steps, t = row - s * q.steps, steps = q.steps;
+// The steps of a thread's stretch in a tensor, one group of channels each.  Loads are not conditional - steps behind the last row
+// read that row again, lanes without channels the first ones - because a load under a condition is waited for where the
+// condition ends: the 16 or 24 of a tile would come one after the other.  Rows: blocks of `steps` rows seq apart, or one block.
+// `plain`: a whole tile of one block whose rows can be read 8 or 16 bytes at a time: a base in scalar registers, a step per row.
+template <typename T, int V>
+__device__ __forceinline__ void LoadSteps(Group<T, V> (&g)[kRecSteps], const void *base, const daliamdSequenceRows &q, int first, int stretch, int limit,
+                                          int64_t row_stride, int64_t seq_stride, int channel, int n, bool wide, bool plain) {
+  if (plain) {
+    const char *p = static_cast<const char *>(base) + (int64_t)first * row_stride * (int)sizeof(T);
+    const uint32_t offset = (uint32_t)(stretch * kRecSteps * (int)row_stride + (n ? channel : 0)) * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) LoadWide(g[k], reinterpret_cast<const T *>(p + (int64_t)k * row_stride * (int)sizeof(T) + offset));
+    return;
+  }
+  const int row = min(first + stretch * kRecSteps, limit - 1);
+  const int steps = (int)(q.offsets ? q.rows : q.steps), s = q.offsets ? 0 : (int)((uint32_t)row / (uint32_t)steps);
+  int t = row - s * steps;
+  const T *p = static_cast<const T *>(base) + s * seq_stride + t * row_stride + (n ? channel : 0);
+  const int64_t next_block = seq_stride - (steps - 1) * row_stride;
+  if (wide) {                  // (n is 0 or V)
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) {
+      LoadWide(g[k], p);
+      const bool wrap = ++t == steps;
+      p += row + k + 1 < limit ? (wrap ? next_block : row_stride) : 0;
+      if (wrap) t = 0;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) {
+#pragma unroll
+      for (int j = 0; j < V; j++) g[k].Set(j, p[j < n ? j : 0]);
+      const bool wrap = ++t == steps;
+      p += row + k + 1 < limit ? (wrap ? next_block : row_stride) : 0;
+      if (wrap) t = 0;
     }
   }
-  __device__ __forceinline__ void Next() { if (++t == steps) t = 0, s++; }
-  __device__ __forceinline__ int64_t At(int64_t row_stride, int64_t seq_stride) const { return s * seq_stride + t * row_stride; }
-};
-
+}
 template <typename T, int V> __device__ __forceinline__ void LoadStep(Group<T, V> &g, const T *p, bool wide, int n) {
-  if (wide && n == V) {
+  if (wide) {
     LoadWide(g, p);
   } else {
 #pragma unroll
-    for (int j = 0; j < V; j++) g.v[j] = j < n ? p[j] : FromFloat<T>(0.0f);
+    for (int j = 0; j < V; j++) g.Set(j, p[j < n ? j : 0]);
   }
 }
 template <typename T, int V> __device__ __forceinline__ void StoreStep(T *p, const float *f, bool wide, int n) {
-  if (wide && n == V) {
+  if (wide) {
     StoreWide<T, V>(p, f);
   } else {
 #pragma unroll
@@ -62,7 +86,7 @@ template <typename XT> struct RecLane {
   int wave, piece, lane_c, channel, n;   // n: its channels that exist
   __device__ __forceinline__ RecLane(int channels, int channel_tile) {
     const int tid = threadIdx.x;
-    wave = tid >> 6;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     piece = (tid & 63) / kRecLanes;
     lane_c = tid % kRecLanes * V;
     channel = channel_tile * CH + lane_c;
@@ -142,16 +166,16 @@ __device__ __forceinline__ float Value(uint64_t word) { return BitsToFloat((uint
 // For one channel of the workgroup's tile: finds the state in front of the tile and says what is behind it.  a, s, r: of the
 // whole tile; `known`: nothing in front counts but `state`.  Returns the state in front.
 template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int64_t channel, double a, float s, bool r, bool known, float state) {
-  uint64_t *mine = p.words + (int64_t)tile * kRecWords * width + channel;
+  uint64_t *mine = p.words + ((int64_t)tile * width + channel) * kRecWords;
   const bool joint = (REV ? p.tiles - 1 - tile : tile) % kRecGroup == kRecGroup - 1;
   if (r || known) {
     Say(mine, __builtin_bit_cast(uint32_t, r ? s : (float)fma(a, (double)state, (double)s)));
     if (known) return state;
   } else if (!joint) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, a);
-    Say(mine + width, __builtin_bit_cast(uint32_t, s));
-    Say(mine + 2 * width, (uint32_t)(bits >> 32));
-    Say(mine + 3 * width, (uint32_t)bits);
+    Say(mine + 1, __builtin_bit_cast(uint32_t, s));
+    Say(mine + 2, (uint32_t)(bits >> 32));
+    Say(mine + 3, (uint32_t)bits);
   }
   // the product of the tiles between the one looked at and this one
   double pa = 1.0;
@@ -166,7 +190,7 @@ template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &
 #pragma unroll
     for (int k = 0; k < kAhead; k++)
 #pragma unroll
-      for (int i = 0; i < kRecWords; i++) w[k][i] = k < left ? Hear(at + k * step + i * width) : 0;
+      for (int i = 0; i < kRecWords; i++) w[k][i] = k < left ? Hear(at + k * step + i) : 0;
     int moved = 0;
     bool go = true;
 #pragma unroll
@@ -219,24 +243,23 @@ __device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecC
 
 // the workgroup's tile: in the order of the chain
 template <bool REV> __device__ __forceinline__ void TakeTile(const RecKernelArgs &p, int *slot, int *tile, int *channel_tile) {
-  int64_t id = blockIdx.x;
+  int id = blockIdx.x;
   if (p.chained) {
     if (threadIdx.x == 0) *slot = (int)atomicAdd(p.ticket, 1u);
     __syncthreads();
-    id = *slot;
+    id = __builtin_amdgcn_readfirstlane(*slot);
   }
-  *channel_tile = (int)(id % p.channel_tiles);
-  *tile = (int)(id / p.channel_tiles);
+  *channel_tile = id % p.channel_tiles;
+  *tile = id / p.channel_tiles;
   if (REV) *tile = p.tiles - 1 - *tile;
 }
 
 // Where sequences begin and end in a thread's stretch: bit k belongs to its k-th step.
 struct RecEvents { uint32_t live, first, last; };
-__device__ __forceinline__ RecEvents FindEvents(const daliamdSequenceRows &q, int64_t row, int64_t limit) {
+__device__ __forceinline__ RecEvents FindEvents(const daliamdSequenceRows &q, int row, int limit, int begin, int end) {
   RecEvents e = {0, 0, 0};
-  int64_t begin = 0, end = 0;
   for (int k = 0; k < kRecSteps && row + k < limit; k++) {
-    const int64_t at = row + k;
+    const int at = row + k;
     if (at < begin || at >= end)
       if (FindSequence(q, at, &begin, &end) < 0) continue;
     e.live |= 1u << k;
@@ -292,19 +315,13 @@ template <typename XT, typename GT, bool PER_CHANNEL> struct RecTile {
   Group<GT, V> g[PER_CHANNEL ? 1 : kRecSteps];
 };
 
-template <typename XT, typename GT, bool PER_CHANNEL, bool X>
-__device__ __forceinline__ void LoadTile(RecTile<XT, GT, PER_CHANNEL> &t, const RecKernelArgs &p, int64_t row, int64_t limit, int channel, int n) {
+template <typename XT, typename GT, bool PER_CHANNEL>
+__device__ __forceinline__ void LoadTile(RecTile<XT, GT, PER_CHANNEL> &t, const RecKernelArgs &p, int first, int stretch, int limit, int channel, int n) {
   constexpr int V = RecV<XT>();
-  if (n == 0 || row >= limit) return;
-  RowCursor at(p.a.seq, row);
-#pragma unroll
-  for (int k = 0; k < kRecSteps; k++) {
-    if (row + k < limit) {
-      if (X) LoadStep<XT, V>(t.x[k], static_cast<const XT *>(p.a.x) + at.At(p.a.x_row, p.a.x_seq) + channel, p.x_wide, n);
-      if (!PER_CHANNEL) LoadStep<GT, V>(t.g[k], static_cast<const GT *>(p.a.decay) + at.At(p.a.decay_row, p.a.decay_seq) + channel, p.decay_wide, n);
-    }
-    at.Next();
-  }
+  const bool full = first + kRecTile <= limit;
+  LoadSteps<XT, V>(t.x, p.a.x, p.a.seq, first, stretch, limit, p.a.x_row, p.a.x_seq, channel, n, p.x_wide, p.x_plain && full);
+  if constexpr (!PER_CHANNEL)
+    LoadSteps<GT, V>(t.g, p.a.decay, p.a.seq, first, stretch, limit, p.a.decay_row, p.a.decay_seq, channel, n, p.decay_wide, p.decay_plain && full);
 }
 
 template <int V> __device__ __forceinline__ void LoadState(float (&h)[V], const float *state, int64_t s, int channels, int channel, int n) {
@@ -324,7 +341,7 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
   if (!to || !(q.offsets || q.lengths || q.steps == 0)) return;
   constexpr int kStretches = kRecWaves * kRecPieces;
   for (int64_t s = (int64_t)tile * kStretches + stretch; s < q.sequences; s += (int64_t)p.tiles * kStretches) {
-    int64_t begin, end;
+    int begin, end;
     SequenceRange(q, (int)s, &begin, &end);
     if (begin < end) continue;
     float h[V];
@@ -335,20 +352,23 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
 
 // What a workgroup knows of its rows: those of one sequence alone, or not.
 struct RecPlace {
-  int64_t row, limit, begin, end;
-  int sequence;
+  int row, limit, begin, end, sequence;   // (the same in every thread)
   bool interior;
   __device__ __forceinline__ RecPlace(const RecKernelArgs &p, int tile) {
     row = tile * p.tile_rows;
-    limit = min(row + p.tile_rows, p.a.seq.rows);
+    limit = min(row + p.tile_rows, (int)p.a.seq.rows);
+    begin = end = 0;
     sequence = row < limit ? FindSequence(p.a.seq, row, &begin, &end) : -1;
+    sequence = __builtin_amdgcn_readfirstlane(sequence);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
     interior = sequence >= 0 && row + kRecTile <= min(end, limit);
   }
-  // the sequence of the last row, and whether it goes on behind
+  // whether the sequence of the last row goes on behind
   __device__ __forceinline__ bool GoesOn(const RecKernelArgs &p) const {
     if (interior) return row + kRecTile < end;
     if (row >= limit) return false;
-    int64_t b, e;
+    int b, e;
     return FindSequence(p.a.seq, limit - 1, &b, &e) >= 0 && limit < e;
   }
 };
@@ -360,7 +380,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 
   // (A, S, R) of a thread's stretch; `c`: the steps' coefficients for the second time
   template <bool EVENTS>
-  __device__ static __forceinline__ bool Compose(const RecKernelArgs &p, const Decay &decay, const Tile &t, const RecEvents &e, int64_t row, int channel,
+  __device__ static __forceinline__ bool Compose(const RecKernelArgs &p, const Decay &decay, const Tile &t, const RecEvents &e, int row, int channel,
                                                  int n, float (&c)[kRecSteps][V], double (&a)[V], float (&s)[V]) {
 #pragma unroll
     for (int j = 0; j < V; j++) a[j] = 1.0, s[j] = 0.0f;
@@ -368,7 +388,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && !(e.live >> k & 1)) continue;
       if (EVENTS && (e.first >> k & 1)) {
-        int64_t begin, end;
+        int begin, end;
         const int q = FindSequence(p.a.seq, row + k, &begin, &end);
         LoadState<V>(s, p.a.initial, q, p.a.channels, channel, n);
       }
@@ -384,14 +404,16 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 
   template <bool EVENTS>
   __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> &shared, const Decay &decay,
-                                                 const Tile &t, const RecPlace &place, int tile, int channel_tile) {
-    const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps, limit = place.limit;
+                                                 Tile &t, const RecPlace &place, int tile, int channel_tile) {
+    const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
-    if (EVENTS) e = FindEvents(p.a.seq, row, limit);
+    if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
     float c[kRecSteps][V], s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
     __syncthreads();
     const bool starts = place.sequence < 0 || place.row == place.begin;
     FindFront<false, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
@@ -402,20 +424,21 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     for (int j = 0; j < V; j++) in[j] = shared.front[lane.lane_c + j];
     if (p.a.saved && lane.Stretch() == 0) StoreState<V>(p.a.saved, in, tile, p.a.channels, lane.channel, lane.n);
     lane.template Start<false, EVENTS>(shared, front, in, state);
-    XT *y = static_cast<XT *>(p.a.y) + row * p.a.channels + lane.channel;
+    XT *y = static_cast<XT *>(p.a.y) + (int64_t)place.row * p.a.channels;
+    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels + lane.channel);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && row + k >= limit) break;
       if (EVENTS && !(e.live >> k & 1)) {
         const float zero[V] = {};
-        StoreStep<XT, V>(y + (int64_t)k * p.a.channels, zero, p.out_wide, lane.n);
+        StoreStep<XT, V>(y + (int64_t)k * p.a.channels + offset, zero, p.out_wide, lane.n);
         continue;
       }
-      int64_t begin, end;
+      int begin, end;
       if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
 #pragma unroll
       for (int j = 0; j < V; j++) state[j] = Decay::Step(c[k][j], t.x[k][j], state[j]);
-      StoreStep<XT, V>(y + (int64_t)k * p.a.channels, state, p.out_wide, lane.n);
+      StoreStep<XT, V>(y + (int64_t)k * p.a.channels + offset, state, p.out_wide, lane.n);
       if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
     }
     if (!EVENTS && place.row + kRecTile == place.end && lane.Stretch() == kRecWaves * kRecPieces - 1)
@@ -424,7 +447,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 };
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
-__global__ __launch_bounds__(kRecThreads) void RecurrenceForwardKernel(RecKernelArgs p) {
+__global__ __launch_bounds__(kRecThreads, 4) void RecurrenceForwardKernel(RecKernelArgs p) {
   typedef RecForward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared;
@@ -434,7 +457,7 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceForwardKernel(RecKernel
   const RecLane<XT> lane(p.a.channels, channel_tile);
   const RecPlace place(p, tile);
   typename Op::Tile t;
-  LoadTile<XT, GT, PER_CHANNEL, true>(t, p, place.row + (int64_t)lane.Stretch() * kRecSteps, place.limit, lane.channel, lane.n);
+  if (place.row < place.limit) LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.channel, lane.n);
   const typename Op::Decay decay(p.a, lane.channel, lane.n);
   if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, place, tile, channel_tile);
   else Op::template Process<true>(p, lane, shared, decay, t, place, tile, channel_tile);
@@ -444,7 +467,7 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceForwardKernel(RecKernel
 // (A, S, R) of a thread's stretch against time; dy NULL: zeros
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool EVENTS>
 __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDecay<XT, GT, FORM, PER_CHANNEL> &decay, const Group<XT, RecV<XT>()> (&dy)[kRecSteps],
-                                            const float (&c)[kRecSteps][RecV<XT>()], const RecEvents &e, int64_t row, int channel, int n,
+                                            const float (&c)[kRecSteps][RecV<XT>()], const RecEvents &e, int row, int channel, int n,
                                             double (&a)[RecV<XT>()], float (&s)[RecV<XT>()]) {
   constexpr int V = RecV<XT>();
 #pragma unroll
@@ -453,7 +476,7 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
   for (int k = kRecSteps - 1; k >= 0; k--) {
     if (EVENTS && !(e.live >> k & 1)) continue;
     if (EVENTS && (e.last >> k & 1)) {
-      int64_t begin, end;
+      int begin, end;
       LoadState<V>(s, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, channel, n);
     }
 #pragma unroll
@@ -465,22 +488,6 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
   return EVENTS && e.last != 0;
 }
 
-template <typename XT> __device__ __forceinline__ void LoadGradient(Group<XT, RecV<XT>()> (&dy)[kRecSteps], const RecKernelArgs &p, int64_t row, int64_t limit,
-                                                                    int channel, int n) {
-  constexpr int V = RecV<XT>();
-  RowCursor at(p.a.seq, row < limit ? row : 0);
-#pragma unroll
-  for (int k = 0; k < kRecSteps; k++) {
-    if (p.a.dy && n && row + k < limit) {
-      LoadStep<XT, V>(dy[k], static_cast<const XT *>(p.a.dy) + at.At(p.a.dy_row, p.a.dy_seq) + channel, p.dy_wide, n);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; j++) dy[k].v[j] = FromFloat<XT>(0.0f);
-    }
-    at.Next();
-  }
-}
-
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackward {
   static constexpr int V = RecV<XT>();
   typedef RecForward<XT, GT, FORM, PER_CHANNEL> Forward;
@@ -489,28 +496,25 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 
   template <bool EVENTS>
   __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> (&shared)[2], const Decay &decay,
-                                                 const Tile &t, const Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, int tile, int channel_tile,
+                                                 Tile &t, Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, int tile, int channel_tile,
                                                  const float (&saved)[V], float (&sum)[V]) {
-    const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps, limit = place.limit;
+    const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
-    if (EVENTS) e = FindEvents(p.a.seq, row, limit);
+    if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
     float c[kRecSteps][V], s[V], state[V], back[V];
     double a[V];
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
     r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, c, e, row, lane.channel, lane.n, a, s);
     const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
     __syncthreads();
     const bool needs = place.GoesOn(p);
     FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
-    __syncthreads();
-    if (lane.n == 0) return;
-    float in[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) in[j] = shared[1].front[lane.lane_c + j];
+    // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
     lane.template Start<false, EVENTS>(shared[0], front, saved, state);
-    lane.template Start<true, EVENTS>(shared[1], behind, in, back);
-    int64_t begin, end;
+    int begin, end;
     float before[kRecSteps][V];
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
@@ -518,10 +522,18 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
       if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        before[k][j] = state[j];
-        state[j] = Decay::Step(c[k][j], t.x[k][j], state[j]);
+        const float x = t.x[k][j];
+        before[k][j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
+        state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-c[k][j], before[k][j], state[j]) : Decay::Step(c[k][j], x, state[j]);
       }
     }
+    __syncthreads();
+    if (lane.n == 0) return;
+    float in[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) in[j] = shared[1].front[lane.lane_c + j];
+    lane.template Start<true, EVENTS>(shared[1], behind, in, back);
+    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels + lane.channel);
 #pragma unroll
     for (int k = kRecSteps - 1; k >= 0; k--) {
       if (EVENTS && row + k >= limit) continue;
@@ -534,7 +546,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
           const float l = back[j] + dy[k][j];
           if (FORM == DALIAMD_RECURRENCE_GATE) {
             dx[j] = c[k][j] * l;
-            dg[j] = Decay::Back(c[k][j], dx[j]) * (before[k][j] - t.x[k][j]);   // (1 - f) L, then times f
+            dg[j] = Decay::Back(c[k][j], dx[j]) * before[k][j];   // (1 - f) L, then times f
           } else {
             dx[j] = l;
             dg[j] = l * before[k][j];
@@ -544,16 +556,16 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
         }
         if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
       }
-      const int64_t at = (row + k) * p.a.channels + lane.channel;
-      StoreStep<XT, V>(static_cast<XT *>(p.a.dx) + at, dx, p.out_wide, lane.n);
-      if (!PER_CHANNEL) StoreStep<GT, V>(static_cast<GT *>(p.a.ddecay) + at, dg, p.decay_out_wide, lane.n);
+      const int64_t at = (int64_t)(place.row + k) * p.a.channels;
+      StoreStep<XT, V>(static_cast<XT *>(p.a.dx) + at + offset, dx, p.out_wide, lane.n);
+      if (!PER_CHANNEL) StoreStep<GT, V>(static_cast<GT *>(p.a.ddecay) + at + offset, dg, p.decay_out_wide, lane.n);
     }
     if (!EVENTS && place.row == place.begin && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, place.sequence, p.a.channels, lane.channel, lane.n);
   }
 };
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
-__global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecKernelArgs p) {
+__global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKernelArgs p) {
   typedef RecBackward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared[2];
@@ -562,12 +574,21 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecKerne
   TakeTile<true>(p, &slot, &tile, &channel_tile);
   const RecLane<XT> lane(p.a.channels, channel_tile);
   const RecPlace place(p, tile);
-  const int64_t row = place.row + (int64_t)lane.Stretch() * kRecSteps;
   typename Op::Tile t;
   Group<XT, V> dy[kRecSteps];
   float saved[V], sum[V] = {};
-  LoadTile<XT, GT, PER_CHANNEL, true>(t, p, row, place.limit, lane.channel, lane.n);
-  LoadGradient(dy, p, row, place.limit, lane.channel, lane.n);
+  if (place.row < place.limit) {
+    LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.channel, lane.n);
+    if (p.a.dy)
+      LoadSteps<XT, V>(dy, p.a.dy, p.a.seq, place.row, lane.Stretch(), place.limit, p.a.dy_row, p.a.dy_seq, lane.channel, lane.n, p.dy_wide,
+                       p.dy_plain && place.row + kRecTile <= place.limit);
+  }
+  if (!p.a.dy) {
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++)
+#pragma unroll
+      for (int j = 0; j < V; j++) dy[k].Set(j, FromFloat<XT>(0.0f));
+  }
   LoadState<V>(saved, p.a.saved, tile, p.a.channels, lane.channel, lane.n);
   const typename Op::Decay decay(p.a, lane.channel, lane.n);
   if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
@@ -596,7 +617,7 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceBackwardKernel(RecKerne
   }
 }
 
-// A few steps per sequence (one token for each of many): a thread has 16 bytes of channels of one sequence.
+// A few steps per sequence (one token for each of many): a thread has 8 bytes of channels of one sequence.
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
 __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArgs p) {
   constexpr int V = RecV<XT>();
@@ -606,7 +627,7 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArg
   if (s >= p.a.seq.sequences) return;
   const int channel = (int)(id - s * groups) * V, n = min(p.a.channels - channel, V);
   const RecDecay<XT, GT, FORM, PER_CHANNEL> decay(p.a, channel, n);
-  int64_t begin, end;
+  int begin, end;
   SequenceRange(p.a.seq, (int)s, &begin, &end);
   const int64_t steps = p.a.seq.steps, length = end - begin;
   float h[V];

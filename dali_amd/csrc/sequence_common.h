@@ -3,6 +3,7 @@
 #ifndef DALI_AMD_CSRC_SEQUENCE_COMMON_H_
 #define DALI_AMD_CSRC_SEQUENCE_COMMON_H_
 
+#include <type_traits>
 #include "common.h"
 
 namespace daliamd {
@@ -28,21 +29,52 @@ template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
 #endif
 }
 
-// V adjacent elements in registers, as they are in memory; read and written 16 bytes at a time where that is possible
-template <typename T, int V> struct alignas(16) Group {
-  T v[V];
-  __device__ __forceinline__ float operator[](int j) const { return ToFloat(v[j]); }
-};
-template <typename T, int V> __device__ __forceinline__ void LoadWide(Group<T, V> &g, const T *p) {
+// V adjacent elements in registers, as they are in memory; read and written 8 or 16 bytes at a time where that is possible
+template <typename T, int V> struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Group {
+  static constexpr int kWords = V * (int)sizeof(T) / 4;
+  uint32_t word[kWords];
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return BitsToFloat(word[j]);
+    } else {
+      const uint32_t w = word[j / 2];
+      if constexpr (std::is_same<T, Bf16>::value) return BitsToFloat(j & 1 ? w & 0xffff0000u : w << 16);
+      else return (float)__builtin_bit_cast(F16, (uint16_t)(j & 1 ? w >> 16 : w));
+    }
+  }
+  __device__ __forceinline__ void Set(int j, T v) {
+    if constexpr (sizeof(T) == 4) {
+      word[j] = __builtin_bit_cast(uint32_t, v);
+    } else {
+      const uint32_t h = __builtin_bit_cast(uint16_t, v);
+      word[j / 2] = j & 1 ? (word[j / 2] & 0xffffu) | h << 16 : h;   // (in ascending order of j)
+    }
+  }
+  // The compiler keeps elements that it has unpacked once for a second use, in twice as many registers; after this it does not
+  // know that they are the same.
+  __device__ __forceinline__ void Repack() {
+#if defined(__AMDGCN__)
+    if constexpr (sizeof(T) < 4) {
 #pragma unroll
-  for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(&g)[k] = reinterpret_cast<const uint4 *>(p)[k];
+      for (int k = 0; k < kWords; k++) asm volatile("" : "+v"(word[k]));
+    }
+#endif
+  }
+};
+template <int BYTES> __device__ __forceinline__ void CopyWide(void *to, const void *from) {
+  if (BYTES % 16 == 0) {
+#pragma unroll
+    for (int k = 0; k < BYTES / 16; k++) static_cast<uint4 *>(to)[k] = static_cast<const uint4 *>(from)[k];
+  } else {
+    *static_cast<uint2 *>(to) = *static_cast<const uint2 *>(from);
+  }
 }
+template <typename T, int V> __device__ __forceinline__ void LoadWide(Group<T, V> &g, const T *p) { CopyWide<sizeof(g)>(&g, p); }
 template <typename T, int V> __device__ __forceinline__ void StoreWide(T *p, const float *f) {
   Group<T, V> g;
 #pragma unroll
-  for (int j = 0; j < V; j++) g.v[j] = FromFloat<T>(f[j]);
-#pragma unroll
-  for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(&g)[k];
+  for (int j = 0; j < V; j++) g.Set(j, FromFloat<T>(f[j]));
+  CopyWide<sizeof(g)>(p, &g);
 }
 
 // Which channels a thread of a row has, in `n` pieces of V: adjacent ones where every row of every tensor can be read 16 bytes
@@ -61,10 +93,10 @@ template <typename T, int V> __device__ __forceinline__ void LoadChannels(Group<
       return;
     }
 #pragma unroll
-    for (int k = 0; k < (int)sizeof(g) / 16; k++) reinterpret_cast<uint4 *>(&g)[k] = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < V; j++) g.Set(j, FromFloat<T>(0.0f));
   } else {
 #pragma unroll
-    for (int j = 0; j < V; j++) g.v[j] = c + j * m.threads < m.channels ? row[c + j * m.threads] : FromFloat<T>(0.0f);
+    for (int j = 0; j < V; j++) g.Set(j, c + j * m.threads < m.channels ? row[c + j * m.threads] : FromFloat<T>(0.0f));
   }
 }
 template <typename T, int V> __device__ __forceinline__ void StoreChannels(T *row, const ChannelMap &m, int i, const float *f) {
@@ -77,9 +109,9 @@ template <typename T, int V> __device__ __forceinline__ void StoreChannels(T *ro
       if (c + j * m.threads < m.channels) row[c + j * m.threads] = FromFloat<T>(f[j]);
   }
 }
-// whether rows of `elem`-byte elements, `stride` elements apart, all start at multiples of 16 bytes
-inline bool RowsAligned(const void *p, int64_t stride, int elem) {
-  return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride * elem)) & 15) == 0;
+// whether rows of `elem`-byte elements, `stride` elements apart, all start at multiples of `bytes` bytes
+inline bool RowsAligned(const void *p, int64_t stride, int elem, int bytes = 16) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride * elem)) & (bytes - 1)) == 0;
 }
 
 __device__ __forceinline__ float LoadElement(const void *p, int64_t i, int dtype) {
@@ -100,19 +132,19 @@ __device__ __forceinline__ int64_t LoadIndex(const void *p, int64_t i, int dtype
 }
 
 // the rows [begin, end) of sequence s, whatever the device holds in offsets / lengths
-__device__ __forceinline__ void SequenceRange(const daliamdSequenceRows &q, int s, int64_t *begin, int64_t *end) {
+__device__ __forceinline__ int ClampRow(int64_t v, int64_t rows) { return (int)min(max(v, (int64_t)0), rows); }
+__device__ __forceinline__ void SequenceRange(const daliamdSequenceRows &q, int s, int *begin, int *end) {
   if (q.offsets) {
-    const int64_t b = min(max(LoadIndex(q.offsets, s, q.index_dtype), (int64_t)0), q.rows);
-    *begin = b;
-    *end = max(b, min(LoadIndex(q.offsets, s + 1, q.index_dtype), q.rows));
+    *begin = ClampRow(LoadIndex(q.offsets, s, q.index_dtype), q.rows);
+    *end = max(*begin, ClampRow(LoadIndex(q.offsets, s + 1, q.index_dtype), q.rows));
   } else {
-    *begin = (int64_t)s * q.steps;
-    *end = *begin + (q.lengths ? min(max(LoadIndex(q.lengths, s, q.index_dtype), (int64_t)0), q.steps) : q.steps);
+    *begin = s * (int)q.steps;
+    *end = *begin + (q.lengths ? ClampRow(LoadIndex(q.lengths, s, q.index_dtype), q.steps) : (int)q.steps);
   }
 }
 
 // the sequence that `row` belongs to, or -1: with ascending offsets the last one that begins at or before it
-__device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int64_t row, int64_t *begin, int64_t *end) {
+__device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int row, int *begin, int *end) {
   int s;
   if (q.offsets) {
     int lo = 0, hi = q.sequences - 1;
@@ -122,7 +154,7 @@ __device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int64_
     }
     s = lo;
   } else {
-    s = (int)((uint32_t)row / (uint32_t)q.steps);
+    s = (uint32_t)row / (uint32_t)q.steps;
   }
   SequenceRange(q, s, begin, end);
   return *begin <= row && row < *end ? s : -1;

@@ -22,6 +22,7 @@ _DTYPE = {torch.float32: capi.FLOAT, torch.float16: capi.FLOAT16, torch.bfloat16
 _INDEX = {torch.int32: capi.INT32, torch.int64: capi.INT64}
 _FORMS = {"decay": capi.RECURRENCE_DECAY, "gate": capi.RECURRENCE_GATE}
 _MAX = 1 << 31
+_MAX_ROWS, _MAX_CHANNELS = 0x7fff0000, 1 << 20
 
 
 # ------------------------------------------------------------------ checks and plumbing
@@ -201,8 +202,8 @@ def linear_recurrence(x, decay, *, form="decay", initial_state=None, offsets=Non
             _tensor("lengths", lengths, dev, tuple(_INDEX), (sequences,))
             lengths = lengths.contiguous()
     channels = x.shape[-1]
-    if channels < 1 or x.numel() // max(channels, 1) >= _MAX:
-        raise ValueError(f"x must have channels and fewer than 2^31 rows, got the shape {tuple(x.shape)}")
+    if not 1 <= channels <= _MAX_CHANNELS or x.numel() // channels > _MAX_ROWS:
+        raise ValueError(f"x must have between 1 and {_MAX_CHANNELS} channels and at most {_MAX_ROWS} rows, got the shape {tuple(x.shape)}")
     _tensor("decay", decay, dev, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32))
     if tuple(decay.shape) != (channels,) and decay.shape != x.shape:
         raise ValueError(f"decay must have x's shape {tuple(x.shape)} or [{channels}], got {tuple(decay.shape)}")

@@ -771,6 +771,8 @@ typedef struct {
   int32_t sequences, index_dtype; /* INT32 or INT64                                                     */
 } daliamdSequenceRows;
 
+enum { DALIAMD_SEQUENCE_MAX_ROWS = 0x7fff0000 };
+
 /* Linear recurrence along each sequence, per channel, from h_0 = initial (0 if NULL):
  *   DECAY  h_t = a_t h_{t-1} + x_t                           a = decay
  *   GATE   h_t = f_t h_{t-1} + (1 - f_t) x_t                 f = 1 / (1 + exp(-decay))

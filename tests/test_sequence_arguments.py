@@ -113,7 +113,7 @@ def recurrence_args(**kw):
 
 
 @pytest.mark.parametrize("kw,code", [
-    ({}, 0), (dict(rows=7), 1), (dict(rows=-1), 3), (dict(rows=1 << 31), 3), (dict(sequences=-2), 3), (dict(channels=0), 3), (dict(channels=(1 << 24) + 1), 3),
+    ({}, 0), (dict(rows=7), 1), (dict(rows=-1), 3), (dict(rows=1 << 31), 3), (dict(sequences=-2), 3), (dict(channels=0), 3), (dict(channels=(1 << 20) + 1), 3),
     (dict(dtype=capi.INT8), 2), (dict(decay_dtype=capi.FLOAT16), 2), (dict(form=2), 1), (dict(offsets=8, lengths=8, index_dtype=capi.INT32), 1),
     (dict(offsets=8, index_dtype=capi.FLOAT), 2), (dict(offsets=8, index_dtype=capi.INT64, sequences=0, steps=0), 1),
     (dict(offsets=8, index_dtype=capi.INT64, rows=100, steps=0), 0)])
