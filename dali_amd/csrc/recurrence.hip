@@ -44,14 +44,11 @@ static daliamdResult_t CheckRows(const daliamdSequenceRows &q, const char *what)
   return DALIAMD_SUCCESS;
 }
 
-// (a tile's rows of an output stay within 32 bits)
-constexpr int kRecMaxChannels = 1 << 20;
-
 static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrence: NULL argument");
   const daliamdRecurrenceArgs &a = *args;
   if (daliamdResult_t r = CheckRows(a.seq, "daliamdRecurrence")) return r;
-  DALIAMD_REQUIRE(a.channels >= 1 && a.channels <= kRecMaxChannels, DALIAMD_ERROR_OUT_OF_RANGE, "daliamdRecurrence: channels must be in [1, %d]", kRecMaxChannels);
+  DALIAMD_REQUIRE(a.channels >= 1 && a.channels <= DALIAMD_RECURRENCE_MAX_CHANNELS, DALIAMD_ERROR_OUT_OF_RANGE, "daliamdRecurrence: channels must be in [1, %d]", (int)DALIAMD_RECURRENCE_MAX_CHANNELS);
   DALIAMD_REQUIRE(IsSequenceType(a.dtype), DALIAMD_ERROR_UNSUPPORTED, "daliamdRecurrence: x must be FLOAT, FLOAT16 or BFLOAT16");
   DALIAMD_REQUIRE(a.decay_dtype == a.dtype || a.decay_dtype == DALIAMD_FLOAT, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdRecurrence: decay must have x's type or be FLOAT");

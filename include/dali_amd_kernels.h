@@ -771,7 +771,8 @@ typedef struct {
   int32_t sequences, index_dtype; /* INT32 or INT64                                                     */
 } daliamdSequenceRows;
 
-enum { DALIAMD_SEQUENCE_MAX_ROWS = 0x7fff0000 };
+/* (the kernels count rows, and elements of a tile of rows, in 32 bits) */
+enum { DALIAMD_SEQUENCE_MAX_ROWS = 0x7fff0000, DALIAMD_RECURRENCE_MAX_CHANNELS = 1 << 20 };
 
 /* Linear recurrence along each sequence, per channel, from h_0 = initial (0 if NULL):
  *   DECAY  h_t = a_t h_{t-1} + x_t                           a = decay

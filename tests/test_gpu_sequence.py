@@ -12,7 +12,7 @@ from tests import sequence_reference as R
 pytestmark = pytest.mark.gpu
 
 if os.environ.get("DALI_AMD_HIPEMU"):   # the kernels on the CPU model: its "device" tensors are torch's CPU tensors
-    sequence._on_device = lambda t: True
+    sequence._HOST_MEMORY = True
 
 BF, HF, F = torch.bfloat16, torch.float16, torch.float32
 
