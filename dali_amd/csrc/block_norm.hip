@@ -32,25 +32,47 @@ template <int TPR> __device__ __forceinline__ float RowSum(float v, float (*shar
   return v;
 }
 
-template <typename XT, int V> __device__ __forceinline__ void LoadWeights(float *w, const void *p, int dtype, const ChannelMap &m, int i) {
+template <typename XT, int V> __device__ __forceinline__ void LoadWeights(float *w, const void *p, int dtype, const Channels<V> &m) {
   if (dtype == DALIAMD_FLOAT) {
     Group<float, V> g;
-    LoadChannels(g, static_cast<const float *>(p), m, i);
+    m.Load(g, static_cast<const float *>(p));
 #pragma unroll
     for (int j = 0; j < V; j++) w[j] = g[j];
   } else {
     Group<XT, V> g;
-    LoadChannels(g, static_cast<const XT *>(p), m, i);
+    m.Load(g, static_cast<const XT *>(p));
 #pragma unroll
     for (int j = 0; j < V; j++) w[j] = g[j];
   }
 }
 
+// A thread's weights: with one piece of the row, in registers for all rows; with more, read again (from the L1) for each row.
+template <typename XT, int V, int NV> struct NormWeights {
+  static constexpr bool kKeep = NV == 1;
+  const daliamdBlockNormArgs &p;
+  float kept[kKeep ? 3 : 1][V];
+  __device__ __forceinline__ NormWeights(const daliamdBlockNormArgs &p_, const Channels<V> &m) : p(p_) {
+    if (!kKeep) return;
+    if (p.post_weight) LoadWeights<XT, V>(kept[0], p.post_weight, p.weight_dtype, m);
+    if (p.scale) LoadWeights<XT, V>(kept[kKeep ? 1 : 0], p.scale, p.weight_dtype, m);
+    if (p.pre_weight) LoadWeights<XT, V>(kept[kKeep ? 2 : 0], p.pre_weight, p.weight_dtype, m);
+  }
+  template <int WHICH> __device__ __forceinline__ void Get(float (&w)[V], const Channels<V> &m) const {
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int j = 0; j < V; j++) w[j] = kept[WHICH][j];
+    } else {
+      LoadWeights<XT, V>(w, WHICH == 0 ? p.post_weight : WHICH == 1 ? p.scale : p.pre_weight, p.weight_dtype, m);
+    }
+  }
+};
+
 template <typename XT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlockNormArgs p, int wide) {
+__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlockNormArgs p) {
   constexpr int V = 16 / sizeof(XT), kRows = NormThreads<TPR>() / TPR;
   __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
-  const ChannelMap m{p.channels, TPR, (int)threadIdx.x % TPR, wide != 0};
+  const int lane = (int)threadIdx.x % TPR;
+  const NormWeights<XT, V, NV> weights(p, Channels<V>(lane * V, p.channels));
   const float inv = 1.0f / p.channels;
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / TPR;
@@ -60,161 +82,190 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
     Group<RT, V> r[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      LoadChannels(x[i], static_cast<const XT *>(p.x) + at * p.x_row, m, i);
-      if (p.gate) LoadChannels(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row, m, i);
-      if (p.residual) LoadChannels(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row, m, i);
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
+      m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
+      if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
+      if (p.residual) m.Load(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row);
     }
     float rstd = 1.0f;
     if (p.post_weight) {
       float sum = 0;
 #pragma unroll
-      for (int i = 0; i < NV; i++)
+      for (int i = 0; i < NV; i++) {
+        Channels<V>((i * TPR + lane) * V, p.channels).Mask(x[i]);
 #pragma unroll
         for (int j = 0; j < V; j++) sum = fmaf(x[i][j], x[i][j], sum);
+        x[i].Repack();
+      }
       rstd = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 0) * inv + p.eps);
-      if (p.rstd_post && m.lane == 0 && live) p.rstd_post[row] = rstd;
+      if (p.rstd_post && lane == 0 && live) p.rstd_post[row] = rstd;
     }
     float h[NV][V], sum = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
       float post[V], scale[V];
-      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
-      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
+      if (p.post_weight) weights.template Get<0>(post, m);
+      if (p.scale) weights.template Get<1>(scale, m);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float v = x[i][j];
         if (p.post_weight) v = v * rstd * post[j];
-        if (p.gate) {
-          float f, k;
-          Logistic(g[i][j], &f, &k);
-          v *= g[i][j] * f;
-        }
+        if (p.gate) v *= Silu(g[i][j]);
         if (p.scale) v *= scale[j];
         if (p.residual) v += r[i][j];
         h[i][j] = v;
-        sum = fmaf(v, v, sum);
+        sum = j >= m.begin && j < m.end ? fmaf(v, v, sum) : sum;
       }
-      if (live) StoreChannels<RT, V>(static_cast<RT *>(p.hidden) + row * p.channels, m, i, h[i]);
+      if (live) m.Store(static_cast<RT *>(p.hidden) + row * p.channels, h[i]);
     }
     if (p.pre_weight) {
       const float rstd2 = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 1) * inv + p.eps);
-      if (p.rstd_pre && m.lane == 0 && live) p.rstd_pre[row] = rstd2;
+      if (p.rstd_pre && lane == 0 && live) p.rstd_pre[row] = rstd2;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
+        const Channels<V> m((i * TPR + lane) * V, p.channels);
         float pre[V];
-        LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+        weights.template Get<2>(pre, m);
 #pragma unroll
         for (int j = 0; j < V; j++) pre[j] = h[i][j] * rstd2 * pre[j];
-        if (live) StoreChannels<XT, V>(static_cast<XT *>(p.normed) + row * p.channels, m, i, pre);
+        if (live) m.Store(static_cast<XT *>(p.normed) + row * p.channels, pre);
       }
     }
     if (TPR > 64 && (!p.post_weight || !p.pre_weight)) __syncthreads();   // one sum per row: the slot is written again
   }
 }
 
+// What a row brings to its gradients, as it is in memory.
+template <typename XT, typename RT, int TPR, int NV> struct NormRow {
+  static constexpr int V = 16 / sizeof(XT);
+  Group<XT, V> x[NV], g[NV], dn[NV];
+  Group<RT, V> r[NV], dh[NV];
+  float rstd, rstd2;
+  __device__ __forceinline__ void Load(const daliamdBlockNormArgs &p, int64_t at, int lane, bool second) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
+      m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
+      if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
+      if (second) {
+        m.Load(dn[i], static_cast<const XT *>(p.dnormed) + at * p.dnormed_row);
+        if (p.residual) m.Load(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row);
+      }
+      if (p.dhidden) m.Load(dh[i], static_cast<const RT *>(p.dhidden) + at * p.dhidden_row);
+    }
+    rstd = p.post_weight ? p.rstd_post[at] : 1.0f;
+    rstd2 = second ? p.rstd_pre[at] : 1.0f;
+  }
+  // zeros for what is another thread's: it then adds nothing to any sum
+  __device__ __forceinline__ void Mask(const daliamdBlockNormArgs &p, int lane, bool second) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
+      if (second) m.Mask(dn[i]);
+      if (p.dhidden) m.Mask(dh[i]);
+      m.Mask(x[i]);
+    }
+  }
+  __device__ __forceinline__ void Repack() {
+#pragma unroll
+    for (int i = 0; i < NV; i++) x[i].Repack(), g[i].Repack(), dn[i].Repack();
+  }
+};
+
 // partial: [gridDim.x][3][channels], sums of the workgroup's rows for post_weight, scale and pre_weight
 template <typename XT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, int wide, float *partial) {
+__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, float *partial) {
   constexpr int V = 16 / sizeof(XT), kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
   __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
-  const ChannelMap m{p.channels, TPR, (int)threadIdx.x % TPR, wide != 0};
+  const int lane = (int)threadIdx.x % TPR;
+  const NormWeights<XT, V, NV> weights(p, Channels<V>(lane * V, p.channels));
   const float inv = 1.0f / p.channels;
   const bool second = p.pre_weight && p.dnormed;
   float apost[NV][V] = {}, ascale[NV][V] = {}, apre[NV][V] = {};
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
     const int64_t row = base + threadIdx.x / TPR;
     const bool live = kRows == 1 || row < p.rows;
-    const int64_t at = live ? row : base;
-    Group<XT, V> x[NV], g[NV], dn[NV];
-    Group<RT, V> r[NV], dh[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      LoadChannels(x[i], static_cast<const XT *>(p.x) + at * p.x_row, m, i);
-      if (p.gate) LoadChannels(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row, m, i);
-      if (second) {
-        LoadChannels(dn[i], static_cast<const XT *>(p.dnormed) + at * p.dnormed_row, m, i);
-        if (p.residual) LoadChannels(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row, m, i);
-      }
-      if (p.dhidden) LoadChannels(dh[i], static_cast<const RT *>(p.dhidden) + at * p.dhidden_row, m, i);
-    }
-    const float rstd = p.post_weight ? p.rstd_post[at] : 1.0f, rstd2 = second ? p.rstd_pre[at] : 1.0f;
+    NormRow<XT, RT, TPR, NV> t;
+    t.Load(p, live ? row : base, lane, second);
+    t.Mask(p, lane, second);
+    const float rstd = t.rstd, rstd2 = t.rstd2;
     // v, and with the second norm h^ and the mean of dn w_pre h^
     float v[NV][V], hat[NV][V], mean2 = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
       float post[V], scale[V], pre[V];
-      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
-      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
-      if (second) LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+      if (p.post_weight) weights.template Get<0>(post, m);
+      if (p.scale) weights.template Get<1>(scale, m);
+      if (second) weights.template Get<2>(pre, m);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        float e = x[i][j];
+        float e = t.x[i][j];
         if (p.post_weight) e = e * rstd * post[j];
-        if (p.gate) {
-          float f, k;
-          Logistic(g[i][j], &f, &k);
-          e *= g[i][j] * f;
-        }
+        if (p.gate) e *= Silu(t.g[i][j]);
         v[i][j] = e;
         if (second) {
           if (p.scale) e *= scale[j];
-          if (p.residual) e += r[i][j];
+          if (p.residual) e += t.r[i][j];
           e *= rstd2;
           hat[i][j] = e;
-          mean2 = fmaf(dn[i][j] * pre[j], e, mean2);
+          mean2 = fmaf(t.dn[i][j] * pre[j], e, mean2);
         }
       }
     }
     if (second) mean2 = RowSum<TPR>(mean2, shared, 0) * inv;
+    t.Repack();
     float d[NV][V], mean1 = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
       float post[V], scale[V], pre[V], dgate[V];
-      if (p.post_weight) LoadWeights<XT, V>(post, p.post_weight, p.weight_dtype, m, i);
-      if (p.scale) LoadWeights<XT, V>(scale, p.scale, p.weight_dtype, m, i);
-      if (second) LoadWeights<XT, V>(pre, p.pre_weight, p.weight_dtype, m, i);
+      if (p.post_weight) weights.template Get<0>(post, m);
+      if (p.scale) weights.template Get<1>(scale, m);
+      if (second) weights.template Get<2>(pre, m);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        float e = p.dhidden ? dh[i][j] : 0.0f;
+        float e = p.dhidden ? t.dh[i][j] : 0.0f;
         if (second) {
-          e += rstd2 * (dn[i][j] * pre[j] - hat[i][j] * mean2);
-          if (live) apre[i][j] = fmaf(dn[i][j], hat[i][j], apre[i][j]);
+          e += rstd2 * (t.dn[i][j] * pre[j] - hat[i][j] * mean2);
+          apre[i][j] = fmaf(live ? t.dn[i][j] : 0.0f, hat[i][j], apre[i][j]);
         }
         d[i][j] = e;
-        if (live) ascale[i][j] = fmaf(e, v[i][j], ascale[i][j]);
+        ascale[i][j] = fmaf(live ? e : 0.0f, v[i][j], ascale[i][j]);
       }
-      if (p.residual && live) StoreChannels<RT, V>(static_cast<RT *>(p.dresidual) + row * p.channels, m, i, d[i]);
+      if (p.residual && live) m.Store(static_cast<RT *>(p.dresidual) + row * p.channels, d[i]);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float e = d[i][j];
         if (p.scale) e *= scale[j];
-        const float hat1 = x[i][j] * rstd;
+        const float hat1 = t.x[i][j] * rstd;
         if (p.gate) {
           float f, k;
-          const float gg = g[i][j];
-          Logistic(gg, &f, &k);
+          const float gg = t.g[i][j];
+          LogisticPair(gg, &f, &k);
           dgate[j] = e * (p.post_weight ? hat1 * post[j] : hat1) * (f * fmaf(gg, k, 1.0f));
           e *= gg * f;
         }
         if (p.post_weight) {
-          if (live) apost[i][j] = fmaf(e, hat1, apost[i][j]);
+          apost[i][j] = fmaf(live ? e : 0.0f, hat1, apost[i][j]);
           e *= post[j];
           mean1 = fmaf(e, hat1, mean1);
         }
         d[i][j] = e;
       }
-      if (p.gate && live) StoreChannels<XT, V>(static_cast<XT *>(p.dgate) + row * p.channels, m, i, dgate);
+      if (p.gate && live) m.Store(static_cast<XT *>(p.dgate) + row * p.channels, dgate);
     }
     if (p.post_weight) {
       mean1 = RowSum<TPR>(mean1, shared, 1) * inv;
 #pragma unroll
       for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int j = 0; j < V; j++) d[i][j] = rstd * (d[i][j] - x[i][j] * rstd * mean1);
+        for (int j = 0; j < V; j++) d[i][j] = rstd * (d[i][j] - t.x[i][j] * rstd * mean1);
     }
     if (live) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) StoreChannels<XT, V>(static_cast<XT *>(p.dx) + row * p.channels, m, i, d[i]);
+      for (int i = 0; i < NV; i++) Channels<V>((i * TPR + lane) * V, p.channels).Store(static_cast<XT *>(p.dx) + row * p.channels, d[i]);
     }
     if (TPR > 64 && (!p.post_weight || !second)) __syncthreads();
   }
@@ -223,15 +274,17 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
   if (kRows == 1) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      if (p.post_weight) StoreChannels<float, V>(out, m, i, apost[i]);
-      if (p.scale) StoreChannels<float, V>(out + p.channels, m, i, ascale[i]);
-      if (p.pre_weight) StoreChannels<float, V>(out + 2 * p.channels, m, i, apre[i]);
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
+      if (p.post_weight) m.Store(out, apost[i]);
+      if (p.scale) m.Store(out + p.channels, ascale[i]);
+      if (p.pre_weight) m.Store(out + 2 * p.channels, apre[i]);
     }
   } else {
     // the threads with the same channels in all rows of the workgroup: the first row's adds them up
     __shared__ float rows[3][kRows > 1 ? kThreads : 1];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+      const Channels<V> m((i * TPR + lane) * V, p.channels);
       float post[V], scale[V], pre[V];
 #pragma unroll
       for (int j = 0; j < V; j++) {
@@ -249,9 +302,9 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
           }
       }
       if (threadIdx.x < TPR) {
-        if (p.post_weight) StoreChannels<float, V>(out, m, i, post);
-        if (p.scale) StoreChannels<float, V>(out + p.channels, m, i, scale);
-        if (p.pre_weight) StoreChannels<float, V>(out + 2 * p.channels, m, i, pre);
+        if (p.post_weight) m.Store(out, post);
+        if (p.scale) m.Store(out + p.channels, scale);
+        if (p.pre_weight) m.Store(out + 2 * p.channels, pre);
       }
     }
   }
@@ -280,7 +333,7 @@ __global__ __launch_bounds__(kSumColumns * kSumParts) void BlockNormWeightsKerne
 
 // workgroups of the backward pass, at most: enough to fill the card, few enough that their partial sums are a small part of
 // what it moves
-static int64_t BackwardWorkgroups(int64_t rows) { return rows < 512 ? rows : 512; }
+static int64_t BackwardWorkgroups(int64_t rows) { return rows < 768 ? rows : 768; }
 
 static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdBlockNormPlan *plan) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNorm: NULL argument");
@@ -298,33 +351,18 @@ static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdB
   return DALIAMD_SUCCESS;
 }
 
-// every tensor in use can be read and written 16 bytes at a time: then a thread has adjacent channels
-static bool Wide(const daliamdBlockNormArgs &a, bool backward) {
-  const int e = ElementSize(a.dtype), r = a.residual ? ElementSize(a.residual_dtype) : e;
-  const int w = a.post_weight || a.scale || a.pre_weight ? ElementSize(a.weight_dtype) : e;
-  if (a.channels % (16 / e)) return false;
-  bool ok = RowsAligned(a.x, a.x_row, e) && RowsAligned(a.gate, a.gate ? a.gate_row : 0, e) && RowsAligned(a.residual, a.residual ? a.residual_row : 0, r) &&
-            RowsAligned(a.post_weight, 0, w) && RowsAligned(a.scale, 0, w) && RowsAligned(a.pre_weight, 0, w);
-  if (backward)
-    ok = ok && RowsAligned(a.dhidden, a.dhidden ? a.dhidden_row : 0, r) && RowsAligned(a.dnormed, a.dnormed ? a.dnormed_row : 0, e) &&
-         RowsAligned(a.dx, 0, e) && RowsAligned(a.dgate, 0, e) && RowsAligned(a.dresidual, 0, r);
-  else
-    ok = ok && RowsAligned(a.hidden, 0, r) && RowsAligned(a.normed, 0, e);
-  return ok;
-}
-
 template <typename XT, typename RT, int TPR, int NV> struct NormLaunch {
   static constexpr int kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
   static void Forward(hipStream_t s, const daliamdBlockNormArgs &a) {
     const int64_t groups = std::min<int64_t>((a.rows + kRows - 1) / kRows, 1 << 20);
     KernelTimer timer("BlockNormKernel", s);
-    hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV>), dim3((unsigned)groups), dim3(kThreads), 0, s, a, (int)Wide(a, false));
+    hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV>), dim3((unsigned)groups), dim3(kThreads), 0, s, a);
   }
   static void Backward(hipStream_t s, const daliamdBlockNormArgs &a, float *partial, int *count) {
     const int64_t groups = (a.rows + kRows - 1) / kRows;
     *count = (int)(groups < BackwardWorkgroups(a.rows) ? groups : BackwardWorkgroups(a.rows));
     KernelTimer timer("BlockNormBackwardKernel", s);
-    hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV>), dim3((unsigned)*count), dim3(kThreads), 0, s, a, (int)Wide(a, true), partial);
+    hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV>), dim3((unsigned)*count), dim3(kThreads), 0, s, a, partial);
   }
 };
 

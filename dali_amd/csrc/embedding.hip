@@ -8,8 +8,7 @@ namespace daliamd {
 constexpr int kEmbThreads = 256, kEmbV = 8;
 
 template <typename TT, typename OT, int kTokens>
-__global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingArgs p, int tpr, int wide) {
-  const ChannelMap m{p.channels, tpr, (int)threadIdx.x % tpr, wide != 0};
+__global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingArgs p, int tpr) {
   const int64_t first = ((int64_t)blockIdx.x * (kEmbThreads / tpr) + threadIdx.x / tpr) * kTokens;
   int64_t row[kTokens];
 #pragma unroll
@@ -17,16 +16,17 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingA
     const int64_t id = first + k < p.tokens ? LoadIndex(p.ids, first + k, p.index_dtype) : -1;
     row[k] = id >= 0 && id < p.vocab ? id : -1;
   }
-  for (int i = 0; i * tpr * kEmbV < p.channels; i++) {
+  for (int c = (int)threadIdx.x % tpr * kEmbV; c < p.channels; c += tpr * kEmbV) {
+    const Channels<kEmbV> m(c, p.channels);
     Group<TT, kEmbV> g[kTokens];
 #pragma unroll
-    for (int k = 0; k < kTokens; k++) LoadChannels(g[k], static_cast<const TT *>(p.table) + max(row[k], (int64_t)0) * p.table_row, m, i);
+    for (int k = 0; k < kTokens; k++) m.Load(g[k], static_cast<const TT *>(p.table) + max(row[k], (int64_t)0) * p.table_row);
 #pragma unroll
     for (int k = 0; k < kTokens; k++) {
       float v[kEmbV];
 #pragma unroll
       for (int j = 0; j < kEmbV; j++) v[j] = row[k] >= 0 ? g[k][j] * p.scale : 0.0f;
-      if (first + k < p.tokens) StoreChannels<OT, kEmbV>(static_cast<OT *>(p.out) + (first + k) * p.channels, m, i, v);
+      if (first + k < p.tokens) m.Store(static_cast<OT *>(p.out) + (first + k) * p.channels, v);
     }
   }
 }
@@ -213,7 +213,7 @@ constexpr int kChunk = 32, kFillRows = 64;
 struct EmbSums {
   const uint32_t *key, *index;
   float *part;                  // [chunks][2][channels]: of the run that came from the chunk before, of the one that goes on behind
-  int chunks, chunk_groups, tpr, wide;
+  int chunks, chunk_groups, tpr;
 };
 
 // the first place whose key is not below `key`
@@ -243,15 +243,13 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
       if (threadIdx.x == 0) empty = mask;
     }
     __syncthreads();
-    const ChannelMap m{p.channels, kEmbThreads, (int)threadIdx.x, s.wide != 0};
     const float zero[kEmbV] = {};
     for (uint64_t mask = empty; mask; mask &= mask - 1) {
       TT *out = static_cast<TT *>(p.dtable) + (row + __ffsll((unsigned long long)mask) - 1) * p.channels;
-      for (int i = 0; i * kEmbThreads * kEmbV < p.channels; i++) StoreChannels<TT, kEmbV>(out, m, i, zero);
+      for (int c = (int)threadIdx.x * kEmbV; c < p.channels; c += kEmbThreads * kEmbV) Channels<kEmbV>(c, p.channels).Store(out, zero);
     }
     return;
   }
-  const ChannelMap m{p.channels, s.tpr, (int)threadIdx.x % s.tpr, s.wide != 0};
   const int64_t chunk = (int64_t)blockIdx.x * (kEmbThreads / s.tpr) + threadIdx.x / s.tpr;
   const int64_t begin = chunk * kChunk, end = min(begin + kChunk, n);
   if (begin >= end) return;
@@ -259,7 +257,8 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
   const bool from_before = begin > 0 && s.key[begin - 1] == s.key[begin];
   const bool goes_on = end < n && s.key[end] == s.key[end - 1];
   constexpr int kAhead = 8;   // rows in flight
-  for (int i = 0; i * s.tpr * kEmbV < p.channels; i++) {
+  for (int c = (int)threadIdx.x % s.tpr * kEmbV; c < p.channels; c += s.tpr * kEmbV) {
+    const Channels<kEmbV> m(c, p.channels);
     float sum[kEmbV] = {};
     uint32_t run = s.key[begin];
     bool first = true;        // the chunk's first run
@@ -269,19 +268,20 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
 #pragma unroll
       for (int a = 0; a < kAhead; a++) {
         key[a] = t0 + a < end ? s.key[t0 + a] : vocab;
-        if (key[a] < vocab) LoadChannels(g[a], static_cast<const OT *>(p.dout) + (int64_t)s.index[t0 + a] * p.dout_row, m, i);
+        const int64_t token = key[a] < vocab ? s.index[t0 + a] : 0;
+        m.Load(g[a], static_cast<const OT *>(p.dout) + token * p.dout_row);
       }
 #pragma unroll
       for (int a = 0; a < kAhead; a++) {
         if (key[a] != run && run < vocab) {   // a run ends, not the chunk's last
           if (first && from_before) {
-            StoreChannels<float, kEmbV>(s.part + chunk * 2 * p.channels, m, i, sum);
+            m.Store(s.part + chunk * 2 * p.channels, sum);
           } else if (t0 + a < end || !goes_on) {
 #pragma unroll
             for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
-            StoreChannels<TT, kEmbV>(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, m, i, sum);
+            m.Store(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, sum);
           } else {
-            StoreChannels<float, kEmbV>(s.part + (chunk * 2 + 1) * p.channels, m, i, sum);
+            m.Store(s.part + (chunk * 2 + 1) * p.channels, sum);
           }
           first = false;
 #pragma unroll
@@ -296,13 +296,13 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     }
     if (run < vocab) {        // the chunk's last token was the last of a group of kAhead
       if (first && from_before) {
-        StoreChannels<float, kEmbV>(s.part + chunk * 2 * p.channels, m, i, sum);
+        m.Store(s.part + chunk * 2 * p.channels, sum);
       } else if (goes_on) {
-        StoreChannels<float, kEmbV>(s.part + (chunk * 2 + 1) * p.channels, m, i, sum);
+        m.Store(s.part + (chunk * 2 + 1) * p.channels, sum);
       } else {
 #pragma unroll
         for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
-        StoreChannels<TT, kEmbV>(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, m, i, sum);
+        m.Store(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, sum);
       }
     }
   }
@@ -323,16 +323,16 @@ __global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(d
   const int64_t count = last - chunk, each = (count + kJoinParts - 1) / kJoinParts;
   const int64_t from = chunk + 1 + k * each, to = min(from + each, last + 1);
   for (int c0 = blockIdx.y * kJoinColumns; c0 < p.channels; c0 += gridDim.y * kJoinColumns) {
-    const ChannelMap m{p.channels - c0, kJoinLanes, lane, (p.channels & 3) == 0};
+    const Channels<4> m(c0 + lane * 4, p.channels);
     float sum[4] = {};
     Group<float, 4> g;
     if (k == 0) {
-      LoadChannels(g, s.part + (chunk * 2 + 1) * p.channels + c0, m, 0);
+      m.Load(g, s.part + (chunk * 2 + 1) * p.channels);
       for (int j = 0; j < 4; j++) sum[j] = g[j];
     }
 #pragma unroll 8
     for (int64_t n = from; n < to; n++) {
-      LoadChannels(g, s.part + n * 2 * p.channels + c0, m, 0);
+      m.Load(g, s.part + n * 2 * p.channels);
       for (int j = 0; j < 4; j++) sum[j] += g[j];
     }
     __syncthreads();
@@ -340,9 +340,8 @@ __global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(d
     __syncthreads();
     if (k == 0)
       for (int j = 0; j < 4; j++) {
-        const int c = m.First<4>(0) + j * m.Step();
         for (int n = 1; n < kJoinParts; n++) sum[j] += part[n][lane * 4 + j];
-        if (c < m.channels) StoreElement(p.dtable, (int64_t)key * p.channels + c0 + c, p.dtype, sum[j] * p.scale);
+        if (j >= m.begin && j < m.end) StoreElement(p.dtable, (int64_t)key * p.channels + m.base + j, p.dtype, sum[j] * p.scale);
       }
   }
 }
@@ -389,25 +388,17 @@ static EmbLayout LayOut(const daliamdEmbeddingArgs &a, void *workspace) {
   return l;
 }
 
-static bool WideEmbedding(const daliamdEmbeddingArgs &a, bool backward) {
-  const int e = ElementSize(a.dtype), o = ElementSize(a.out_dtype);
-  if (a.channels % kEmbV) return false;
-  if (backward) return RowsAligned(a.dout, a.dout_row, o) && RowsAligned(a.dtable, 0, e);
-  return RowsAligned(a.table, a.table_row, e) && RowsAligned(a.out, 0, o);
-}
-
 template <typename TT, typename OT> struct EmbLaunch {
   static void Forward(hipStream_t s, const daliamdEmbeddingArgs &a) {
     int tpr = 8;
     while (tpr < kEmbThreads && tpr * kEmbV < a.channels) tpr *= 2;
     const int64_t per_group = kEmbThreads / tpr;
-    const int wide = WideEmbedding(a, false);
     KernelTimer timer("EmbeddingKernel", s);
     // four rows per thread where that still leaves workgroups for every compute unit
     if (a.tokens >= 4 * per_group * 1024)
-      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 4>), dim3((unsigned)((a.tokens + 4 * per_group - 1) / (4 * per_group))), dim3(kEmbThreads), 0, s, a, tpr, wide);
+      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 4>), dim3((unsigned)((a.tokens + 4 * per_group - 1) / (4 * per_group))), dim3(kEmbThreads), 0, s, a, tpr);
     else
-      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 1>), dim3((unsigned)((a.tokens + per_group - 1) / per_group)), dim3(kEmbThreads), 0, s, a, tpr, wide);
+      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 1>), dim3((unsigned)((a.tokens + per_group - 1) / per_group)), dim3(kEmbThreads), 0, s, a, tpr);
   }
   static void Backward(hipStream_t s, const daliamdEmbeddingArgs &a, const EmbSums &sums) {
     const int64_t fill = (a.vocab + kFillRows - 1) / kFillRows;
@@ -473,8 +464,7 @@ daliamdResult_t daliamdEmbeddingBackwardRun(daliamdStream_t stream, const daliam
   hipStream_t s = (hipStream_t)stream;
   const daliamdEmbeddingArgs &a = *args;
   const EmbLayout l = LayOut(a, workspace);
-  EmbSums sums = l.sums;
-  sums.wide = WideEmbedding(a, true);
+  const EmbSums &sums = l.sums;
   if (a.tokens && a.tokens <= kSmallTokens) {
     KernelTimer timer("EmbeddingSortKernel", s);
     hipLaunchKernelGGL(SortSmallKernel, dim3(1), dim3(kSmallThreads), 0, s, a, l.sort);

@@ -50,8 +50,7 @@ struct RecKernelArgs {
   int tiles, channel_tiles;
   bool few_steps;                     // a thread goes through a sequence's steps
   bool chained;                       // a tile may need the state behind the one before
-  bool x_wide, decay_wide, dy_wide, out_wide, decay_out_wide;
-  bool x_plain, decay_plain, dy_plain; // ... and rows one distance apart, those of a tile within 32 bits
+  bool x_plain, decay_plain, dy_plain; // rows one distance apart, those of a tile within 32 bits
   uint32_t *ticket;                   // the chain: cleared before each launch, with the words behind it
   uint64_t *words;                    // [tiles][channel_tiles * channels of a tile][kRecWords]
   float *partial;                     // per-channel gradients [tiles][channels]

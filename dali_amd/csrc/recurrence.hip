@@ -78,21 +78,12 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   k.tile_rows = whole ? kRecTile / (int)q.steps * (int)q.steps : kRecTile;
   k.tiles = (int)std::max<int64_t>(1, (q.rows + k.tile_rows - 1) / k.tile_rows);
   k.chained = !whole && k.tiles > 1;
-  // (channels by 8 bytes of x: a thread then has all of its channels or none)
-  const bool whole_groups = a.channels % (kRecBytes / e) == 0;
-  auto wide = [&](const void *p, int64_t row, int64_t seq, int elem) {
-    const int bytes = kRecBytes / e * elem;
-    return whole_groups && RowsAligned(p, row, elem, bytes) && RowsAligned(nullptr, seq, elem, bytes);
+  auto plain = [&](int64_t row, int64_t seq, int elem) {
+    return (q.offsets || q.sequences <= 1 || seq == q.steps * row) && row >= 0 && row <= ((int64_t)1 << 31) / (kRecTile * elem) - kRecTile;
   };
-  k.x_wide = wide(a.x, a.x_row, a.x_seq, e);
-  k.decay_wide = wide(a.decay, a.decay_row, a.decay_seq, d);
-  k.dy_wide = wide(a.dy, a.dy_row, a.dy_seq, e);
-  auto plain = [&](bool wide, int64_t row, int64_t seq, int elem) {
-    return wide && (q.offsets || q.sequences <= 1 || seq == q.steps * row) && row >= 0 && row <= ((int64_t)1 << 31) / (kRecTile * elem) - kRecTile;
-  };
-  k.x_plain = plain(k.x_wide, a.x_row, a.x_seq, e);
-  k.decay_plain = plain(k.decay_wide, a.decay_row, a.decay_seq, d);
-  k.dy_plain = plain(k.dy_wide, a.dy_row, a.dy_seq, e);
+  k.x_plain = plain(a.x_row, a.x_seq, e);
+  k.decay_plain = plain(a.decay_row, a.decay_seq, d);
+  k.dy_plain = plain(a.dy_row, a.dy_seq, e);
   l.saved_bytes = sizeof(float) * (size_t)k.tiles * a.channels;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   size_t used = 0;
@@ -120,11 +111,6 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   if (a.per_channel) k.partial = reinterpret_cast<float *>(take(sizeof(float) * (size_t)k.tiles * a.channels));
   l.backward_bytes = used;
   return l;
-}
-
-static bool OutWide(const daliamdRecurrenceArgs &a, const void *p, int dtype) {
-  const int v = kRecBytes / ElementSize(a.dtype), elem = ElementSize(dtype);
-  return a.channels % v == 0 && RowsAligned(p, a.channels, elem, v * elem);
 }
 
 static void ClearChain(hipStream_t s, const RecLayout &l) {
@@ -159,7 +145,6 @@ daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurr
   DALIAMD_REQUIRE(workspace_bytes >= l.forward_bytes && (workspace || !l.forward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceRun: the workspace is too small");
   if (!q.sequences) return DALIAMD_SUCCESS;
-  l.k.out_wide = OutWide(*args, args->y, args->dtype);
   hipStream_t s = (hipStream_t)stream;
   if (l.initial_copy) {
     const int64_t n = (int64_t)q.sequences * args->channels;
@@ -187,8 +172,6 @@ daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const dalia
   DALIAMD_REQUIRE(workspace_bytes >= l.backward_bytes && (workspace || !l.backward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceBackwardRun: the workspace is too small");
   hipStream_t s = (hipStream_t)stream;
-  l.k.out_wide = OutWide(*args, args->dx, args->dtype);
-  l.k.decay_out_wide = OutWide(*args, args->ddecay, args->decay_dtype);
   l.k.few_steps = false;
   ClearChain(s, l);
   if (args->dtype == DALIAMD_FLOAT) LaunchRecurrenceBackward<float>(s, l.k);

@@ -10,15 +10,15 @@ template <typename XT> constexpr int RecV() { return kRecBytes / (int)sizeof(XT)
 template <typename XT> constexpr int RecChannels() { return kRecLanes * RecV<XT>(); }
 
 // The steps of a thread's stretch in a tensor, one group of channels each.  Loads are not conditional - steps behind the last row
-// read that row again, lanes without channels the first ones - because a load under a condition is waited for where the
+// read that row again, lanes without channels the last ones - because a load under a condition is waited for where the
 // condition ends: the 16 or 24 of a tile would come one after the other.  Rows: blocks of `steps` rows seq apart, or one block.
-// `plain`: a whole tile of one block whose rows can be read 8 or 16 bytes at a time: a base in scalar registers, a step per row.
+// `plain`: a whole tile of one block: a base in scalar registers, a step per row.
 template <typename T, int V>
 __device__ __forceinline__ void LoadSteps(Group<T, V> (&g)[kRecSteps], const void *base, const daliamdSequenceRows &q, int first, int stretch, int limit,
-                                          int64_t row_stride, int64_t seq_stride, int channel, int n, bool wide, bool plain) {
-  if (plain) {
+                                          int64_t row_stride, int64_t seq_stride, const Channels<V> &own, bool plain) {
+  if (plain && !own.narrow) {
     const char *p = static_cast<const char *>(base) + (int64_t)first * row_stride * (int)sizeof(T);
-    const uint32_t offset = (uint32_t)(stretch * kRecSteps * (int)row_stride + (n ? channel : 0)) * (uint32_t)sizeof(T);
+    const uint32_t offset = (uint32_t)(stretch * kRecSteps * (int)row_stride + own.base) * (uint32_t)sizeof(T);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) LoadWide(g[k], reinterpret_cast<const T *>(p + (int64_t)k * row_stride * (int)sizeof(T) + offset));
     return;
@@ -26,42 +26,14 @@ __device__ __forceinline__ void LoadSteps(Group<T, V> (&g)[kRecSteps], const voi
   const int row = min(first + stretch * kRecSteps, limit - 1);
   const int steps = (int)(q.offsets ? q.rows : q.steps), s = q.offsets ? 0 : (int)((uint32_t)row / (uint32_t)steps);
   int t = row - s * steps;
-  const T *p = static_cast<const T *>(base) + s * seq_stride + t * row_stride + (n ? channel : 0);
+  const T *p = static_cast<const T *>(base) + s * seq_stride + t * row_stride;
   const int64_t next_block = seq_stride - (steps - 1) * row_stride;
-  if (wide) {                  // (n is 0 or V)
 #pragma unroll
-    for (int k = 0; k < kRecSteps; k++) {
-      LoadWide(g[k], p);
-      const bool wrap = ++t == steps;
-      p += row + k + 1 < limit ? (wrap ? next_block : row_stride) : 0;
-      if (wrap) t = 0;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kRecSteps; k++) {
-#pragma unroll
-      for (int j = 0; j < V; j++) g[k].Set(j, p[j < n ? j : 0]);
-      const bool wrap = ++t == steps;
-      p += row + k + 1 < limit ? (wrap ? next_block : row_stride) : 0;
-      if (wrap) t = 0;
-    }
-  }
-}
-template <typename T, int V> __device__ __forceinline__ void LoadStep(Group<T, V> &g, const T *p, bool wide, int n) {
-  if (wide) {
-    LoadWide(g, p);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j++) g.Set(j, p[j < n ? j : 0]);
-  }
-}
-template <typename T, int V> __device__ __forceinline__ void StoreStep(T *p, const float *f, bool wide, int n) {
-  if (wide) {
-    StoreWide<T, V>(p, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j++)
-      if (j < n) p[j] = FromFloat<T>(f[j]);
+  for (int k = 0; k < kRecSteps; k++) {
+    own.Load(g[k], p);
+    const bool wrap = ++t == steps;
+    p += row + k + 1 < limit ? (wrap ? next_block : row_stride) : 0;
+    if (wrap) t = 0;
   }
 }
 
@@ -83,15 +55,15 @@ template <int V> struct RecFront {
 // A thread's place and the scans of its workgroup.
 template <typename XT> struct RecLane {
   static constexpr int V = RecV<XT>(), CH = RecChannels<XT>();
-  int wave, piece, lane_c, channel, n;   // n: its channels that exist
-  __device__ __forceinline__ RecLane(int channels, int channel_tile) {
+  int wave, piece, lane_c;
+  Channels<V> own;   // (where the row ends inside a group, its first channels are computed by two threads alike, and written by one)
+  __device__ __forceinline__ RecLane(int channels, int channel_tile) : own(channel_tile * CH + (int)threadIdx.x % kRecLanes * V, channels) {
     const int tid = threadIdx.x;
     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     piece = (tid & 63) / kRecLanes;
     lane_c = tid % kRecLanes * V;
-    channel = channel_tile * CH + lane_c;
-    n = min(max(channels - channel, 0), V);
   }
+  __device__ __forceinline__ bool Idle() const { return own.begin >= own.end; }
   __device__ __forceinline__ int Stretch() const { return wave * kRecPieces + piece; }
 
   // Scan over the stretches of a wave, in the order of time or (REV) against it; a, s, r: of this thread's stretch.  The wave's
@@ -163,10 +135,10 @@ __device__ __forceinline__ uint64_t Hear(const uint64_t *word) { return __hip_at
 __device__ __forceinline__ bool Said(uint64_t word) { return (word >> 32) != 0; }
 __device__ __forceinline__ float Value(uint64_t word) { return BitsToFloat((uint32_t)word); }
 
-// For one channel of the workgroup's tile: finds the state in front of the tile and says what is behind it.  a, s, r: of the
+// For one channel of the workgroup's tile (`place`: its place among all tiles' channels): finds the state in front of the tile and says what is behind it.  a, s, r: of the
 // whole tile; `known`: nothing in front counts but `state`.  Returns the state in front.
-template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int64_t channel, double a, float s, bool r, bool known, float state) {
-  uint64_t *mine = p.words + ((int64_t)tile * width + channel) * kRecWords;
+template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int place, double a, float s, bool r, bool known, float state) {
+  uint64_t *mine = p.words + ((int64_t)tile * width + place) * kRecWords;
   const bool joint = (REV ? p.tiles - 1 - tile : tile) % kRecGroup == kRecGroup - 1;
   if (r || known) {
     Say(mine, __builtin_bit_cast(uint32_t, r ? s : (float)fma(a, (double)state, (double)s)));
@@ -223,7 +195,9 @@ __device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecC
                                           const float *initial, int sequence) {
   constexpr int CH = RecChannels<XT>();
   if (threadIdx.x >= CH) return;
-  const int channel = channel_tile * CH + threadIdx.x;
+  const int first = channel_tile * CH + (int)threadIdx.x / RecV<XT>() * RecV<XT>();
+  const Channels<RecV<XT>()> own(first, p.a.channels);
+  const int channel = own.base + (int)threadIdx.x % RecV<XT>();
   double a = 1.0;
   float s = 0.0f;
   bool r = false;
@@ -238,7 +212,7 @@ __device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecC
     r |= forget;
   }
   const float state = initial && sequence >= 0 && channel < p.a.channels ? initial[(int64_t)sequence * p.a.channels + channel] : 0.0f;
-  shared.front[threadIdx.x] = p.chained ? Chain<REV>(p, tile, (int64_t)p.channel_tiles * CH, channel, a, s, r, !needs, state) : state;
+  shared.front[threadIdx.x] = p.chained ? Chain<REV>(p, tile, (int64_t)p.channel_tiles * CH, channel_tile * CH + (int)threadIdx.x, a, s, r, !needs, state) : state;
 }
 
 // the workgroup's tile: in the order of the chain
@@ -275,11 +249,11 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecDecay 
   float k_fixed[PER_CHANNEL ? V : 1];
   double a_fixed[PER_CHANNEL ? V : 1];
 
-  __device__ __forceinline__ RecDecay(const daliamdRecurrenceArgs &p, int channel, int n) {
+  __device__ __forceinline__ RecDecay(const daliamdRecurrenceArgs &p, const Channels<V> &own) {
     if (!PER_CHANNEL) return;
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const double g = j < n ? (double)LoadElement(p.decay, channel + j, p.decay_dtype) : 0.0;
+      const double g = j < own.end ? (double)LoadElement(p.decay, own.base + j, p.decay_dtype) : 0.0;
       if (FORM == DALIAMD_RECURRENCE_GATE) {
         const double t = exp(-fabs(g)), big = 1 / (1 + t);
         a_fixed[j] = g < 0 ? t * big : big;
@@ -316,27 +290,26 @@ template <typename XT, typename GT, bool PER_CHANNEL> struct RecTile {
 };
 
 template <typename XT, typename GT, bool PER_CHANNEL>
-__device__ __forceinline__ void LoadTile(RecTile<XT, GT, PER_CHANNEL> &t, const RecKernelArgs &p, int first, int stretch, int limit, int channel, int n) {
+__device__ __forceinline__ void LoadTile(RecTile<XT, GT, PER_CHANNEL> &t, const RecKernelArgs &p, int first, int stretch, int limit, const Channels<RecV<XT>()> &own) {
   constexpr int V = RecV<XT>();
   const bool full = first + kRecTile <= limit;
-  LoadSteps<XT, V>(t.x, p.a.x, p.a.seq, first, stretch, limit, p.a.x_row, p.a.x_seq, channel, n, p.x_wide, p.x_plain && full);
-  if constexpr (!PER_CHANNEL)
-    LoadSteps<GT, V>(t.g, p.a.decay, p.a.seq, first, stretch, limit, p.a.decay_row, p.a.decay_seq, channel, n, p.decay_wide, p.decay_plain && full);
+  LoadSteps<XT, V>(t.x, p.a.x, p.a.seq, first, stretch, limit, p.a.x_row, p.a.x_seq, own, p.x_plain && full);
+  if constexpr (!PER_CHANNEL) LoadSteps<GT, V>(t.g, p.a.decay, p.a.seq, first, stretch, limit, p.a.decay_row, p.a.decay_seq, own, p.decay_plain && full);
 }
 
-template <int V> __device__ __forceinline__ void LoadState(float (&h)[V], const float *state, int64_t s, int channels, int channel, int n) {
+template <int V> __device__ __forceinline__ void LoadState(float (&h)[V], const float *state, int64_t s, int channels, const Channels<V> &own) {
 #pragma unroll
-  for (int j = 0; j < V; j++) h[j] = state && j < n ? state[s * channels + channel + j] : 0.0f;
+  for (int j = 0; j < V; j++) h[j] = state && j < own.end ? state[s * channels + own.base + j] : 0.0f;
 }
-template <int V> __device__ __forceinline__ void StoreState(float *state, const float (&h)[V], int64_t s, int channels, int channel, int n) {
+template <int V> __device__ __forceinline__ void StoreState(float *state, const float (&h)[V], int64_t s, int channels, const Channels<V> &own) {
   if (!state) return;
 #pragma unroll
   for (int j = 0; j < V; j++)
-    if (j < n) state[s * channels + channel + j] = h[j];
+    if (j >= own.begin && j < own.end) state[s * channels + own.base + j] = h[j];
 }
 
 // Sequences of no steps: their state is the initial one, their initial state's gradient that of the state.
-template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &p, int tile, int stretch, int channel, int n, const float *from, float *to) {
+template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &p, int tile, int stretch, const Channels<V> &own, const float *from, float *to) {
   const daliamdSequenceRows &q = p.a.seq;
   if (!to || !(q.offsets || q.lengths || q.steps == 0)) return;
   constexpr int kStretches = kRecWaves * kRecPieces;
@@ -345,8 +318,8 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
     SequenceRange(q, (int)s, &begin, &end);
     if (begin < end) continue;
     float h[V];
-    LoadState<V>(h, from, s, p.a.channels, channel, n);
-    StoreState<V>(to, h, s, p.a.channels, channel, n);
+    LoadState<V>(h, from, s, p.a.channels, own);
+    StoreState<V>(to, h, s, p.a.channels, own);
   }
 }
 
@@ -380,8 +353,8 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 
   // (A, S, R) of a thread's stretch; `c`: the steps' coefficients for the second time
   template <bool EVENTS>
-  __device__ static __forceinline__ bool Compose(const RecKernelArgs &p, const Decay &decay, const Tile &t, const RecEvents &e, int row, int channel,
-                                                 int n, float (&c)[kRecSteps][V], double (&a)[V], float (&s)[V]) {
+  __device__ static __forceinline__ bool Compose(const RecKernelArgs &p, const Decay &decay, const Tile &t, const RecEvents &e, int row,
+                                                 const Channels<V> &own, float (&c)[kRecSteps][V], double (&a)[V], float (&s)[V]) {
 #pragma unroll
     for (int j = 0; j < V; j++) a[j] = 1.0, s[j] = 0.0f;
 #pragma unroll
@@ -390,7 +363,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
       if (EVENTS && (e.first >> k & 1)) {
         int begin, end;
         const int q = FindSequence(p.a.seq, row + k, &begin, &end);
-        LoadState<V>(s, p.a.initial, q, p.a.channels, channel, n);
+        LoadState<V>(s, p.a.initial, q, p.a.channels, own);
       }
 #pragma unroll
       for (int j = 0; j < V; j++) {
@@ -410,7 +383,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
     float c[kRecSteps][V], s[V], state[V];
     double a[V];
-    const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
+    const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
@@ -418,31 +391,31 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     const bool starts = place.sequence < 0 || place.row == place.begin;
     FindFront<false, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
     __syncthreads();
-    if (lane.n == 0) return;
+    if (lane.Idle()) return;
     float in[V];
 #pragma unroll
     for (int j = 0; j < V; j++) in[j] = shared.front[lane.lane_c + j];
-    if (p.a.saved && lane.Stretch() == 0) StoreState<V>(p.a.saved, in, tile, p.a.channels, lane.channel, lane.n);
+    if (p.a.saved && lane.Stretch() == 0) StoreState<V>(p.a.saved, in, tile, p.a.channels, lane.own);
     lane.template Start<false, EVENTS>(shared, front, in, state);
     XT *y = static_cast<XT *>(p.a.y) + (int64_t)place.row * p.a.channels;
-    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels + lane.channel);
+    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && row + k >= limit) break;
       if (EVENTS && !(e.live >> k & 1)) {
         const float zero[V] = {};
-        StoreStep<XT, V>(y + (int64_t)k * p.a.channels + offset, zero, p.out_wide, lane.n);
+        lane.own.Store(y + (int64_t)k * p.a.channels + offset, zero);
         continue;
       }
       int begin, end;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
 #pragma unroll
       for (int j = 0; j < V; j++) state[j] = Decay::Step(c[k][j], t.x[k][j], state[j]);
-      StoreStep<XT, V>(y + (int64_t)k * p.a.channels + offset, state, p.out_wide, lane.n);
-      if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
+      lane.own.Store(y + (int64_t)k * p.a.channels + offset, state);
+      if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
     }
     if (!EVENTS && place.row + kRecTile == place.end && lane.Stretch() == kRecWaves * kRecPieces - 1)
-      StoreState<V>(p.a.final_state, state, place.sequence, p.a.channels, lane.channel, lane.n);
+      StoreState<V>(p.a.final_state, state, place.sequence, p.a.channels, lane.own);
   }
 };
 
@@ -457,17 +430,17 @@ __global__ __launch_bounds__(kRecThreads, 4) void RecurrenceForwardKernel(RecKer
   const RecLane<XT> lane(p.a.channels, channel_tile);
   const RecPlace place(p, tile);
   typename Op::Tile t;
-  if (place.row < place.limit) LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.channel, lane.n);
-  const typename Op::Decay decay(p.a, lane.channel, lane.n);
+  if (place.row < place.limit) LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.own);
+  const typename Op::Decay decay(p.a, lane.own);
   if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, place, tile, channel_tile);
   else Op::template Process<true>(p, lane, shared, decay, t, place, tile, channel_tile);
-  PassEmpty<V>(p, tile, lane.Stretch(), lane.channel, lane.n, p.a.initial, p.a.final_state);
+  PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.initial, p.a.final_state);
 }
 
 // (A, S, R) of a thread's stretch against time; dy NULL: zeros
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool EVENTS>
 __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDecay<XT, GT, FORM, PER_CHANNEL> &decay, const Group<XT, RecV<XT>()> (&dy)[kRecSteps],
-                                            const float (&c)[kRecSteps][RecV<XT>()], const RecEvents &e, int row, int channel, int n,
+                                            const float (&c)[kRecSteps][RecV<XT>()], const RecEvents &e, int row, const Channels<RecV<XT>()> &own,
                                             double (&a)[RecV<XT>()], float (&s)[RecV<XT>()]) {
   constexpr int V = RecV<XT>();
 #pragma unroll
@@ -477,7 +450,7 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
     if (EVENTS && !(e.live >> k & 1)) continue;
     if (EVENTS && (e.last >> k & 1)) {
       int begin, end;
-      LoadState<V>(s, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, channel, n);
+      LoadState<V>(s, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, own);
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -503,9 +476,9 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
     float c[kRecSteps][V], s[V], state[V], back[V];
     double a[V];
-    bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.channel, lane.n, c, a, s);
+    bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
-    r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, c, e, row, lane.channel, lane.n, a, s);
+    r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, c, e, row, lane.own, a, s);
     const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
@@ -519,7 +492,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && !(e.live >> k & 1)) continue;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         const float x = t.x[k][j];
@@ -528,19 +501,19 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
       }
     }
     __syncthreads();
-    if (lane.n == 0) return;
+    if (lane.Idle()) return;
     float in[V];
 #pragma unroll
     for (int j = 0; j < V; j++) in[j] = shared[1].front[lane.lane_c + j];
     lane.template Start<true, EVENTS>(shared[1], behind, in, back);
-    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels + lane.channel);
+    const uint32_t offset = (uint32_t)(lane.Stretch() * kRecSteps * p.a.channels);
 #pragma unroll
     for (int k = kRecSteps - 1; k >= 0; k--) {
       if (EVENTS && row + k >= limit) continue;
       float dx[V] = {}, dg[V] = {};
       const bool live = !EVENTS || (e.live >> k & 1);
       if (live) {
-        if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
+        if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
 #pragma unroll
         for (int j = 0; j < V; j++) {
           const float l = back[j] + dy[k][j];
@@ -554,13 +527,13 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
           if (PER_CHANNEL) sum[j] += dg[j];
           back[j] = Decay::Back(c[k][j], l);
         }
-        if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.channel, lane.n);
+        if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
       }
       const int64_t at = (int64_t)(place.row + k) * p.a.channels;
-      StoreStep<XT, V>(static_cast<XT *>(p.a.dx) + at + offset, dx, p.out_wide, lane.n);
-      if (!PER_CHANNEL) StoreStep<GT, V>(static_cast<GT *>(p.a.ddecay) + at + offset, dg, p.decay_out_wide, lane.n);
+      lane.own.Store(static_cast<XT *>(p.a.dx) + at + offset, dx);
+      if (!PER_CHANNEL) lane.own.Store(static_cast<GT *>(p.a.ddecay) + at + offset, dg);
     }
-    if (!EVENTS && place.row == place.begin && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, place.sequence, p.a.channels, lane.channel, lane.n);
+    if (!EVENTS && place.row == place.begin && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, place.sequence, p.a.channels, lane.own);
   }
 };
 
@@ -578,9 +551,9 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
   Group<XT, V> dy[kRecSteps];
   float saved[V], sum[V] = {};
   if (place.row < place.limit) {
-    LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.channel, lane.n);
+    LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.own);
     if (p.a.dy)
-      LoadSteps<XT, V>(dy, p.a.dy, p.a.seq, place.row, lane.Stretch(), place.limit, p.a.dy_row, p.a.dy_seq, lane.channel, lane.n, p.dy_wide,
+      LoadSteps<XT, V>(dy, p.a.dy, p.a.seq, place.row, lane.Stretch(), place.limit, p.a.dy_row, p.a.dy_seq, lane.own,
                        p.dy_plain && place.row + kRecTile <= place.limit);
   }
   if (!p.a.dy) {
@@ -589,11 +562,11 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
 #pragma unroll
       for (int j = 0; j < V; j++) dy[k].Set(j, FromFloat<XT>(0.0f));
   }
-  LoadState<V>(saved, p.a.saved, tile, p.a.channels, lane.channel, lane.n);
-  const typename Op::Decay decay(p.a, lane.channel, lane.n);
+  LoadState<V>(saved, p.a.saved, tile, p.a.channels, lane.own);
+  const typename Op::Decay decay(p.a, lane.own);
   if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
   else Op::template Process<true>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
-  PassEmpty<V>(p, tile, lane.Stretch(), lane.channel, lane.n, p.a.dfinal, p.a.dinitial);
+  PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.dfinal, p.a.dinitial);
   if (PER_CHANNEL) {
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -611,7 +584,7 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
       for (int j = 0; j < V; j++) {
         float total = 0;
         for (int w = 0; w < kRecWaves; w++) total += shared[0].s[w][lane.lane_c + j];
-        if (j < lane.n) p.partial[(int64_t)tile * p.a.channels + lane.channel + j] = total;
+        if (j >= lane.own.begin && j < lane.own.end) p.partial[(int64_t)tile * p.a.channels + lane.own.base + j] = total;
       }
     }
   }
@@ -625,29 +598,34 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArg
   const int64_t id = (int64_t)blockIdx.x * kRecThreads + threadIdx.x;
   const int64_t s = (uint32_t)id / (uint32_t)groups;
   if (s >= p.a.seq.sequences) return;
+  // (a state may be written over the one it is read from: threads have no channels in common)
   const int channel = (int)(id - s * groups) * V, n = min(p.a.channels - channel, V);
-  const RecDecay<XT, GT, FORM, PER_CHANNEL> decay(p.a, channel, n);
+  Channels<V> own(channel, p.a.channels);
+  if (n < V) own.base = channel, own.begin = 0, own.end = n, own.narrow = true;
+  const RecDecay<XT, GT, FORM, PER_CHANNEL> decay(p.a, own);
   int begin, end;
   SequenceRange(p.a.seq, (int)s, &begin, &end);
-  const int64_t steps = p.a.seq.steps, length = end - begin;
+  const int steps = (int)p.a.seq.steps, length = end - begin;
   float h[V];
-  LoadState<V>(h, p.a.initial, s, p.a.channels, channel, n);
-  for (int64_t t = 0; t < steps; t++) {
-    XT *y = static_cast<XT *>(p.a.y) + (s * steps + t) * p.a.channels + channel;
+  LoadState<V>(h, p.a.initial, s, p.a.channels, own);
+  for (int t = 0; t < steps; t++) {
+    XT *y = static_cast<XT *>(p.a.y) + (s * steps + t) * p.a.channels;
     if (t < length) {
       Group<XT, V> x;
       Group<GT, V> g;
-      LoadStep<XT, V>(x, static_cast<const XT *>(p.a.x) + s * p.a.x_seq + t * p.a.x_row + channel, p.x_wide, n);
-      if (!PER_CHANNEL) LoadStep<GT, V>(g, static_cast<const GT *>(p.a.decay) + s * p.a.decay_seq + t * p.a.decay_row + channel, p.decay_wide, n);
+      const XT *px = static_cast<const XT *>(p.a.x) + s * p.a.x_seq + t * p.a.x_row;
+      const GT *pg = static_cast<const GT *>(p.a.decay) + s * p.a.decay_seq + t * p.a.decay_row;
+      own.Load(x, px + (own.narrow ? own.base : 0));
+      if (!PER_CHANNEL) own.Load(g, pg + (own.narrow ? own.base : 0));
 #pragma unroll
       for (int j = 0; j < V; j++) h[j] = RecDecay<XT, GT, FORM, PER_CHANNEL>::Step(decay.Coefficient(g, j), x[j], h[j]);
-      StoreStep<XT, V>(y, h, p.out_wide, n);
+      own.Store(y, h);
     } else {
       const float zero[V] = {};
-      StoreStep<XT, V>(y, zero, p.out_wide, n);
+      own.Store(y, zero);
     }
   }
-  StoreState<V>(p.a.final_state, h, s, p.a.channels, channel, n);
+  StoreState<V>(p.a.final_state, h, s, p.a.channels, own);
 }
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecLaunch {

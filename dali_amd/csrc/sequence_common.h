@@ -61,58 +61,83 @@ template <typename T, int V> struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) :
 #endif
   }
 };
-template <int BYTES> __device__ __forceinline__ void CopyWide(void *to, const void *from) {
-  if (BYTES % 16 == 0) {
+// Rows start wherever their elements may: the hardware takes 8 and 16 byte accesses at any address, and the types say so.
+typedef uint32_t UnalignedWords __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t UnalignedPair __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T, int V> __device__ __forceinline__ void LoadWide(Group<T, V> &g, const T *p) {
+  constexpr int kWords = Group<T, V>::kWords;
+  if constexpr (kWords % 4 == 0) {
 #pragma unroll
-    for (int k = 0; k < BYTES / 16; k++) static_cast<uint4 *>(to)[k] = static_cast<const uint4 *>(from)[k];
+    for (int k = 0; k < kWords / 4; k++) {
+      const UnalignedWords w = reinterpret_cast<const UnalignedWords *>(p)[k];
+#pragma unroll
+      for (int i = 0; i < 4; i++) g.word[4 * k + i] = w[i];
+    }
   } else {
-    *static_cast<uint2 *>(to) = *static_cast<const uint2 *>(from);
+    const UnalignedPair w = *reinterpret_cast<const UnalignedPair *>(p);
+    g.word[0] = w[0], g.word[1] = w[1];
   }
 }
-template <typename T, int V> __device__ __forceinline__ void LoadWide(Group<T, V> &g, const T *p) { CopyWide<sizeof(g)>(&g, p); }
 template <typename T, int V> __device__ __forceinline__ void StoreWide(T *p, const float *f) {
+  constexpr int kWords = Group<T, V>::kWords;
   Group<T, V> g;
 #pragma unroll
   for (int j = 0; j < V; j++) g.Set(j, FromFloat<T>(f[j]));
-  CopyWide<sizeof(g)>(p, &g);
+  if constexpr (kWords % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < kWords / 4; k++)
+      reinterpret_cast<UnalignedWords *>(p)[k] = UnalignedWords{g.word[4 * k], g.word[4 * k + 1], g.word[4 * k + 2], g.word[4 * k + 3]};
+  } else {
+    *reinterpret_cast<UnalignedPair *>(p) = UnalignedPair{g.word[0], g.word[1]};
+  }
 }
 
-// Which channels a thread of a row has, in `n` pieces of V: adjacent ones where every row of every tensor can be read 16 bytes
-// at a time (`wide`), else every `threads`-th, so that a wave's loads of single elements are adjacent.
-struct ChannelMap {
-  int channels, threads, lane;
-  bool wide;
-  template <int V> __device__ __forceinline__ int First(int i) const { return wide ? (i * threads + lane) * V : i * V * threads + lane; }
-  __device__ __forceinline__ int Step() const { return wide ? 1 : threads; }
-};
-template <typename T, int V> __device__ __forceinline__ void LoadChannels(Group<T, V> &g, const T *row, const ChannelMap &m, int i) {
-  const int c = m.First<V>(i);
-  if (m.wide) {
-    if (c < m.channels) {
-      LoadWide(g, row + c);
-      return;
+// The V channels that a thread has of a row, the `first`-th on.  Where the row ends inside them, the thread takes the row's last V
+// and leaves those out that are another thread's: every load is a whole one, and none is conditional (a load under a condition is
+// waited for where the condition ends).  Rows of fewer than V channels: one by one.
+template <int V> struct Channels {
+  int base, begin, end;   // elements [begin, end) of the V from channel `base` on are this thread's; none: begin >= end
+  bool narrow;
+  __device__ __forceinline__ Channels(int first, int channels) {
+    narrow = channels < V;
+    base = max(0, min(first, channels - V));
+    begin = first - base;
+    end = min(V, channels);
+  }
+  template <typename T> __device__ __forceinline__ void Load(Group<T, V> &g, const T *row) const {
+    if (narrow) {
+#pragma unroll
+      for (int j = 0; j < V; j++) g.Set(j, row[min(j, end - 1)]);
+    } else {
+      LoadWide(g, row + base);
     }
-#pragma unroll
-    for (int j = 0; j < V; j++) g.Set(j, FromFloat<T>(0.0f));
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j++) g.Set(j, c + j * m.threads < m.channels ? row[c + j * m.threads] : FromFloat<T>(0.0f));
   }
-}
-template <typename T, int V> __device__ __forceinline__ void StoreChannels(T *row, const ChannelMap &m, int i, const float *f) {
-  const int c = m.First<V>(i);
-  if (m.wide) {
-    if (c < m.channels) StoreWide<T, V>(row + c, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j++)
-      if (c + j * m.threads < m.channels) row[c + j * m.threads] = FromFloat<T>(f[j]);
+  // ... with zeros in the places of others
+  template <typename T> __device__ __forceinline__ void LoadOwn(Group<T, V> &g, const T *row) const {
+    Load(g, row);
+    Mask(g);
   }
-}
-// whether rows of `elem`-byte elements, `stride` elements apart, all start at multiples of `bytes` bytes
-inline bool RowsAligned(const void *p, int64_t stride, int elem, int bytes = 16) {
-  return ((reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride * elem)) & (bytes - 1)) == 0;
-}
+  template <typename T> __device__ __forceinline__ void Mask(Group<T, V> &g) const {
+#pragma unroll
+    for (int k = 0; k < Group<T, V>::kWords; k++) {
+      if constexpr (sizeof(T) == 4) {
+        g.word[k] = k >= begin && k < end ? g.word[k] : 0u;
+      } else {
+        const uint32_t low = 2 * k >= begin && 2 * k < end ? 0xffffu : 0u, high = 2 * k + 1 >= begin && 2 * k + 1 < end ? 0xffff0000u : 0u;
+        g.word[k] &= low | high;
+      }
+    }
+  }
+  template <typename T> __device__ __forceinline__ void Store(T *row, const float *f) const {
+    if (begin == 0 && end == V) {
+      StoreWide<T, V>(row + base, f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (j >= begin && j < end) row[base + j] = FromFloat<T>(f[j]);
+    }
+  }
+};
 
 __device__ __forceinline__ float LoadElement(const void *p, int64_t i, int dtype) {
   return dtype == DALIAMD_FLOAT ? static_cast<const float *>(p)[i]
@@ -160,30 +185,39 @@ __device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int ro
   return *begin <= row && row < *end ? s : -1;
 }
 
-__device__ __forceinline__ float Exp(float v) { return expf(v); }
-// f = 1 / (1 + exp(-g)) and k = 1 - f, both to the last bits: k is small where a gate holds, and it is what h moves by
-__device__ __forceinline__ void Logistic(float g, float *f, float *k) {
-  const float t = Exp(-fabsf(g)), big = 1.0f / (1.0f + t), small = t * big;
-  *f = g < 0 ? small : big;
-  *k = g < 0 ? big : small;
-}
-
-// 1 - f alone, in the instructions that the hardware has for it.  The product with log2(e) is off by 2^-24 of itself, which is
-// |g| 2^-24 of the result: EXACT puts that back.
-template <bool EXACT> __device__ __forceinline__ float OneMinusLogistic(float g) {
-  constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+// The logistic function f(g) = 1 / (1 + exp(-g)) in the instructions that the hardware has for it: 2^x and 1 / x, each good to the
+// last bit or two.  The product with log2(e) is off by 2^-24 of itself, which is |g| 2^-24 of the power; EXACT puts that back.
+template <bool EXACT> __device__ __forceinline__ float ExpOf(float g) {
 #if defined(__AMDGCN__)
+  constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
   const float p = g * kLog2e;
   float t = __builtin_amdgcn_exp2f(p);
   if (EXACT) {
     const float more = t * (fmaf(g, kLog2e, -p) * kLn2);
     t += t < __builtin_inff() ? more : 0.0f;
   }
-  return __builtin_amdgcn_rcpf(1.0f + t);
+  return t;
 #else
-  return (float)(1.0 / (1.0 + exp((double)g)));
+  return (float)exp((double)g);
 #endif
 }
+__device__ __forceinline__ float Reciprocal(float v) {
+#if defined(__AMDGCN__)
+  return __builtin_amdgcn_rcpf(v);
+#else
+  return 1.0f / v;
+#endif
+}
+// f and 1 - f, both to their last bits
+__device__ __forceinline__ void LogisticPair(float g, float *f, float *k) {
+  const float t = ExpOf<true>(-fabsf(g)), big = Reciprocal(1.0f + t), small = t * big;
+  *f = g < 0 ? small : big;
+  *k = g < 0 ? big : small;
+}
+// 1 - f alone
+template <bool EXACT> __device__ __forceinline__ float OneMinusLogistic(float g) { return Reciprocal(1.0f + ExpOf<EXACT>(g)); }
+// g f(g)
+__device__ __forceinline__ float Silu(float g) { return g * Reciprocal(1.0f + ExpOf<true>(-g)); }
 
 }  // namespace daliamd
 #endif  // DALI_AMD_CSRC_SEQUENCE_COMMON_H_
