@@ -1,314 +1,7 @@
-// What stands between two blocks of a layer: norm of the block's output, gate, scaled residual, norm before the next block.
-//   u = x rstd(x) w_post     v = u silu(g)     h = r + s v     n = h rstd(h) w_pre
-// Backward, with z^ = z rstd(z) and <.> the mean over a row's channels:
-//   dh <- dh + rstd(h) (dn w_pre - h^ <dn w_pre h^>)          dw_pre  = sum over rows of dn h^
-//   dr = dh     dv = dh s                                      ds      = sum over rows of dh v
-//   dg = dv u silu'(g)     du = dv silu(g)                     dw_post = sum over rows of du x^
-//   dx = rstd(x) (du w_post - x^ <du w_post x^>)
-#include <algorithm>
-#include "sequence_common.h"
+// C entries of the block norm: checks and workspaces; the sums over rows.  block_norm.h has the formulas.
+#include "block_norm.h"
 
 namespace daliamd {
-
-// A row's channels stay in the registers of TPR threads, NV pieces of V = 16 bytes of x each: one pass over memory, whatever
-// the number of sums.  TPR <= 64: 256 / TPR rows per workgroup, sums by shuffles inside a wave; above: one row per workgroup
-// step, sums by shuffles and one exchange through LDS.  Workgroups go through the rows with a stride; the backward pass keeps
-// its sums over rows (three weights) in registers meanwhile and leaves one partial sum per workgroup, which ColumnSumKernel
-// adds up in a fixed order.
-template <int TPR> constexpr int NormThreads() { return TPR > 256 ? TPR : 256; }
-
-// the sum over the TPR threads of a row, in each of them; `slot` alternates between calls: one barrier per sum, because a wave
-// that writes a slot again has passed the barrier behind the last reads of it
-template <int TPR> __device__ __forceinline__ float RowSum(float v, float (*shared)[TPR > 64 ? TPR / 64 : 1], int slot) {
-#pragma unroll
-  for (int off = (TPR > 64 ? 64 : TPR) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  if (TPR > 64) {
-    if ((threadIdx.x & 63) == 0) shared[slot][threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < TPR / 64; w++) v += shared[slot][w];
-  }
-  return v;
-}
-
-template <typename XT, int V> __device__ __forceinline__ void LoadWeights(float *w, const void *p, int dtype, const Channels<V> &m) {
-  if (dtype == DALIAMD_FLOAT) {
-    Group<float, V> g;
-    m.Load(g, static_cast<const float *>(p));
-#pragma unroll
-    for (int j = 0; j < V; j++) w[j] = g[j];
-  } else {
-    Group<XT, V> g;
-    m.Load(g, static_cast<const XT *>(p));
-#pragma unroll
-    for (int j = 0; j < V; j++) w[j] = g[j];
-  }
-}
-
-// A thread's weights: with one piece of the row, in registers for all rows; with more, read again (from the L1) for each row.
-template <typename XT, int V, int NV> struct NormWeights {
-  static constexpr bool kKeep = NV == 1;
-  const daliamdBlockNormArgs &p;
-  float kept[kKeep ? 3 : 1][V];
-  __device__ __forceinline__ NormWeights(const daliamdBlockNormArgs &p_, const Channels<V> &m) : p(p_) {
-    if (!kKeep) return;
-    if (p.post_weight) LoadWeights<XT, V>(kept[0], p.post_weight, p.weight_dtype, m);
-    if (p.scale) LoadWeights<XT, V>(kept[kKeep ? 1 : 0], p.scale, p.weight_dtype, m);
-    if (p.pre_weight) LoadWeights<XT, V>(kept[kKeep ? 2 : 0], p.pre_weight, p.weight_dtype, m);
-  }
-  template <int WHICH> __device__ __forceinline__ void Get(float (&w)[V], const Channels<V> &m) const {
-    if constexpr (kKeep) {
-#pragma unroll
-      for (int j = 0; j < V; j++) w[j] = kept[WHICH][j];
-    } else {
-      LoadWeights<XT, V>(w, WHICH == 0 ? p.post_weight : WHICH == 1 ? p.scale : p.pre_weight, p.weight_dtype, m);
-    }
-  }
-};
-
-template <typename XT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlockNormArgs p) {
-  constexpr int V = 16 / sizeof(XT), kRows = NormThreads<TPR>() / TPR;
-  __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
-  const int lane = (int)threadIdx.x % TPR;
-  const NormWeights<XT, V, NV> weights(p, Channels<V>(lane * V, p.channels));
-  const float inv = 1.0f / p.channels;
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = base + threadIdx.x / TPR;
-    const bool live = kRows == 1 || row < p.rows;
-    const int64_t at = live ? row : base;   // (rows of a wave that do not exist: the first one's again, not written)
-    Group<XT, V> x[NV], g[NV];
-    Group<RT, V> r[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
-      if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
-      if (p.residual) m.Load(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row);
-    }
-    float rstd = 1.0f;
-    if (p.post_weight) {
-      float sum = 0;
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        Channels<V>((i * TPR + lane) * V, p.channels).Mask(x[i]);
-#pragma unroll
-        for (int j = 0; j < V; j++) sum = fmaf(x[i][j], x[i][j], sum);
-        x[i].Repack();
-      }
-      rstd = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 0) * inv + p.eps);
-      if (p.rstd_post && lane == 0 && live) p.rstd_post[row] = rstd;
-    }
-    float h[NV][V], sum = 0;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      float post[V], scale[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        float v = x[i][j];
-        if (p.post_weight) v = v * rstd * post[j];
-        if (p.gate) v *= Silu(g[i][j]);
-        if (p.scale) v *= scale[j];
-        if (p.residual) v += r[i][j];
-        h[i][j] = v;
-        sum = j >= m.begin && j < m.end ? fmaf(v, v, sum) : sum;
-      }
-      if (live) m.Store(static_cast<RT *>(p.hidden) + row * p.channels, h[i]);
-    }
-    if (p.pre_weight) {
-      const float rstd2 = 1.0f / sqrtf(RowSum<TPR>(sum, shared, 1) * inv + p.eps);
-      if (p.rstd_pre && lane == 0 && live) p.rstd_pre[row] = rstd2;
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const Channels<V> m((i * TPR + lane) * V, p.channels);
-        float pre[V];
-        weights.template Get<2>(pre, m);
-#pragma unroll
-        for (int j = 0; j < V; j++) pre[j] = h[i][j] * rstd2 * pre[j];
-        if (live) m.Store(static_cast<XT *>(p.normed) + row * p.channels, pre);
-      }
-    }
-    if (TPR > 64 && (!p.post_weight || !p.pre_weight)) __syncthreads();   // one sum per row: the slot is written again
-  }
-}
-
-// What a row brings to its gradients, as it is in memory.
-template <typename XT, typename RT, int TPR, int NV> struct NormRow {
-  static constexpr int V = 16 / sizeof(XT);
-  Group<XT, V> x[NV], g[NV], dn[NV];
-  Group<RT, V> r[NV], dh[NV];
-  float rstd, rstd2;
-  __device__ __forceinline__ void Load(const daliamdBlockNormArgs &p, int64_t at, int lane, bool second) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
-      if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
-      if (second) {
-        m.Load(dn[i], static_cast<const XT *>(p.dnormed) + at * p.dnormed_row);
-        if (p.residual) m.Load(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row);
-      }
-      if (p.dhidden) m.Load(dh[i], static_cast<const RT *>(p.dhidden) + at * p.dhidden_row);
-    }
-    rstd = p.post_weight ? p.rstd_post[at] : 1.0f;
-    rstd2 = second ? p.rstd_pre[at] : 1.0f;
-  }
-  // zeros for what is another thread's: it then adds nothing to any sum
-  __device__ __forceinline__ void Mask(const daliamdBlockNormArgs &p, int lane, bool second) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      if (second) m.Mask(dn[i]);
-      if (p.dhidden) m.Mask(dh[i]);
-      m.Mask(x[i]);
-    }
-  }
-  __device__ __forceinline__ void Repack() {
-#pragma unroll
-    for (int i = 0; i < NV; i++) x[i].Repack(), g[i].Repack(), dn[i].Repack();
-  }
-};
-
-// partial: [gridDim.x][3][channels], sums of the workgroup's rows for post_weight, scale and pre_weight
-template <typename XT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, float *partial) {
-  constexpr int V = 16 / sizeof(XT), kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
-  __shared__ float shared[2][TPR > 64 ? TPR / 64 : 1];
-  const int lane = (int)threadIdx.x % TPR;
-  const NormWeights<XT, V, NV> weights(p, Channels<V>(lane * V, p.channels));
-  const float inv = 1.0f / p.channels;
-  const bool second = p.pre_weight && p.dnormed;
-  float apost[NV][V] = {}, ascale[NV][V] = {}, apre[NV][V] = {};
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = base + threadIdx.x / TPR;
-    const bool live = kRows == 1 || row < p.rows;
-    NormRow<XT, RT, TPR, NV> t;
-    t.Load(p, live ? row : base, lane, second);
-    t.Mask(p, lane, second);
-    const float rstd = t.rstd, rstd2 = t.rstd2;
-    // v, and with the second norm h^ and the mean of dn w_pre h^
-    float v[NV][V], hat[NV][V], mean2 = 0;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      float post[V], scale[V], pre[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
-      if (second) weights.template Get<2>(pre, m);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        float e = t.x[i][j];
-        if (p.post_weight) e = e * rstd * post[j];
-        if (p.gate) e *= Silu(t.g[i][j]);
-        v[i][j] = e;
-        if (second) {
-          if (p.scale) e *= scale[j];
-          if (p.residual) e += t.r[i][j];
-          e *= rstd2;
-          hat[i][j] = e;
-          mean2 = fmaf(t.dn[i][j] * pre[j], e, mean2);
-        }
-      }
-    }
-    if (second) mean2 = RowSum<TPR>(mean2, shared, 0) * inv;
-    t.Repack();
-    float d[NV][V], mean1 = 0;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      float post[V], scale[V], pre[V], dgate[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
-      if (second) weights.template Get<2>(pre, m);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        float e = p.dhidden ? t.dh[i][j] : 0.0f;
-        if (second) {
-          e += rstd2 * (t.dn[i][j] * pre[j] - hat[i][j] * mean2);
-          apre[i][j] = fmaf(live ? t.dn[i][j] : 0.0f, hat[i][j], apre[i][j]);
-        }
-        d[i][j] = e;
-        ascale[i][j] = fmaf(live ? e : 0.0f, v[i][j], ascale[i][j]);
-      }
-      if (p.residual && live) m.Store(static_cast<RT *>(p.dresidual) + row * p.channels, d[i]);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        float e = d[i][j];
-        if (p.scale) e *= scale[j];
-        const float hat1 = t.x[i][j] * rstd;
-        if (p.gate) {
-          float f, k;
-          const float gg = t.g[i][j];
-          LogisticPair(gg, &f, &k);
-          dgate[j] = e * (p.post_weight ? hat1 * post[j] : hat1) * (f * fmaf(gg, k, 1.0f));
-          e *= gg * f;
-        }
-        if (p.post_weight) {
-          apost[i][j] = fmaf(live ? e : 0.0f, hat1, apost[i][j]);
-          e *= post[j];
-          mean1 = fmaf(e, hat1, mean1);
-        }
-        d[i][j] = e;
-      }
-      if (p.gate && live) m.Store(static_cast<XT *>(p.dgate) + row * p.channels, dgate);
-    }
-    if (p.post_weight) {
-      mean1 = RowSum<TPR>(mean1, shared, 1) * inv;
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) d[i][j] = rstd * (d[i][j] - t.x[i][j] * rstd * mean1);
-    }
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < NV; i++) Channels<V>((i * TPR + lane) * V, p.channels).Store(static_cast<XT *>(p.dx) + row * p.channels, d[i]);
-    }
-    if (TPR > 64 && (!p.post_weight || !second)) __syncthreads();
-  }
-  if (!partial) return;
-  float *out = partial + (int64_t)blockIdx.x * 3 * p.channels;
-  if (kRows == 1) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      if (p.post_weight) m.Store(out, apost[i]);
-      if (p.scale) m.Store(out + p.channels, ascale[i]);
-      if (p.pre_weight) m.Store(out + 2 * p.channels, apre[i]);
-    }
-  } else {
-    // the threads with the same channels in all rows of the workgroup: the first row's adds them up
-    __shared__ float rows[3][kRows > 1 ? kThreads : 1];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const Channels<V> m((i * TPR + lane) * V, p.channels);
-      float post[V], scale[V], pre[V];
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        __syncthreads();
-        rows[0][threadIdx.x] = apost[i][j];
-        rows[1][threadIdx.x] = ascale[i][j];
-        rows[2][threadIdx.x] = apre[i][j];
-        __syncthreads();
-        post[j] = scale[j] = pre[j] = 0;
-        if (threadIdx.x < TPR)
-          for (int k = 0; k < kRows; k++) {
-            post[j] += rows[0][k * TPR + threadIdx.x];
-            scale[j] += rows[1][k * TPR + threadIdx.x];
-            pre[j] += rows[2][k * TPR + threadIdx.x];
-          }
-      }
-      if (threadIdx.x < TPR) {
-        if (p.post_weight) m.Store(out, post);
-        if (p.scale) m.Store(out + p.channels, scale);
-        if (p.pre_weight) m.Store(out + 2 * p.channels, pre);
-      }
-    }
-  }
-}
 
 // the sum of each column of `partial`, in a fixed order: kParts threads take every kParts-th row, then one adds them up
 constexpr int kSumColumns = 64, kSumParts = 16;
@@ -331,10 +24,6 @@ __global__ __launch_bounds__(kSumColumns * kSumParts) void BlockNormWeightsKerne
   }
 }
 
-// workgroups of the backward pass, at most: enough to fill the card, few enough that their partial sums are a small part of
-// what it moves
-static int64_t BackwardWorkgroups(int64_t rows) { return rows < 768 ? rows : 768; }
-
 static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdBlockNormPlan *plan) {
   DALIAMD_REQUIRE(args, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNorm: NULL argument");
   const daliamdBlockNormArgs &a = *args;
@@ -347,44 +36,8 @@ static daliamdResult_t CheckBlockNorm(const daliamdBlockNormArgs *args, daliamdB
   DALIAMD_REQUIRE(!(a.post_weight || a.scale || a.pre_weight) || a.weight_dtype == a.dtype || a.weight_dtype == DALIAMD_FLOAT, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdBlockNorm: the weights must have x's type or be FLOAT");
   DALIAMD_REQUIRE(a.eps >= 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNorm: eps must not be negative");
-  plan->backward_workspace_bytes = sizeof(float) * 3 * (size_t)BackwardWorkgroups(a.rows) * a.channels;
+  plan->backward_workspace_bytes = sizeof(float) * 3 * (size_t)BackwardWorkgroups(a.rows, a.channels) * a.channels;
   return DALIAMD_SUCCESS;
-}
-
-template <typename XT, typename RT, int TPR, int NV> struct NormLaunch {
-  static constexpr int kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
-  static void Forward(hipStream_t s, const daliamdBlockNormArgs &a) {
-    const int64_t groups = std::min<int64_t>((a.rows + kRows - 1) / kRows, 1 << 20);
-    KernelTimer timer("BlockNormKernel", s);
-    hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV>), dim3((unsigned)groups), dim3(kThreads), 0, s, a);
-  }
-  static void Backward(hipStream_t s, const daliamdBlockNormArgs &a, float *partial, int *count) {
-    const int64_t groups = (a.rows + kRows - 1) / kRows;
-    *count = (int)(groups < BackwardWorkgroups(a.rows) ? groups : BackwardWorkgroups(a.rows));
-    KernelTimer timer("BlockNormBackwardKernel", s);
-    hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV>), dim3((unsigned)*count), dim3(kThreads), 0, s, a, partial);
-  }
-};
-
-// the number of threads per row and pieces per thread: the fewest that hold the row
-template <typename XT, typename RT, typename F> static void WithShape(int channels, F f) {
-  const int pieces = (channels + 16 / (int)sizeof(XT) - 1) / (16 / (int)sizeof(XT));
-  if (pieces <= 8) f(NormLaunch<XT, RT, 8, 1>());
-  else if (pieces <= 16) f(NormLaunch<XT, RT, 16, 1>());
-  else if (pieces <= 32) f(NormLaunch<XT, RT, 32, 1>());
-  else if (pieces <= 64) f(NormLaunch<XT, RT, 64, 1>());
-  else if (pieces <= 128) f(NormLaunch<XT, RT, 64, 2>());
-  else if (pieces <= 256) f(NormLaunch<XT, RT, 256, 1>());
-  else if (pieces <= 512) f(NormLaunch<XT, RT, 256, 2>());
-  else if (pieces <= 1024) f(NormLaunch<XT, RT, 1024, 1>());
-  else if (pieces <= 2048) f(NormLaunch<XT, RT, 1024, 2>());
-  else f(NormLaunch<XT, RT, 1024, 4>());
-}
-template <typename F> static void WithTypes(const daliamdBlockNormArgs &a, F f) {
-  const bool wide_residual = a.residual && a.residual_dtype == DALIAMD_FLOAT;
-  if (a.dtype == DALIAMD_FLOAT) WithShape<float, float>(a.channels, f);
-  else if (a.dtype == DALIAMD_FLOAT16) wide_residual ? WithShape<F16, float>(a.channels, f) : WithShape<F16, F16>(a.channels, f);
-  else wide_residual ? WithShape<Bf16, float>(a.channels, f) : WithShape<Bf16, Bf16>(a.channels, f);
 }
 
 }  // namespace daliamd
@@ -404,7 +57,9 @@ daliamdResult_t daliamdBlockNormRun(daliamdStream_t stream, const daliamdBlockNo
   DALIAMD_REQUIRE(args->x && args->hidden && (!args->pre_weight || args->normed), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdBlockNormRun: NULL tensor");
   hipStream_t s = (hipStream_t)stream;
-  WithTypes(*args, [&](auto launch) { launch.Forward(s, *args); });
+  if (args->dtype == DALIAMD_FLOAT) LaunchBlockNorm<float>(s, *args);
+  else if (args->dtype == DALIAMD_FLOAT16) LaunchBlockNorm<F16>(s, *args);
+  else LaunchBlockNorm<Bf16>(s, *args);
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;
 }
@@ -424,7 +79,11 @@ daliamdResult_t daliamdBlockNormBackwardRun(daliamdStream_t stream, const daliam
   const bool weights = a.post_weight || a.scale || a.pre_weight;
   float *partial = weights ? static_cast<float *>(workspace) : nullptr;
   int count = 0;
-  if (a.rows) WithTypes(a, [&](auto launch) { launch.Backward(s, a, partial, &count); });
+  if (a.rows) {
+    if (a.dtype == DALIAMD_FLOAT) LaunchBlockNormBackward<float>(s, a, partial, &count);
+    else if (a.dtype == DALIAMD_FLOAT16) LaunchBlockNormBackward<F16>(s, a, partial, &count);
+    else LaunchBlockNormBackward<Bf16>(s, a, partial, &count);
+  }
   if (weights) {
     KernelTimer timer("BlockNormWeightsKernel", s);
     hipLaunchKernelGGL(BlockNormWeightsKernel, dim3((a.channels + kSumColumns - 1) / kSumColumns, 3), dim3(kSumColumns * kSumParts), 0, s, a,

@@ -7,25 +7,28 @@ namespace daliamd {
 // TPR threads per row, 8 channels per thread and step; kTokens rows per thread, whose loads are all in flight at once.
 constexpr int kEmbThreads = 256, kEmbV = 8;
 
-template <typename TT, typename OT, int kTokens>
+template <typename TT, typename OT, typename IT, int kTokens, bool WHOLE>
 __global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingArgs p, int tpr) {
   const int64_t first = ((int64_t)blockIdx.x * (kEmbThreads / tpr) + threadIdx.x / tpr) * kTokens;
-  int64_t row[kTokens];
+  if (first >= p.tokens) return;
+  const TT *row[kTokens];
+  bool inside[kTokens];
 #pragma unroll
   for (int k = 0; k < kTokens; k++) {
-    const int64_t id = first + k < p.tokens ? LoadIndex(p.ids, first + k, p.index_dtype) : -1;
-    row[k] = id >= 0 && id < p.vocab ? id : -1;
+    const int64_t id = static_cast<const IT *>(p.ids)[min(first + k, p.tokens - 1)];
+    inside[k] = id >= 0 && id < p.vocab;
+    row[k] = static_cast<const TT *>(p.table) + (inside[k] ? id : 0) * p.table_row;
   }
   for (int c = (int)threadIdx.x % tpr * kEmbV; c < p.channels; c += tpr * kEmbV) {
-    const Channels<kEmbV> m(c, p.channels);
+    const Channels<kEmbV, WHOLE> m(c, p.channels);
     Group<TT, kEmbV> g[kTokens];
 #pragma unroll
-    for (int k = 0; k < kTokens; k++) m.Load(g[k], static_cast<const TT *>(p.table) + max(row[k], (int64_t)0) * p.table_row);
+    for (int k = 0; k < kTokens; k++) m.Load(g[k], row[k]);
 #pragma unroll
     for (int k = 0; k < kTokens; k++) {
       float v[kEmbV];
 #pragma unroll
-      for (int j = 0; j < kEmbV; j++) v[j] = row[k] >= 0 ? g[k][j] * p.scale : 0.0f;
+      for (int j = 0; j < kEmbV; j++) v[j] = inside[k] ? g[k][j] * p.scale : 0.0f;
       if (first + k < p.tokens) m.Store(static_cast<OT *>(p.out) + (first + k) * p.channels, v);
     }
   }
@@ -226,7 +229,7 @@ __device__ __forceinline__ int64_t LowerBound(const uint32_t *keys, int64_t n, u
   return lo;
 }
 
-template <typename TT, typename OT>
+template <typename TT, typename OT, bool WHOLE>
 __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEmbeddingArgs p, EmbSums s) {
   const int64_t n = p.tokens;
   if ((int)blockIdx.x >= s.chunk_groups) {   // rows without a token
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     const float zero[kEmbV] = {};
     for (uint64_t mask = empty; mask; mask &= mask - 1) {
       TT *out = static_cast<TT *>(p.dtable) + (row + __ffsll((unsigned long long)mask) - 1) * p.channels;
-      for (int c = (int)threadIdx.x * kEmbV; c < p.channels; c += kEmbThreads * kEmbV) Channels<kEmbV>(c, p.channels).Store(out, zero);
+      for (int c = (int)threadIdx.x * kEmbV; c < p.channels; c += kEmbThreads * kEmbV) Channels<kEmbV, WHOLE>(c, p.channels).Store(out, zero);
     }
     return;
   }
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
   const bool goes_on = end < n && s.key[end] == s.key[end - 1];
   constexpr int kAhead = 8;   // rows in flight
   for (int c = (int)threadIdx.x % s.tpr * kEmbV; c < p.channels; c += s.tpr * kEmbV) {
-    const Channels<kEmbV> m(c, p.channels);
+    const Channels<kEmbV, WHOLE> m(c, p.channels);
     float sum[kEmbV] = {};
     uint32_t run = s.key[begin];
     bool first = true;        // the chunk's first run
@@ -395,15 +398,26 @@ template <typename TT, typename OT> struct EmbLaunch {
     const int64_t per_group = kEmbThreads / tpr;
     KernelTimer timer("EmbeddingKernel", s);
     // four rows per thread where that still leaves workgroups for every compute unit
-    if (a.tokens >= 4 * per_group * 1024)
-      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 4>), dim3((unsigned)((a.tokens + 4 * per_group - 1) / (4 * per_group))), dim3(kEmbThreads), 0, s, a, tpr);
-    else
-      hipLaunchKernelGGL((EmbeddingKernel<TT, OT, 1>), dim3((unsigned)((a.tokens + per_group - 1) / per_group)), dim3(kEmbThreads), 0, s, a, tpr);
+    if (a.tokens >= 4 * per_group * 1024) ForwardOf<4>(s, a, tpr, (a.tokens + 4 * per_group - 1) / (4 * per_group));
+    else ForwardOf<1>(s, a, tpr, (a.tokens + per_group - 1) / per_group);
+  }
+  template <int kTokens> static void ForwardOf(hipStream_t s, const daliamdEmbeddingArgs &a, int tpr, int64_t groups) {
+    const dim3 grid((unsigned)groups), block(kEmbThreads);
+    const bool whole = a.channels % kEmbV == 0;
+    if (a.index_dtype == DALIAMD_INT64) {
+      if (whole) hipLaunchKernelGGL((EmbeddingKernel<TT, OT, int64_t, kTokens, true>), grid, block, 0, s, a, tpr);
+      else hipLaunchKernelGGL((EmbeddingKernel<TT, OT, int64_t, kTokens, false>), grid, block, 0, s, a, tpr);
+    } else {
+      if (whole) hipLaunchKernelGGL((EmbeddingKernel<TT, OT, int32_t, kTokens, true>), grid, block, 0, s, a, tpr);
+      else hipLaunchKernelGGL((EmbeddingKernel<TT, OT, int32_t, kTokens, false>), grid, block, 0, s, a, tpr);
+    }
   }
   static void Backward(hipStream_t s, const daliamdEmbeddingArgs &a, const EmbSums &sums) {
     const int64_t fill = (a.vocab + kFillRows - 1) / kFillRows;
+    const dim3 grid((unsigned)(sums.chunk_groups + fill)), block(kEmbThreads);
     KernelTimer timer("EmbeddingBackwardKernel", s);
-    hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT>), dim3((unsigned)(sums.chunk_groups + fill)), dim3(kEmbThreads), 0, s, a, sums);
+    if (a.channels % kEmbV == 0) hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, true>), grid, block, 0, s, a, sums);
+    else hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, false>), grid, block, 0, s, a, sums);
   }
 };
 template <typename F> static void WithTypes(const daliamdEmbeddingArgs &a, F f) {

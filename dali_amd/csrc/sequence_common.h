@@ -95,11 +95,13 @@ template <typename T, int V> __device__ __forceinline__ void StoreWide(T *p, con
 // The V channels that a thread has of a row, the `first`-th on.  Where the row ends inside them, the thread takes the row's last V
 // and leaves those out that are another thread's: every load is a whole one, and none is conditional (a load under a condition is
 // waited for where the condition ends).  Rows of fewer than V channels: one by one.
-template <int V> struct Channels {
+// WHOLE: the row's channels are a multiple of V; a thread has V of them or none.  Then stores need no second path either, whose
+// branches would make the compiler wait for all memory operations in front of them.
+template <int V, bool WHOLE = false> struct Channels {
   int base, begin, end;   // elements [begin, end) of the V from channel `base` on are this thread's; none: begin >= end
   bool narrow;
   __device__ __forceinline__ Channels(int first, int channels) {
-    narrow = channels < V;
+    narrow = !WHOLE && channels < V;
     base = max(0, min(first, channels - V));
     begin = first - base;
     end = min(V, channels);
@@ -120,7 +122,9 @@ template <int V> struct Channels {
   template <typename T> __device__ __forceinline__ void Mask(Group<T, V> &g) const {
 #pragma unroll
     for (int k = 0; k < Group<T, V>::kWords; k++) {
-      if constexpr (sizeof(T) == 4) {
+      if constexpr (WHOLE) {
+        g.word[k] = begin == 0 ? g.word[k] : 0u;
+      } else if constexpr (sizeof(T) == 4) {
         g.word[k] = k >= begin && k < end ? g.word[k] : 0u;
       } else {
         const uint32_t low = 2 * k >= begin && 2 * k < end ? 0xffffu : 0u, high = 2 * k + 1 >= begin && 2 * k + 1 < end ? 0xffff0000u : 0u;
@@ -129,7 +133,9 @@ template <int V> struct Channels {
     }
   }
   template <typename T> __device__ __forceinline__ void Store(T *row, const float *f) const {
-    if (begin == 0 && end == V) {
+    if constexpr (WHOLE) {
+      if (begin == 0) StoreWide<T, V>(row + base, f);
+    } else if (begin == 0 && end == V) {
       StoreWide<T, V>(row + base, f);
     } else {
 #pragma unroll
