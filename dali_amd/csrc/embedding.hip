@@ -207,16 +207,16 @@ __global__ __launch_bounds__(kSmallThreads) void SortSmallKernel(daliamdEmbeddin
 }
 
 // ---- sums of the sorted tokens' gradients --------------------------------------------------------------------------------
-// The sorted tokens are cut into chunks of kChunk, whatever their ids: a token that fills half a batch is as much work per
+// The sorted tokens are cut into chunks of 8 to 32, whatever their ids: a token that fills half a batch is as much work per
 // workgroup as rare ones.  A chunk adds up each run of equal ids in it.  A run that lies within a chunk is a row of the result; of
 // one that goes on, each chunk leaves its part, and EmbeddingJoinKernel adds those of one run in their order.  Rows without a
 // token are filled with zeros by further workgroups of the same launch.
-constexpr int kChunk = 32, kFillRows = 64;
+constexpr int kFillRows = 64;
 
 struct EmbSums {
   const uint32_t *key, *index;
-  float *part;                  // [chunks][2][channels]: of the run that came from the chunk before, of the one that goes on behind
-  int chunks, chunk_groups, tpr;
+  float *part;                  // [chunks][2][part_row]: of the run that came from the chunk before, of the one that goes on behind
+  int chunk, chunks, chunk_groups, tpr, part_row;
 };
 
 // the first place whose key is not below `key`
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     return;
   }
   const int64_t chunk = (int64_t)blockIdx.x * (kEmbThreads / s.tpr) + threadIdx.x / s.tpr;
-  const int64_t begin = chunk * kChunk, end = min(begin + kChunk, n);
+  const int64_t begin = chunk * s.chunk, end = min(begin + s.chunk, n);
   if (begin >= end) return;
   const uint32_t vocab = (uint32_t)p.vocab;
   const bool from_before = begin > 0 && s.key[begin - 1] == s.key[begin];
@@ -267,24 +267,29 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     bool first = true;        // the chunk's first run
     for (int64_t t0 = begin; t0 < end && s.key[t0] < vocab; t0 += kAhead) {
       Group<OT, kEmbV> g[kAhead];
-      uint32_t key[kAhead];
+      uint32_t key[kAhead], token[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; a++) {
-        key[a] = t0 + a < end ? s.key[t0 + a] : vocab;
-        const int64_t token = key[a] < vocab ? s.index[t0 + a] : 0;
-        m.Load(g[a], static_cast<const OT *>(p.dout) + token * p.dout_row);
+        const int64_t at = min(t0 + a, end - 1);
+        key[a] = s.key[at];
+        token[a] = s.index[at];
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        m.Load(g[a], static_cast<const OT *>(p.dout) + (int64_t)token[a] * p.dout_row);
+        if (t0 + a >= end) key[a] = vocab;
       }
 #pragma unroll
       for (int a = 0; a < kAhead; a++) {
         if (key[a] != run && run < vocab) {   // a run ends, not the chunk's last
           if (first && from_before) {
-            m.Store(s.part + chunk * 2 * p.channels, sum);
+            m.Store(s.part + chunk * 2 * s.part_row, sum);
           } else if (t0 + a < end || !goes_on) {
 #pragma unroll
             for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
             m.Store(static_cast<TT *>(p.dtable) + (int64_t)run * p.channels, sum);
           } else {
-            m.Store(s.part + (chunk * 2 + 1) * p.channels, sum);
+            m.Store(s.part + (chunk * 2 + 1) * s.part_row, sum);
           }
           first = false;
 #pragma unroll
@@ -299,9 +304,9 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     }
     if (run < vocab) {        // the chunk's last token was the last of a group of kAhead
       if (first && from_before) {
-        m.Store(s.part + chunk * 2 * p.channels, sum);
+        m.Store(s.part + chunk * 2 * s.part_row, sum);
       } else if (goes_on) {
-        m.Store(s.part + (chunk * 2 + 1) * p.channels, sum);
+        m.Store(s.part + (chunk * 2 + 1) * s.part_row, sum);
       } else {
 #pragma unroll
         for (int j = 0; j < kEmbV; j++) sum[j] *= p.scale;
@@ -315,37 +320,39 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
 // nothing to do or two or three parts: small ones, so that a frequent token's long run is the only one that takes time.
 constexpr int kJoinLanes = 64, kJoinParts = 4, kJoinColumns = kJoinLanes * 4;
 __global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(daliamdEmbeddingArgs p, EmbSums s) {
-  __shared__ float part[kJoinParts][kJoinColumns];
-  const int64_t chunk = blockIdx.x, begin = chunk * kChunk, end = begin + kChunk;
+  __shared__ float4 part[kJoinParts][kJoinLanes];
+  const int64_t chunk = blockIdx.x, begin = chunk * s.chunk, end = begin + s.chunk;
   if (end >= p.tokens || s.key[end] != s.key[end - 1]) return;                  // nothing goes on behind this chunk
   const uint32_t key = s.key[end - 1];
   if (key >= (uint32_t)p.vocab) return;
   if (begin > 0 && s.key[begin - 1] == key) return;                             // it began in a chunk before
-  const int64_t last = (LowerBound(s.key, p.tokens, key + 1) - 1) / kChunk;     // the chunk that the run ends in
+  const int64_t last = (LowerBound(s.key, p.tokens, key + 1) - 1) / s.chunk;     // the chunk that the run ends in
   const int lane = threadIdx.x % kJoinLanes, k = threadIdx.x / kJoinLanes;
   const int64_t count = last - chunk, each = (count + kJoinParts - 1) / kJoinParts;
   const int64_t from = chunk + 1 + k * each, to = min(from + each, last + 1);
   for (int c0 = blockIdx.y * kJoinColumns; c0 < p.channels; c0 += gridDim.y * kJoinColumns) {
-    const Channels<4> m(c0 + lane * 4, p.channels);
-    float sum[4] = {};
-    Group<float, 4> g;
-    if (k == 0) {
-      m.Load(g, s.part + (chunk * 2 + 1) * p.channels);
-      for (int j = 0; j < 4; j++) sum[j] = g[j];
-    }
+    const int c = c0 + lane * 4;
+    const float4 *parts = reinterpret_cast<const float4 *>(s.part + min(c, s.part_row - 4));   // (rows of parts are a multiple of 4 long)
+    const int64_t row = s.part_row / 4;
+    float4 sum = make_float4(0, 0, 0, 0);
+    if (k == 0) sum = parts[(chunk * 2 + 1) * row];
 #pragma unroll 8
     for (int64_t n = from; n < to; n++) {
-      m.Load(g, s.part + n * 2 * p.channels);
-      for (int j = 0; j < 4; j++) sum[j] += g[j];
+      const float4 v = parts[n * 2 * row];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     __syncthreads();
-    for (int j = 0; j < 4; j++) part[k][lane * 4 + j] = sum[j];
+    part[k][lane] = sum;
     __syncthreads();
-    if (k == 0)
-      for (int j = 0; j < 4; j++) {
-        for (int n = 1; n < kJoinParts; n++) sum[j] += part[n][lane * 4 + j];
-        if (j >= m.begin && j < m.end) StoreElement(p.dtable, (int64_t)key * p.channels + m.base + j, p.dtype, sum[j] * p.scale);
+    if (k == 0) {
+      for (int n = 1; n < kJoinParts; n++) {
+        const float4 v = part[n][lane];
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
+      const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+      for (int j = 0; j < 4; j++)
+        if (c + j < p.channels) StoreElement(p.dtable, (int64_t)key * p.channels + c + j, p.dtype, f[j] * p.scale);
+    }
   }
 }
 
@@ -370,9 +377,13 @@ static EmbLayout LayOut(const daliamdEmbeddingArgs &a, void *workspace) {
     s.tile = ((a.tokens + kMaxTiles - 1) / kMaxTiles + kSortThreads - 1) / kSortThreads * kSortThreads;
   s.tiles = (int)((a.tokens + s.tile - 1) / s.tile);
   EmbSums &u = l.sums;
-  u.chunks = (int)((a.tokens + kChunk - 1) / kChunk);
   u.tpr = 8;
   while (u.tpr < kEmbThreads && u.tpr * kEmbV < a.channels) u.tpr *= 2;
+  // Long chunks leave fewer parts, short ones more workgroups: the longest that still gives every compute unit four.
+  u.chunk = 32;
+  while (u.chunk > 8 && a.tokens / u.chunk / (kEmbThreads / u.tpr) < 1024) u.chunk /= 2;
+  u.chunks = (int)((a.tokens + u.chunk - 1) / u.chunk);
+  u.part_row = (a.channels + 3) / 4 * 4;
   u.chunk_groups = (u.chunks + kEmbThreads / u.tpr - 1) / (kEmbThreads / u.tpr);
   uint8_t *at = static_cast<uint8_t *>(workspace);
   auto take = [&](size_t bytes) {
@@ -385,7 +396,7 @@ static EmbLayout LayOut(const daliamdEmbeddingArgs &a, void *workspace) {
     s.index[k] = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t) * (size_t)a.tokens));
   }
   s.count = reinterpret_cast<uint32_t *>(take(sizeof(uint32_t) * kDigits * (size_t)s.tiles));
-  u.part = reinterpret_cast<float *>(take(sizeof(float) * 2 * (size_t)u.chunks * a.channels));
+  u.part = reinterpret_cast<float *>(take(sizeof(float) * 2 * (size_t)u.chunks * u.part_row));
   u.key = s.key[s.passes & 1];
   u.index = s.index[s.passes & 1];
   return l;

@@ -228,18 +228,95 @@ template <bool REV> __device__ __forceinline__ void TakeTile(const RecKernelArgs
   if (REV) *tile = p.tiles - 1 - *tile;
 }
 
-// Where sequences begin and end in a thread's stretch: bit k belongs to its k-th step.
-struct RecEvents { uint32_t live, first, last; };
-__device__ __forceinline__ RecEvents FindEvents(const daliamdSequenceRows &q, int row, int limit, int begin, int end) {
-  RecEvents e = {0, 0, 0};
-  for (int k = 0; k < kRecSteps && row + k < limit; k++) {
-    const int at = row + k;
-    if (at < begin || at >= end)
-      if (FindSequence(q, at, &begin, &end) < 0) continue;
-    e.live |= 1u << k;
-    e.first |= (uint32_t)(at == begin) << k;
-    e.last |= (uint32_t)(at == end - 1) << k;
+// Where sequences begin and end in a tile, by row: the sequence, or -1.
+struct RecMarks {
+  int first[kRecTile], last[kRecTile];
+  uint8_t live[kRecTile];
+};
+// ... in a thread's stretch: bit k belongs to its k-th step.
+struct RecEvents {
+  uint32_t live, first, last;
+  const int *first_of, *last_of;
+};
+
+// The last sequence that begins at or before `row` (0 if none does), found by a whole wave: 64 places at a time.
+__device__ __forceinline__ int FindInWave(const daliamdSequenceRows &q, int row) {
+  const int lane = threadIdx.x & 63;
+  int base = 0, count = q.sequences;
+  while (count > 1) {
+    const int stride = (count + 63) / 64, at = lane * stride;
+    const bool before = at < count && LoadIndex(q.offsets, base + min(at, count - 1), q.index_dtype) <= row;
+    const int found = __popcll(__ballot(before));
+    if (found == 0) break;
+    base += (found - 1) * stride;
+    count = min(stride, count - (found - 1) * stride);
   }
+  return base;
+}
+
+// What a workgroup knows of its rows: those of one sequence alone, or not.
+struct RecPlace {
+  int row, limit, begin, end, sequence, near;   // (the same in every thread)  near: packed, a sequence not behind the first row's
+  bool interior;
+  __device__ __forceinline__ RecPlace(const RecKernelArgs &p, int tile) {
+    row = tile * p.tile_rows;
+    limit = min(row + p.tile_rows, (int)p.a.seq.rows);
+  }
+  __device__ __forceinline__ void Find(const RecKernelArgs &p) {
+    const daliamdSequenceRows &q = p.a.seq;
+    begin = end = near = 0;
+    sequence = -1;
+    if (row < limit) {
+      near = q.offsets ? FindInWave(q, row) : row / (int)q.steps;
+      SequenceRange(q, near, &begin, &end);
+      begin = __builtin_amdgcn_readfirstlane(begin);
+      end = __builtin_amdgcn_readfirstlane(end);
+      near = __builtin_amdgcn_readfirstlane(near);
+      if (begin <= row && row < end) sequence = near;
+    }
+    interior = sequence >= 0 && row + kRecTile <= min(end, limit);
+  }
+};
+
+// Fills the marks of a tile that is not interior; all threads of the workgroup.
+__device__ __forceinline__ void Mark(const RecKernelArgs &p, const RecPlace &place, RecMarks &marks) {
+  const daliamdSequenceRows &q = p.a.seq;
+  const int tid = threadIdx.x, row = place.row + tid;
+  static_assert(kRecThreads >= kRecTile, "a thread per row");
+  if (q.offsets) {
+    if (tid < kRecTile) {
+      marks.first[tid] = marks.last[tid] = -1;
+      marks.live[tid] = row < place.limit && row >= ClampRow(LoadIndex(q.offsets, 0, q.index_dtype), q.rows) &&
+                        row < ClampRow(LoadIndex(q.offsets, q.sequences, q.index_dtype), q.rows);
+    }
+    __syncthreads();
+    for (int s = place.near + tid; s < q.sequences && place.row < place.limit; s += kRecThreads) {
+      int begin, end;
+      SequenceRange(q, s, &begin, &end);
+      if (begin >= place.limit) break;
+      if (begin == end) continue;
+      if (begin >= place.row) marks.first[begin - place.row] = s;
+      if (end > place.row && end <= place.limit) marks.last[end - 1 - place.row] = s;
+    }
+  } else if (tid < kRecTile) {
+    int begin = 0, end = 0;
+    const int s = row < place.limit ? FindSequence(q, row, &begin, &end) : -1;
+    marks.live[tid] = s >= 0;
+    marks.first[tid] = s >= 0 && row == begin ? s : -1;
+    marks.last[tid] = s >= 0 && row == end - 1 ? s : -1;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ RecEvents EventsOf(const RecMarks &marks, int stretch) {
+  const int at = stretch * kRecSteps;
+  RecEvents e = {0, 0, 0, marks.first + at, marks.last + at};
+#pragma unroll
+  for (int k = 0; k < kRecSteps; k++) {
+    e.live |= (uint32_t)marks.live[at + k] << k;
+    e.first |= (uint32_t)(marks.first[at + k] >= 0) << k;
+    e.last |= (uint32_t)(marks.last[at + k] >= 0) << k;
+  }
+  e.first &= e.live, e.last &= e.live;
   return e;
 }
 
@@ -323,29 +400,6 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
   }
 }
 
-// What a workgroup knows of its rows: those of one sequence alone, or not.
-struct RecPlace {
-  int row, limit, begin, end, sequence;   // (the same in every thread)
-  bool interior;
-  __device__ __forceinline__ RecPlace(const RecKernelArgs &p, int tile) {
-    row = tile * p.tile_rows;
-    limit = min(row + p.tile_rows, (int)p.a.seq.rows);
-    begin = end = 0;
-    sequence = row < limit ? FindSequence(p.a.seq, row, &begin, &end) : -1;
-    sequence = __builtin_amdgcn_readfirstlane(sequence);
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    interior = sequence >= 0 && row + kRecTile <= min(end, limit);
-  }
-  // whether the sequence of the last row goes on behind
-  __device__ __forceinline__ bool GoesOn(const RecKernelArgs &p) const {
-    if (interior) return row + kRecTile < end;
-    if (row >= limit) return false;
-    int b, e;
-    return FindSequence(p.a.seq, limit - 1, &b, &e) >= 0 && limit < e;
-  }
-};
-
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForward {
   static constexpr int V = RecV<XT>();
   typedef RecDecay<XT, GT, FORM, PER_CHANNEL> Decay;
@@ -360,11 +414,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && !(e.live >> k & 1)) continue;
-      if (EVENTS && (e.first >> k & 1)) {
-        int begin, end;
-        const int q = FindSequence(p.a.seq, row + k, &begin, &end);
-        LoadState<V>(s, p.a.initial, q, p.a.channels, own);
-      }
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(s, p.a.initial, e.first_of[k], p.a.channels, own);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         c[k][j] = decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
@@ -377,10 +427,10 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 
   template <bool EVENTS>
   __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> &shared, const Decay &decay,
-                                                 Tile &t, const RecPlace &place, int tile, int channel_tile) {
+                                                 Tile &t, const RecPlace &place, const RecMarks &marks, int tile, int channel_tile) {
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
-    if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
+    if (EVENTS) e = EventsOf(marks, lane.Stretch());
     float c[kRecSteps][V], s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
@@ -407,12 +457,11 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
         lane.own.Store(y + (int64_t)k * p.a.channels + offset, zero);
         continue;
       }
-      int begin, end;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
 #pragma unroll
       for (int j = 0; j < V; j++) state[j] = Decay::Step(c[k][j], t.x[k][j], state[j]);
       lane.own.Store(y + (int64_t)k * p.a.channels + offset, state);
-      if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
+      if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, e.last_of[k], p.a.channels, lane.own);
     }
     if (!EVENTS && place.row + kRecTile == place.end && lane.Stretch() == kRecWaves * kRecPieces - 1)
       StoreState<V>(p.a.final_state, state, place.sequence, p.a.channels, lane.own);
@@ -428,12 +477,18 @@ __global__ __launch_bounds__(kRecThreads, 4) void RecurrenceForwardKernel(RecKer
   int tile, channel_tile;
   TakeTile<false>(p, &slot, &tile, &channel_tile);
   const RecLane<XT> lane(p.a.channels, channel_tile);
-  const RecPlace place(p, tile);
+  __shared__ RecMarks marks;
+  RecPlace place(p, tile);
   typename Op::Tile t;
   if (place.row < place.limit) LoadTile<XT, GT, PER_CHANNEL>(t, p, place.row, lane.Stretch(), place.limit, lane.own);
   const typename Op::Decay decay(p.a, lane.own);
-  if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, place, tile, channel_tile);
-  else Op::template Process<true>(p, lane, shared, decay, t, place, tile, channel_tile);
+  place.Find(p);
+  if (place.interior) {
+    Op::template Process<false>(p, lane, shared, decay, t, place, marks, tile, channel_tile);
+  } else {
+    Mark(p, place, marks);
+    Op::template Process<true>(p, lane, shared, decay, t, place, marks, tile, channel_tile);
+  }
   PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.initial, p.a.final_state);
 }
 
@@ -448,10 +503,7 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
 #pragma unroll
   for (int k = kRecSteps - 1; k >= 0; k--) {
     if (EVENTS && !(e.live >> k & 1)) continue;
-    if (EVENTS && (e.last >> k & 1)) {
-      int begin, end;
-      LoadState<V>(s, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, own);
-    }
+    if (EVENTS && (e.last >> k & 1)) LoadState<V>(s, p.a.dfinal, e.last_of[k], p.a.channels, own);
 #pragma unroll
     for (int j = 0; j < V; j++) {
       a[j] *= decay.Product(c[k][j], j);
@@ -469,11 +521,11 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 
   template <bool EVENTS>
   __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> (&shared)[2], const Decay &decay,
-                                                 Tile &t, Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, int tile, int channel_tile,
+                                                 Tile &t, Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, const RecMarks &marks, int tile, int channel_tile,
                                                  const float (&saved)[V], float (&sum)[V]) {
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
-    if (EVENTS) e = FindEvents(p.a.seq, row, limit, place.begin, place.end);
+    if (EVENTS) e = EventsOf(marks, lane.Stretch());
     float c[kRecSteps][V], s[V], state[V], back[V];
     double a[V];
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
@@ -483,16 +535,17 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
     __syncthreads();
-    const bool needs = place.GoesOn(p);
+    // the last row's sequence goes on behind the tile
+    const int last_row = limit - 1 - place.row;
+    const bool needs = EVENTS ? limit > place.row && marks.live[last_row] && marks.last[last_row] < 0 : place.row + kRecTile < place.end;
     FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
     // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
     lane.template Start<false, EVENTS>(shared[0], front, saved, state);
-    int begin, end;
     float before[kRecSteps][V];
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (EVENTS && !(e.live >> k & 1)) continue;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         const float x = t.x[k][j];
@@ -513,7 +566,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
       float dx[V] = {}, dg[V] = {};
       const bool live = !EVENTS || (e.live >> k & 1);
       if (live) {
-        if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
+        if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, e.last_of[k], p.a.channels, lane.own);
 #pragma unroll
         for (int j = 0; j < V; j++) {
           const float l = back[j] + dy[k][j];
@@ -527,7 +580,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
           if (PER_CHANNEL) sum[j] += dg[j];
           back[j] = Decay::Back(c[k][j], l);
         }
-        if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, FindSequence(p.a.seq, row + k, &begin, &end), p.a.channels, lane.own);
+        if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, e.first_of[k], p.a.channels, lane.own);
       }
       const int64_t at = (int64_t)(place.row + k) * p.a.channels;
       lane.own.Store(static_cast<XT *>(p.a.dx) + at + offset, dx);
@@ -546,7 +599,8 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
   int tile, channel_tile;
   TakeTile<true>(p, &slot, &tile, &channel_tile);
   const RecLane<XT> lane(p.a.channels, channel_tile);
-  const RecPlace place(p, tile);
+  __shared__ RecMarks marks;
+  RecPlace place(p, tile);
   typename Op::Tile t;
   Group<XT, V> dy[kRecSteps];
   float saved[V], sum[V] = {};
@@ -564,8 +618,13 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
   }
   LoadState<V>(saved, p.a.saved, tile, p.a.channels, lane.own);
   const typename Op::Decay decay(p.a, lane.own);
-  if (place.interior) Op::template Process<false>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
-  else Op::template Process<true>(p, lane, shared, decay, t, dy, place, tile, channel_tile, saved, sum);
+  place.Find(p);
+  if (place.interior) {
+    Op::template Process<false>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum);
+  } else {
+    Mark(p, place, marks);
+    Op::template Process<true>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum);
+  }
   PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.dfinal, p.a.dinitial);
   if (PER_CHANNEL) {
 #pragma unroll
