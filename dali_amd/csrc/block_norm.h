@@ -13,11 +13,16 @@
 
 namespace daliamd {
 
+// Threads of a row of more than 256 channels: whole waves, with one piece of 4 channels each up to 4096 channels, two up to 8192.
+inline int NormRowThreads(int channels) {
+  const int pieces = (channels + 3) / 4, each = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : 4;
+  return ((pieces + each - 1) / each + 63) / 64 * 64;
+}
 // Workgroups of the backward pass, at most: as many as the card holds at once (four waves per SIMD), so that no second round is
 // left half empty and the partial sums stay a small part of what it moves.
 inline int64_t BackwardWorkgroups(int64_t rows, int channels) {
-  const int threads = channels <= 1024 ? 256 : channels <= 2048 ? 512 : 1024;
-  return std::min<int64_t>(rows, 256 * 1024 / threads);
+  const int threads = channels <= 256 ? 256 : NormRowThreads(channels);
+  return std::min<int64_t>(rows, 256 * (1024 / threads));
 }
 
 // one source file per type of x; `count`: the workgroups that leave partial sums

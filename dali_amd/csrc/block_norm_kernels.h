@@ -6,28 +6,32 @@
 
 namespace daliamd {
 
-// A row's channels stay in the registers of TPR threads, NV pieces of 4 channels each: one pass over memory, whatever the number of
-// sums.  Four channels - 8 bytes of a 16-bit type - rather than 16 bytes: the backward pass holds a dozen numbers per channel, and
-// with half the channels per thread twice the waves fit a compute unit.  A workgroup has 256 threads or one row; sums go by
-// shuffles inside a wave and, for rows of several waves, one exchange through LDS.  Workgroups go through the rows with a stride;
-// the backward pass keeps its sums over rows (three weights) in registers meanwhile and leaves one partial sum per workgroup, which
-// BlockNormWeightsKernel adds up in a fixed order.
-constexpr int kNormV = 4;
-template <int TPR> constexpr int NormThreads() { return TPR > 256 ? TPR : 256; }
-template <int TPR> constexpr int NormWaves() { return NormThreads<TPR>() / 64; }
+// A row's channels stay in registers, NV pieces of 4 channels per thread: one pass over memory, whatever the number of sums.  Four
+// channels - 8 bytes of a 16-bit type - rather than 16 bytes: the backward pass holds a dozen numbers per channel, and with half the
+// channels per thread twice the waves fit a compute unit.
+// TPR 8 to 64: so many threads per row, 256 / TPR rows in a workgroup, sums by shuffles.  TPR kWaves: a workgroup per row, of as
+// many waves as the row needs (a row of 1111 channels five, not eight), sums through LDS.  Workgroups go through the rows with a
+// stride; the backward pass keeps its sums over rows (three weights) in registers meanwhile and leaves one partial sum per
+// workgroup, which BlockNormWeightsKernel adds up in a fixed order.
+constexpr int kNormV = 4, kWaves = 1024, kMaxWaves = 16;
+template <int TPR> constexpr int NormThreads() { return TPR == kWaves ? 1024 : 256; }
 
-// the sum over the TPR threads of a row, in each of them; `slot` alternates between calls: one barrier per sum, because a wave
-// that writes a slot again has passed the barrier behind the last reads of it
-template <int TPR> __device__ __forceinline__ float RowSum(float v, float (*shared)[NormWaves<TPR>()], int slot) {
+// the sum over the threads of a row, in each of them; `slot` alternates between calls: one barrier per sum, because a wave
+// that writes a slot again has passed the barrier behind the last reads of it.  The places of waves that do not exist hold zeros.
+struct alignas(16) NormShared { float wave[2][kMaxWaves]; };
+template <int TPR> __device__ __forceinline__ void ClearShared(NormShared &shared) {
+  if (TPR == kWaves && threadIdx.x < 2 * kMaxWaves) shared.wave[threadIdx.x / kMaxWaves][threadIdx.x % kMaxWaves] = 0;
+  if (TPR == kWaves) __syncthreads();
+}
+template <int TPR> __device__ __forceinline__ float RowSum(float v, NormShared &shared, int slot) {
 #pragma unroll
   for (int off = (TPR > 64 ? 64 : TPR) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  if (TPR > 64) {
-    if ((threadIdx.x & 63) == 0) shared[slot][threadIdx.x >> 6] = v;
+  if (TPR == kWaves) {
+    if ((threadIdx.x & 63) == 0) shared.wave[slot][threadIdx.x >> 6] = v;
     __syncthreads();
-    const int first = (int)threadIdx.x / TPR * (TPR / 64);
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < TPR / 64; w++) v += shared[slot][first + w];
+    const float4 *w = reinterpret_cast<const float4 *>(shared.wave[slot]);
+    const float4 p = w[0], q = w[1], r = w[2], s = w[3];
+    v = ((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w)) + (((r.x + r.y) + (r.z + r.w)) + ((s.x + s.y) + (s.z + s.w)));
   }
   return v;
 }
@@ -70,19 +74,21 @@ template <typename XT, int V, int NV, bool WHOLE> struct NormWeights {
 template <typename XT, typename RT, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlockNormArgs p) {
   constexpr int V = kNormV, kRows = NormThreads<TPR>() / TPR;
-  __shared__ float shared[2][NormWaves<TPR>()];
-  const int lane = (int)threadIdx.x % TPR;
+  const int tpr = TPR == kWaves ? (int)blockDim.x : TPR;
+  __shared__ NormShared shared;
+  ClearShared<TPR>(shared);
+  const int lane = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
   const NormWeights<XT, V, NV, WHOLE> weights(p, Channels<V, WHOLE>(lane * V, p.channels));
   const float inv = 1.0f / p.channels;
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = base + threadIdx.x / TPR;
+    const int64_t row = TPR == kWaves ? base : base + threadIdx.x / TPR;
     const bool live = kRows == 1 || row < p.rows;
     const int64_t at = live ? row : base;   // (rows of a wave that do not exist: the first one's again, not written)
     Group<XT, V> x[NV], g[NV];
     Group<RT, V> r[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
       if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
       if (p.residual) m.Load(r[i], static_cast<const RT *>(p.residual) + at * p.residual_row);
@@ -92,7 +98,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
       float sum = 0;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        Channels<V, WHOLE>((i * TPR + lane) * V, p.channels).Mask(x[i]);
+        Channels<V, WHOLE>((i * tpr + lane) * V, p.channels).Mask(x[i]);
 #pragma unroll
         for (int j = 0; j < V; j++) sum = fmaf(x[i][j], x[i][j], sum);
         x[i].Repack();
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
     float h[NV][V], sum = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V];
       if (p.post_weight) weights.template Get<0>(post, m);
       if (p.scale) weights.template Get<1>(scale, m);
@@ -124,7 +130,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
       if (p.rstd_pre && lane == 0 && live) p.rstd_pre[row] = rstd2;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+        const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
         float pre[V];
         weights.template Get<2>(pre, m);
 #pragma unroll
@@ -132,20 +138,20 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
         if (live) m.Store(static_cast<XT *>(p.normed) + row * p.channels, pre);
       }
     }
-    if (TPR > 64 && (!p.post_weight || !p.pre_weight)) __syncthreads();   // one sum per row: the slot is written again
+    if (TPR == kWaves && (!p.post_weight || !p.pre_weight)) __syncthreads();   // one sum per row: the slot is written again
   }
 }
 
 // What a row brings to its gradients, as it is in memory.
-template <typename XT, typename RT, int TPR, int NV, bool WHOLE> struct NormRow {
+template <typename XT, typename RT, int NV, bool WHOLE> struct NormRow {
   static constexpr int V = kNormV;
   Group<XT, V> x[NV], g[NV], dn[NV];
   Group<RT, V> r[NV], dh[NV];
   float rstd, rstd2;
-  __device__ __forceinline__ void Load(const daliamdBlockNormArgs &p, int64_t at, int lane, bool second) {
+  __device__ __forceinline__ void Load(const daliamdBlockNormArgs &p, int64_t at, int lane, int tpr, bool second) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       m.Load(x[i], static_cast<const XT *>(p.x) + at * p.x_row);
       if (p.gate) m.Load(g[i], static_cast<const XT *>(p.gate) + at * p.gate_row);
       if (second) {
@@ -158,10 +164,10 @@ template <typename XT, typename RT, int TPR, int NV, bool WHOLE> struct NormRow 
     rstd2 = second ? p.rstd_pre[at] : 1.0f;
   }
   // zeros for what is another thread's: it then adds nothing to any sum
-  __device__ __forceinline__ void Mask(const daliamdBlockNormArgs &p, int lane, bool second) {
+  __device__ __forceinline__ void Mask(const daliamdBlockNormArgs &p, int lane, int tpr, bool second) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       if (second) m.Mask(dn[i]);
       if (p.dhidden) m.Mask(dh[i]);
       m.Mask(x[i]);
@@ -177,24 +183,26 @@ template <typename XT, typename RT, int TPR, int NV, bool WHOLE> struct NormRow 
 template <typename XT, typename RT, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, float *partial) {
   constexpr int V = kNormV, kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
-  __shared__ float shared[2][NormWaves<TPR>()];
-  const int lane = (int)threadIdx.x % TPR;
+  const int tpr = TPR == kWaves ? (int)blockDim.x : TPR;
+  __shared__ NormShared shared;
+  ClearShared<TPR>(shared);
+  const int lane = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
   const NormWeights<XT, V, NV, WHOLE> weights(p, Channels<V, WHOLE>(lane * V, p.channels));
   const float inv = 1.0f / p.channels;
   const bool second = p.pre_weight && p.dnormed;
   float apost[NV][V] = {}, ascale[NV][V] = {}, apre[NV][V] = {};
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = base + threadIdx.x / TPR;
+    const int64_t row = TPR == kWaves ? base : base + threadIdx.x / TPR;
     const bool live = kRows == 1 || row < p.rows;
-    NormRow<XT, RT, TPR, NV, WHOLE> t;
-    t.Load(p, live ? row : base, lane, second);
-    t.Mask(p, lane, second);
+    NormRow<XT, RT, NV, WHOLE> t;
+    t.Load(p, live ? row : base, lane, tpr, second);
+    t.Mask(p, lane, tpr, second);
     const float rstd = t.rstd, rstd2 = t.rstd2;
     // v, and with the second norm h^ and the mean of dn w_pre h^
     float v[NV][V], hat[NV][V], mean2 = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V], pre[V];
       if (p.post_weight) weights.template Get<0>(post, m);
       if (p.scale) weights.template Get<1>(scale, m);
@@ -219,7 +227,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
     float d[NV][V], mean1 = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V], pre[V], dgate[V];
       if (p.post_weight) weights.template Get<0>(post, m);
       if (p.scale) weights.template Get<1>(scale, m);
@@ -265,16 +273,16 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
     }
     if (live) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) Channels<V, WHOLE>((i * TPR + lane) * V, p.channels).Store(static_cast<XT *>(p.dx) + row * p.channels, d[i]);
+      for (int i = 0; i < NV; i++) Channels<V, WHOLE>((i * tpr + lane) * V, p.channels).Store(static_cast<XT *>(p.dx) + row * p.channels, d[i]);
     }
-    if (TPR > 64 && (!p.post_weight || !second)) __syncthreads();
+    if (TPR == kWaves && (!p.post_weight || !second)) __syncthreads();
   }
   if (!partial) return;
   float *out = partial + (int64_t)blockIdx.x * 3 * p.channels;
   if (kRows == 1) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       if (p.post_weight) m.Store(out, apost[i]);
       if (p.scale) m.Store(out + p.channels, ascale[i]);
       if (p.pre_weight) m.Store(out + 2 * p.channels, apre[i]);
@@ -284,7 +292,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
     __shared__ float rows[3][kRows > 1 ? kThreads : 1];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * TPR + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V], pre[V];
 #pragma unroll
       for (int j = 0; j < V; j++) {
@@ -311,37 +319,32 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
 }
 
 template <typename XT, typename RT, int TPR, int NV> struct NormLaunch {
-  static constexpr int kThreads = NormThreads<TPR>(), kRows = kThreads / TPR, kV = kNormV;
+  static constexpr int kRows = TPR == kWaves ? 1 : 256 / TPR;
+  static dim3 Threads(int channels) { return dim3(TPR == kWaves ? NormRowThreads(channels) : 256); }
   static void Forward(hipStream_t s, const daliamdBlockNormArgs &a) {
-    const int64_t groups = std::min<int64_t>((a.rows + kRows - 1) / kRows, 1 << 20);
+    const dim3 grid((unsigned)std::min<int64_t>((a.rows + kRows - 1) / kRows, 1 << 20)), block = Threads(a.channels);
     KernelTimer timer("BlockNormKernel", s);
-    const dim3 grid((unsigned)groups), block(kThreads);
-    if (a.channels % kV == 0) hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV, true>), grid, block, 0, s, a);
+    if (a.channels % kNormV == 0) hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((BlockNormKernel<XT, RT, TPR, NV, false>), grid, block, 0, s, a);
   }
   static void Backward(hipStream_t s, const daliamdBlockNormArgs &a, float *partial, int *count) {
-    const int64_t groups = (a.rows + kRows - 1) / kRows;
-    *count = (int)std::min(groups, BackwardWorkgroups(a.rows, a.channels));
+    *count = (int)std::min((a.rows + kRows - 1) / kRows, BackwardWorkgroups(a.rows, a.channels));
+    const dim3 grid((unsigned)*count), block = Threads(a.channels);
     KernelTimer timer("BlockNormBackwardKernel", s);
-    const dim3 grid((unsigned)*count), block(kThreads);
-    if (a.channels % kV == 0) hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV, true>), grid, block, 0, s, a, partial);
+    if (a.channels % kNormV == 0) hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV, true>), grid, block, 0, s, a, partial);
     else hipLaunchKernelGGL((BlockNormBackwardKernel<XT, RT, TPR, NV, false>), grid, block, 0, s, a, partial);
   }
 };
 
-// the number of threads per row and pieces per thread: the fewest that hold the row
 template <typename XT, typename RT, typename F> static void WithShape(int channels, F f) {
   const int pieces = (channels + kNormV - 1) / kNormV;
   if (pieces <= 8) f(NormLaunch<XT, RT, 8, 1>());
   else if (pieces <= 16) f(NormLaunch<XT, RT, 16, 1>());
   else if (pieces <= 32) f(NormLaunch<XT, RT, 32, 1>());
   else if (pieces <= 64) f(NormLaunch<XT, RT, 64, 1>());
-  else if (pieces <= 128) f(NormLaunch<XT, RT, 128, 1>());
-  else if (pieces <= 256) f(NormLaunch<XT, RT, 256, 1>());
-  else if (pieces <= 512) f(NormLaunch<XT, RT, 512, 1>());
-  else if (pieces <= 1024) f(NormLaunch<XT, RT, 1024, 1>());
-  else if (pieces <= 2048) f(NormLaunch<XT, RT, 1024, 2>());
-  else f(NormLaunch<XT, RT, 1024, 4>());
+  else if (pieces <= 1024) f(NormLaunch<XT, RT, kWaves, 1>());
+  else if (pieces <= 2048) f(NormLaunch<XT, RT, kWaves, 2>());
+  else f(NormLaunch<XT, RT, kWaves, 4>());
 }
 template <typename XT, typename F> static void WithResidual(const daliamdBlockNormArgs &a, F f) {
   if (a.residual && a.residual_dtype == DALIAMD_FLOAT) WithShape<XT, float>(a.channels, f);

@@ -164,7 +164,8 @@ __global__ __launch_bounds__(kSmallThreads) void SortSmallKernel(daliamdEmbeddin
   for (int pass = 0; pass < s.passes; pass++) {
     const int shift = pass * s.bits;
     const uint32_t digits = (1u << s.bits) - 1;
-    for (int d = tid; d < kWaves * kDigits; d += kSmallThreads) next[d / kDigits][d % kDigits] = 0;
+    for (int d = tid; d < kWaves * kDigits; d += kSmallThreads)
+      if ((uint32_t)d % kDigits <= digits) next[d / kDigits][d % kDigits] = 0;
 #pragma unroll
     for (int r = 0; r < kSmallRounds; r++) {
       const int t = (wave * kSmallRounds + r) * 64 + lane;
@@ -174,15 +175,17 @@ __global__ __launch_bounds__(kSmallThreads) void SortSmallKernel(daliamdEmbeddin
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSmallRounds; r++)
-      if ((wave * kSmallRounds + r) * 64 + lane < tokens) atomicAdd(&next[wave][(k[r] >> shift) & digits], 1u);
+    for (int r = 0; r < kSmallRounds; r++) {
+      const bool valid = (wave * kSmallRounds + r) * 64 + lane < tokens;
+      to[r] = TakePlace(next[wave], valid ? (k[r] >> shift) & digits : 0, s.bits, valid);
+    }
     __syncthreads();
+    // `next` counts each wave's digits now: to where the first of each goes
     uint32_t all = 0;
-    if (tid < kDigits)
+    if (tid <= (int)digits)
       for (int w = 0; w < kWaves; w++) all += next[w][tid];
     uint32_t place = PrefixOfDigits(all, wave_total);
-    __syncthreads();
-    if (tid < kDigits)
+    if (tid <= (int)digits)
       for (int w = 0; w < kWaves; w++) {
         const uint32_t n = next[w][tid];
         next[w][tid] = place;
@@ -190,14 +193,11 @@ __global__ __launch_bounds__(kSmallThreads) void SortSmallKernel(daliamdEmbeddin
       }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSmallRounds; r++) {
-      const bool valid = (wave * kSmallRounds + r) * 64 + lane < tokens;
-      to[r] = TakePlace(next[wave], valid ? (k[r] >> shift) & digits : 0, s.bits, valid);
-    }
-    __syncthreads();
-#pragma unroll
     for (int r = 0; r < kSmallRounds; r++)
-      if ((wave * kSmallRounds + r) * 64 + lane < tokens) key[to[r]] = k[r], index[to[r]] = at[r];
+      if ((wave * kSmallRounds + r) * 64 + lane < tokens) {
+        const uint32_t at_place = next[wave][(k[r] >> shift) & digits] + to[r];
+        key[at_place] = k[r], index[at_place] = at[r];
+      }
     __syncthreads();
   }
   for (int t = tid; t < tokens; t += kSmallThreads) {
@@ -229,27 +229,40 @@ __device__ __forceinline__ int64_t LowerBound(const uint32_t *keys, int64_t n, u
   return lo;
 }
 
+// ... by a whole wave, 64 places at a time
+__device__ __forceinline__ int64_t LowerBoundOfWave(const uint32_t *keys, int64_t n, uint32_t key) {
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, hi = n;   // all in front of lo are below, none from hi on
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const int below = __popcll(__ballot(at < hi && keys[min(at, hi - 1)] < key));
+    if (below == 0) return lo;
+    hi = min(lo + below * step, hi);
+    lo += (below - 1) * step + 1;
+  }
+  return lo;
+}
+
 template <typename TT, typename OT, bool WHOLE>
 __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEmbeddingArgs p, EmbSums s) {
   const int64_t n = p.tokens;
   if ((int)blockIdx.x >= s.chunk_groups) {   // rows without a token
-    __shared__ uint64_t empty;
+    __shared__ uint8_t none[kFillRows];
+    __shared__ int bound[2];
     const int64_t row = (int64_t)((int)blockIdx.x - s.chunk_groups) * kFillRows;
-    if (threadIdx.x < kFillRows) {
-      const int64_t v = row + threadIdx.x;
-      bool none = false;
-      if (v < p.vocab) {
-        const int64_t at = LowerBound(s.key, n, (uint32_t)v);
-        none = at >= n || s.key[at] != (uint32_t)v;
-      }
-      const uint64_t mask = __ballot(none);
-      if (threadIdx.x == 0) empty = mask;
+    const int tid = threadIdx.x;
+    if (tid < 128) bound[tid >> 6] = (int)LowerBoundOfWave(s.key, n, (uint32_t)(row + (tid >> 6) * kFillRows));
+    __syncthreads();
+    if (tid < kFillRows) {
+      const int64_t at = bound[0] + LowerBound(s.key + bound[0], bound[1] - bound[0], (uint32_t)(row + tid));
+      none[tid] = at >= bound[1] || s.key[at] != (uint32_t)(row + tid);
     }
     __syncthreads();
     const float zero[kEmbV] = {};
-    for (uint64_t mask = empty; mask; mask &= mask - 1) {
-      TT *out = static_cast<TT *>(p.dtable) + (row + __ffsll((unsigned long long)mask) - 1) * p.channels;
-      for (int c = (int)threadIdx.x * kEmbV; c < p.channels; c += kEmbThreads * kEmbV) Channels<kEmbV, WHOLE>(c, p.channels).Store(out, zero);
+    for (int r = tid / s.tpr; r < kFillRows && row + r < p.vocab; r += kEmbThreads / s.tpr) {
+      if (!none[r]) continue;
+      TT *out = static_cast<TT *>(p.dtable) + (row + r) * p.channels;
+      for (int c = tid % s.tpr * kEmbV; c < p.channels; c += s.tpr * kEmbV) Channels<kEmbV, WHOLE>(c, p.channels).Store(out, zero);
     }
     return;
   }
