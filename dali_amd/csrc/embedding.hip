@@ -251,7 +251,10 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
     __shared__ int bound[2];
     const int64_t row = (int64_t)((int)blockIdx.x - s.chunk_groups) * kFillRows;
     const int tid = threadIdx.x;
-    if (tid < 128) bound[tid >> 6] = (int)LowerBoundOfWave(s.key, n, (uint32_t)(row + (tid >> 6) * kFillRows));
+    if (tid < 128) {
+      const int at = (int)LowerBoundOfWave(s.key, n, (uint32_t)(row + (tid >> 6) * kFillRows));
+      if ((tid & 63) == 0) bound[tid >> 6] = at;
+    }
     __syncthreads();
     if (tid < kFillRows) {
       const int64_t at = bound[0] + LowerBound(s.key + bound[0], bound[1] - bound[0], (uint32_t)(row + tid));

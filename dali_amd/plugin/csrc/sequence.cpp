@@ -127,18 +127,21 @@ bool Tracked(std::initializer_list<Tensor> tensors) {
   return false;
 }
 Maybe AsMaybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
-// Gradients that cannot be differentiated again: asked for with create_graph, they say so if that is tried.
-variable_list Once(variable_list grads, const char *what) {
+// Gradients that cannot be differentiated again: asked for with create_graph, they say so if that is tried.  They depend on
+// `inputs` and on the gradients of the outputs, so that a second differentiation with respect to any of these finds the error.
+variable_list Once(variable_list grads, const variable_list &inputs, const variable_list &outputs, const char *what) {
   if (!at::GradMode::is_enabled()) return grads;
-  variable_list some;
+  variable_list all;
   for (const Tensor &g : grads)
-    if (g.defined()) some.push_back(g);
-  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " cannot be differentiated twice", (int64_t)some.size());
-  for (Tensor &g : some) g = g.detach().requires_grad_(true);
-  some = (*error)(std::move(some));
+    if (g.defined()) all.push_back(g.detach().requires_grad_(true));
+  for (const variable_list *list : {&inputs, &outputs})
+    for (const Tensor &t : *list)
+      if (t.defined() && t.requires_grad()) all.push_back(t);
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " cannot be differentiated twice", (int64_t)all.size());
+  all = (*error)(std::move(all));
   size_t k = 0;
   for (Tensor &g : grads)
-    if (g.defined()) g = some[k++];
+    if (g.defined()) g = all[k++];
   return grads;
 }
 
@@ -228,7 +231,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
     a.dinitial = FloatPtr(dinitial);
     const Tensor ws = Workspace(plan.backward_workspace_bytes, x);
     Check(lib.RecurrenceBackwardRun(on.stream, &a, Ptr(ws), plan.backward_workspace_bytes));
-    return Once({dx, ddecay, dinitial, Tensor(), Tensor(), Tensor()}, "linear_recurrence");
+    return Once({dx, ddecay, dinitial, Tensor(), Tensor(), Tensor()}, {x, decay, initial}, grads, "linear_recurrence");
   }
 };
 
@@ -282,6 +285,8 @@ std::tuple<Tensor, Tensor> Recurrence(const Tensor &x0, const Tensor &decay0, co
     return {out[0], out[1]};
   }
   auto [y, state, saved] = RecurrenceForward(x, decay, initial, off, len, form, Get(final_state), false);
+  // written in place: a backward pass that saved the tensor has to notice
+  if (final_state && !final_state->is_inference()) final_state->unsafeGetTensorImpl()->bump_version();
   return {y, state};
 }
 
@@ -354,7 +359,7 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
     a.dpost_weight = Ptr(dpost), a.dscale = Ptr(dscale), a.dpre_weight = Ptr(dpre);
     const Tensor ws = Workspace(plan.backward_workspace_bytes, t.x);
     Check(lib.BlockNormBackwardRun(on.stream, &a, Ptr(ws), plan.backward_workspace_bytes));
-    return Once({dx, dgate, dresidual, dpost, dscale, dpre, Tensor()}, "block_norm");
+    return Once({dx, dgate, dresidual, dpost, dscale, dpre, Tensor()}, {t.x, t.gate, t.residual, t.post, t.scale, t.pre}, grads, "block_norm");
   }
 };
 
@@ -449,7 +454,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     a.dout = Ptr(dout), a.dout_row = dout.stride(0), a.dtable = Ptr(dtable);
     const Tensor ws = Workspace(plan.backward_workspace_bytes, table);
     Check(lib.EmbeddingBackwardRun(on.stream, &a, Ptr(ws), plan.backward_workspace_bytes));
-    return Once({dtable, Tensor(), Tensor(), Tensor(), Tensor()}, "embedding_lookup");
+    return Once({dtable, Tensor(), Tensor(), Tensor(), Tensor()}, {table}, grads, "embedding_lookup");
   }
 };
 

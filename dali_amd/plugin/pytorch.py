@@ -15,6 +15,7 @@ import numpy as np
 import torch
 
 from .. import types
+from ..sequence import block_norm, embedding_lookup, linear_recurrence  # noqa: F401
 from ..tensors import TensorListGPU
 from .base_iterator import LastBatchPolicy, _DaliBaseIterator  # noqa: F401
 
@@ -46,6 +47,25 @@ def feed_ndarray(tensor_or_tl, arr, cuda_stream=None, non_blocking=False, _src=N
     else:
         arr.copy_(src)
     return arr
+
+
+def packed_rows(tensor_list, axis=0, cuda_stream=None):
+    """A ragged batch on the device as the sequence operators take it: (rows, offsets).
+
+    The samples are sequences along `axis` (0 for samples and rows, 1 for the (mels, frames) of a mel filter bank) with equal
+    other dimensions, which become the channels: rows is [sum of lengths, channels], a copy that the caller owns, and
+    sequence s has the rows offsets[s] up to offsets[s + 1] (int64, on the device).  `cuda_stream`: the torch stream to copy on
+    (default: the current one).  The copy is only enqueued: as with a non-blocking feed_ndarray, a pipeline that hands its outputs
+    over without stream order must not reuse the batch before that stream has come to it."""
+    if not isinstance(tensor_list, TensorListGPU):
+        raise TypeError("packed_rows takes a batch on the GPU: the sequence operators have no CPU fallback")
+    with torch.cuda.stream(cuda_stream):     # (None: the current one)
+        samples = [t.as_torch().movedim(axis, 0) for t in tensor_list]
+        if not samples:
+            raise ValueError("packed_rows: the batch has no samples")
+        rows = torch.cat([t.reshape(t.shape[0], int(np.prod(t.shape[1:]))) for t in samples])
+        ends = torch.from_numpy(np.cumsum([0] + [t.shape[0] for t in samples], dtype=np.int64))
+        return rows, ends.pin_memory().to(rows.device, non_blocking=True)
 
 
 class DALIGenericIterator(_DaliBaseIterator):

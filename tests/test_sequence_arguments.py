@@ -2,6 +2,7 @@
 look at devices last, so that tensors of this machine get as far as the refusal in question.)"""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -160,3 +161,15 @@ def test_struct_sizes_match_the_c_header(tmp_path):
     subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "s")])
     sizes = [int(v) for v in subprocess.check_output([str(tmp_path / "s")]).split()]
     assert sizes == [C.sizeof(m) for m in names.values()]
+
+
+def test_packed_rows_refuses_a_batch_in_host_memory():
+    from dali_amd import fn
+    from dali_amd.pipeline import Pipeline
+    from dali_amd.plugin.pytorch import packed_rows
+    pipe = Pipeline(batch_size=2, num_threads=1, device_id=None)
+    with pipe:
+        pipe.set_outputs(fn.external_source(source=lambda: [np.zeros((3, 2), np.float32), np.zeros((1, 2), np.float32)]))
+    pipe.build()
+    with pytest.raises(TypeError, match="no CPU fallback"):
+        packed_rows(pipe.run()[0])
