@@ -327,6 +327,18 @@ def test_block_norm_sizes(rows, channels, dtype):
     run_norm(norm_inputs(PARTS, rows, channels, dtype, F, dtype))
 
 
+@pytest.mark.parametrize("rows,channels", [(4095, 300), (4096, 257), (4097, 511), (4098, 513), (4099, 1001), (4097, 1111), (4101, 1280)])
+@pytest.mark.parametrize("dtype,rdtype", [(BF, F), (HF, HF)])
+def test_block_norm_many_rows(rows, channels, dtype, rdtype):
+    """Rows that a wave has to itself, and their number just below."""
+    run_norm(norm_inputs(PARTS, rows, channels, dtype, rdtype, dtype), train=False)
+
+
+def test_block_norm_many_rows_with_gradients():
+    run_norm(norm_inputs(PARTS, 4097, 300, BF, F, BF))
+    run_norm(norm_inputs(("post", "gate"), 4099, 301, HF, HF, HF))
+
+
 @pytest.mark.parametrize("use", [("h",), ("n",)])
 def test_block_norm_gradient_of_one_output(use):
     run_norm(norm_inputs(PARTS, 19, 200, BF, F, F), use=use)
