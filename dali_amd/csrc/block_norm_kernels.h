@@ -50,21 +50,46 @@ template <typename XT, int V, bool WHOLE> __device__ __forceinline__ void LoadWe
   }
 }
 
-// A thread's weights: with one piece of the row, in registers for all rows; with more, read again (from the L1) for each row.
-template <typename XT, int V, int NV, bool WHOLE> struct NormWeights {
-  static constexpr bool kKeep = NV == 1;
-  const daliamdBlockNormArgs &p;
-  float kept[kKeep ? 3 : 1][V];
-  __device__ __forceinline__ NormWeights(const daliamdBlockNormArgs &p_, const Channels<V, WHOLE> &m) : p(p_) {
-    if (!kKeep) return;
-    if (p.post_weight) LoadWeights<XT, V, WHOLE>(kept[0], p.post_weight, p.weight_dtype, m);
-    if (p.scale) LoadWeights<XT, V, WHOLE>(kept[kKeep ? 1 : 0], p.scale, p.weight_dtype, m);
-    if (p.pre_weight) LoadWeights<XT, V, WHOLE>(kept[kKeep ? 2 : 0], p.pre_weight, p.weight_dtype, m);
+// The compiler keeps the addresses of every tensor's pieces from row to row, 64 bits each, rather than compute them from a row's
+// number in scalar registers and 32 bits per lane; not if it does not know that these are the same in each round.
+template <int TPR> __device__ __forceinline__ int64_t AnyRow(int64_t row) {
+#if defined(__AMDGCN__)
+  if (TPR == kWaves) {
+    int r = __builtin_amdgcn_readfirstlane((int)row);
+    asm volatile("" : "+s"(r));
+    return r;
   }
-  template <int WHICH> __device__ __forceinline__ void Get(float (&w)[V], const Channels<V, WHOLE> &m) const {
+#endif
+  return row;
+}
+template <int TPR> __device__ __forceinline__ int AnyLane(int lane) {
+#if defined(__AMDGCN__)
+  if (TPR == kWaves) asm volatile("" : "+v"(lane));
+#endif
+  return lane;
+}
+
+// A thread's weights: with one or two pieces of the row, in registers for all rows; with more, read again (from the L2) for each row.
+template <typename XT, int V, int NV, bool WHOLE> struct NormWeights {
+  static constexpr bool kKeep = NV <= 2;
+  const daliamdBlockNormArgs &p;
+  float kept[kKeep ? 3 : 1][kKeep ? NV : 1][V];
+  __device__ __forceinline__ NormWeights(const daliamdBlockNormArgs &p_, int lane, int tpr) : p(p_) {
     if constexpr (kKeep) {
 #pragma unroll
-      for (int j = 0; j < V; j++) w[j] = kept[WHICH][j];
+      for (int i = 0; i < NV; i++) {
+        const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
+        if (p.post_weight) LoadWeights<XT, V, WHOLE>(kept[0][i], p.post_weight, p.weight_dtype, m);
+        if (p.scale) LoadWeights<XT, V, WHOLE>(kept[1][i], p.scale, p.weight_dtype, m);
+        if (p.pre_weight) LoadWeights<XT, V, WHOLE>(kept[2][i], p.pre_weight, p.weight_dtype, m);
+      }
+    }
+  }
+  // of piece i, which has the channels m
+  template <int WHICH> __device__ __forceinline__ void Get(float (&w)[V], int i, const Channels<V, WHOLE> &m) const {
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int j = 0; j < V; j++) w[j] = kept[WHICH][i][j];
     } else {
       LoadWeights<XT, V, WHOLE>(w, WHICH == 0 ? p.post_weight : WHICH == 1 ? p.scale : p.pre_weight, p.weight_dtype, m);
     }
@@ -77,11 +102,12 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
   const int tpr = TPR == kWaves ? (int)blockDim.x : TPR;
   __shared__ NormShared shared;
   ClearShared<TPR>(shared);
-  const int lane = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
-  const NormWeights<XT, V, NV, WHOLE> weights(p, Channels<V, WHOLE>(lane * V, p.channels));
+  const int lane0 = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
+  const NormWeights<XT, V, NV, WHOLE> weights(p, lane0, tpr);
   const float inv = 1.0f / p.channels;
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = TPR == kWaves ? base : base + threadIdx.x / TPR;
+    const int64_t row = TPR == kWaves ? AnyRow<TPR>(base) : base + threadIdx.x / TPR;
+    const int lane = AnyLane<TPR>(lane0);
     const bool live = kRows == 1 || row < p.rows;
     const int64_t at = live ? row : base;   // (rows of a wave that do not exist: the first one's again, not written)
     Group<XT, V> x[NV], g[NV];
@@ -111,8 +137,8 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
     for (int i = 0; i < NV; i++) {
       const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
+      if (p.post_weight) weights.template Get<0>(post, i, m);
+      if (p.scale) weights.template Get<1>(scale, i, m);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float v = x[i][j];
@@ -132,7 +158,7 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormKernel(daliamdBlo
       for (int i = 0; i < NV; i++) {
         const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
         float pre[V];
-        weights.template Get<2>(pre, m);
+        weights.template Get<2>(pre, i, m);
 #pragma unroll
         for (int j = 0; j < V; j++) pre[j] = h[i][j] * rstd2 * pre[j];
         if (live) m.Store(static_cast<XT *>(p.normed) + row * p.channels, pre);
@@ -175,93 +201,133 @@ template <typename XT, typename RT, int NV, bool WHOLE> struct NormRow {
   }
   __device__ __forceinline__ void Repack() {
 #pragma unroll
-    for (int i = 0; i < NV; i++) x[i].Repack(), g[i].Repack(), dn[i].Repack();
+    for (int i = 0; i < NV; i++) x[i].Repack(), g[i].Repack(), dn[i].Repack(), r[i].Repack(), dh[i].Repack();
   }
 };
 
+// The compiler holds a value that it has computed once for a second use; after this it computes it again from v.
+template <int V> __device__ __forceinline__ void Forget(float (&v)[V]) {
+#if defined(__AMDGCN__)
+#pragma unroll
+  for (int j = 0; j < V; j++) asm volatile("" : "+v"(v[j]));
+#endif
+}
+
 // partial: [gridDim.x][3][channels], sums of the workgroup's rows for post_weight, scale and pre_weight
+// Rows of more than 4096 channels have up to 16 waves with 128 registers per lane: their sums are in LDS as far as that goes (two of
+// three above 8192 channels), each thread's in its own places, and of a row only what is in memory and v stay in registers between
+// the sums over its channels.
 template <typename XT, typename RT, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(daliamdBlockNormArgs p, float *partial) {
   constexpr int V = kNormV, kThreads = NormThreads<TPR>(), kRows = kThreads / TPR;
+  constexpr bool kLds = NV > 1;
   const int tpr = TPR == kWaves ? (int)blockDim.x : TPR;
   __shared__ NormShared shared;
+  constexpr bool kLdsPre = NV == 2;
+  __shared__ float4 lds_sums[kLds ? (kLdsPre ? 3 : 2) * NV : 1][kLds ? kThreads : 1];
   ClearShared<TPR>(shared);
-  const int lane = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
-  const NormWeights<XT, V, NV, WHOLE> weights(p, Channels<V, WHOLE>(lane * V, p.channels));
+  const int lane0 = TPR == kWaves ? (int)threadIdx.x : (int)threadIdx.x % TPR;
+  const NormWeights<XT, V, NV, WHOLE> weights(p, lane0, tpr);
   const float inv = 1.0f / p.channels;
   const bool second = p.pre_weight && p.dnormed;
-  float apost[NV][V] = {}, ascale[NV][V] = {}, apre[NV][V] = {};
+  float apost[kLds ? 1 : NV][V] = {}, ascale[kLds ? 1 : NV][V] = {}, apre[kLdsPre ? 1 : NV][V] = {};
+  if (kLds) {
+#pragma unroll
+    for (int i = 0; i < (kLdsPre ? 3 : 2) * NV; i++) lds_sums[i][threadIdx.x] = make_float4(0, 0, 0, 0);
+  }
+  // sum `which` (0: post_weight, 1: scale, 2: pre_weight) of piece i += a b
+  auto add = [&](int which, int i, float (&reg)[V], const float (&a)[V], const float (&b)[V]) {
+    if (which == 2 ? kLdsPre : kLds) {
+      float4 &l = lds_sums[which * NV + i][threadIdx.x];
+      float4 f = l;
+      f.x = fmaf(a[0], b[0], f.x), f.y = fmaf(a[1], b[1], f.y), f.z = fmaf(a[2], b[2], f.z), f.w = fmaf(a[3], b[3], f.w);
+      l = f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j++) reg[j] = fmaf(a[j], b[j], reg[j]);
+    }
+  };
   for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t row = TPR == kWaves ? base : base + threadIdx.x / TPR;
+    const int64_t row = TPR == kWaves ? AnyRow<TPR>(base) : base + threadIdx.x / TPR;
+    const int lane = AnyLane<TPR>(lane0);
     const bool live = kRows == 1 || row < p.rows;
     NormRow<XT, RT, NV, WHOLE> t;
     t.Load(p, live ? row : base, lane, tpr, second);
     t.Mask(p, lane, tpr, second);
     const float rstd = t.rstd, rstd2 = t.rstd2;
-    // v, and with the second norm h^ and the mean of dn w_pre h^
-    float v[NV][V], hat[NV][V], mean2 = 0;
+    // v, and with the second norm the mean of dn w_pre h^
+    float v[NV][V], mean2 = 0;
+    auto hat = [&](int i, int j, const float (&scale)[V]) {   // h^ from v
+      float e = v[i][j];
+      if (p.scale) e *= scale[j];
+      if (p.residual) e += t.r[i][j];
+      return e * rstd2;
+    };
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V], pre[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
-      if (second) weights.template Get<2>(pre, m);
+      if (p.post_weight) weights.template Get<0>(post, i, m);
+      if (p.scale) weights.template Get<1>(scale, i, m);
+      if (second) weights.template Get<2>(pre, i, m);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float e = t.x[i][j];
         if (p.post_weight) e = e * rstd * post[j];
         if (p.gate) e *= Silu(t.g[i][j]);
         v[i][j] = e;
-        if (second) {
-          if (p.scale) e *= scale[j];
-          if (p.residual) e += t.r[i][j];
-          e *= rstd2;
-          hat[i][j] = e;
-          mean2 = fmaf(t.dn[i][j] * pre[j], e, mean2);
-        }
+        if (second) mean2 = fmaf(t.dn[i][j] * pre[j], hat(i, j, scale), mean2);
       }
     }
     if (second) mean2 = RowSum<TPR>(mean2, shared, 0) * inv;
     t.Repack();
+    if (kLds) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) Forget(v[i]);
+    }
     float d[NV][V], mean1 = 0;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
       float post[V], scale[V], pre[V], dgate[V];
-      if (p.post_weight) weights.template Get<0>(post, m);
-      if (p.scale) weights.template Get<1>(scale, m);
-      if (second) weights.template Get<2>(pre, m);
+      if (p.post_weight) weights.template Get<0>(post, i, m);
+      if (p.scale) weights.template Get<1>(scale, i, m);
+      if (second) weights.template Get<2>(pre, i, m);
+      float counted[V], hat1[V], hat2[V], counted2[V];   // (0 in rows that do not exist)
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float e = p.dhidden ? t.dh[i][j] : 0.0f;
         if (second) {
-          e += rstd2 * (t.dn[i][j] * pre[j] - hat[i][j] * mean2);
-          apre[i][j] = fmaf(live ? t.dn[i][j] : 0.0f, hat[i][j], apre[i][j]);
+          hat2[j] = hat(i, j, scale);
+          e += rstd2 * (t.dn[i][j] * pre[j] - hat2[j] * mean2);
+          counted2[j] = live ? t.dn[i][j] : 0.0f;
         }
         d[i][j] = e;
-        ascale[i][j] = fmaf(live ? e : 0.0f, v[i][j], ascale[i][j]);
+        counted[j] = live ? e : 0.0f;
       }
+      if (second) add(2, i, apre[kLdsPre ? 0 : i], counted2, hat2);
+      if (p.scale) add(1, i, ascale[kLds ? 0 : i], counted, v[i]);
       if (p.residual && live) m.Store(static_cast<RT *>(p.dresidual) + row * p.channels, d[i]);
 #pragma unroll
       for (int j = 0; j < V; j++) {
         float e = d[i][j];
         if (p.scale) e *= scale[j];
-        const float hat1 = t.x[i][j] * rstd;
+        hat1[j] = t.x[i][j] * rstd;
         if (p.gate) {
           float f, k;
           const float gg = t.g[i][j];
           LogisticPair(gg, &f, &k);
-          dgate[j] = e * (p.post_weight ? hat1 * post[j] : hat1) * (f * fmaf(gg, k, 1.0f));
+          dgate[j] = e * (p.post_weight ? hat1[j] * post[j] : hat1[j]) * (f * fmaf(gg, k, 1.0f));
           e *= gg * f;
         }
+        counted[j] = live ? e : 0.0f;
         if (p.post_weight) {
-          apost[i][j] = fmaf(live ? e : 0.0f, hat1, apost[i][j]);
           e *= post[j];
-          mean1 = fmaf(e, hat1, mean1);
+          mean1 = fmaf(e, hat1[j], mean1);
         }
         d[i][j] = e;
       }
+      if (p.post_weight) add(0, i, apost[kLds ? 0 : i], counted, hat1);
       if (p.gate && live) m.Store(static_cast<XT *>(p.dgate) + row * p.channels, dgate);
     }
     if (p.post_weight) {
@@ -282,24 +348,37 @@ __global__ __launch_bounds__(NormThreads<TPR>()) void BlockNormBackwardKernel(da
   if (kRows == 1) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
-      if (p.post_weight) m.Store(out, apost[i]);
-      if (p.scale) m.Store(out + p.channels, ascale[i]);
-      if (p.pre_weight) m.Store(out + 2 * p.channels, apre[i]);
+      const Channels<V, WHOLE> m((i * tpr + lane0) * V, p.channels);
+      if (kLds) {
+        const float4 f = lds_sums[i][threadIdx.x], g = lds_sums[kLds ? NV + i : 0][threadIdx.x];
+        const float post[V] = {f.x, f.y, f.z, f.w}, scale[V] = {g.x, g.y, g.z, g.w};
+        if (p.post_weight) m.Store(out, post);
+        if (p.scale) m.Store(out + p.channels, scale);
+      } else {
+        if (p.post_weight) m.Store(out, apost[kLds ? 0 : i]);
+        if (p.scale) m.Store(out + p.channels, ascale[kLds ? 0 : i]);
+      }
+      if (kLdsPre) {
+        const float4 f = lds_sums[kLdsPre ? 2 * NV + i : 0][threadIdx.x];
+        const float pre[V] = {f.x, f.y, f.z, f.w};
+        if (p.pre_weight) m.Store(out + 2 * p.channels, pre);
+      } else if (p.pre_weight) {
+        m.Store(out + 2 * p.channels, apre[kLdsPre ? 0 : i]);
+      }
     }
   } else {
     // the threads with the same channels in all rows of the workgroup: the first row's adds them up
     __shared__ float rows[3][kRows > 1 ? kThreads : 1];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const Channels<V, WHOLE> m((i * tpr + lane) * V, p.channels);
+      const Channels<V, WHOLE> m((i * tpr + lane0) * V, p.channels);
       float post[V], scale[V], pre[V];
 #pragma unroll
       for (int j = 0; j < V; j++) {
         __syncthreads();
-        rows[0][threadIdx.x] = apost[i][j];
-        rows[1][threadIdx.x] = ascale[i][j];
-        rows[2][threadIdx.x] = apre[i][j];
+        rows[0][threadIdx.x] = apost[kLds ? 0 : i][j];
+        rows[1][threadIdx.x] = ascale[kLds ? 0 : i][j];
+        rows[2][threadIdx.x] = apre[kLdsPre ? 0 : i][j];
         __syncthreads();
         post[j] = scale[j] = pre[j] = 0;
         if (threadIdx.x < TPR)

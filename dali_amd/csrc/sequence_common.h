@@ -106,12 +106,17 @@ template <int V, bool WHOLE = false> struct Channels {
     begin = first - base;
     end = min(V, channels);
   }
+  // (32 bits of bytes: a row that is the same in all lanes stays in scalar registers)
+  template <typename T> __device__ __forceinline__ T *At(T *row) const {
+    typedef typename std::conditional<std::is_const<T>::value, const char, char>::type Byte;
+    return reinterpret_cast<T *>(reinterpret_cast<Byte *>(row) + (uint32_t)base * (uint32_t)sizeof(T));
+  }
   template <typename T> __device__ __forceinline__ void Load(Group<T, V> &g, const T *row) const {
     if (narrow) {
 #pragma unroll
       for (int j = 0; j < V; j++) g.Set(j, row[min(j, end - 1)]);
     } else {
-      LoadWide(g, row + base);
+      LoadWide(g, At(row));
     }
   }
   // ... with zeros in the places of others
@@ -134,13 +139,13 @@ template <int V, bool WHOLE = false> struct Channels {
   }
   template <typename T> __device__ __forceinline__ void Store(T *row, const float *f) const {
     if constexpr (WHOLE) {
-      if (begin == 0) StoreWide<T, V>(row + base, f);
+      if (begin == 0) StoreWide<T, V>(At(row), f);
     } else if (begin == 0 && end == V) {
-      StoreWide<T, V>(row + base, f);
+      StoreWide<T, V>(At(row), f);
     } else {
 #pragma unroll
       for (int j = 0; j < V; j++)
-        if (j >= begin && j < end) row[base + j] = FromFloat<T>(f[j]);
+        if (j >= begin && j < end) At(row)[j] = FromFloat<T>(f[j]);
     }
   }
 };
