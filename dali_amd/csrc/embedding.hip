@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingKernel(daliamdEmbeddingA
 // every workgroup instead of a launch of their own) and moves its tile's tokens.  Up to kSmallTokens: everything in one workgroup.
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr int kTileTokens = 2048, kMaxTiles = 512;
+constexpr int kTileTokens = 1024, kMaxTiles = 512;
 constexpr int kSmallTokens = 4096, kSmallThreads = 1024, kSmallRounds = kSmallTokens / kSmallThreads;
 
 struct EmbSort {
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kSortThreads) void SortScatterKernel(daliamdEmbeddi
   for (int w = 0; w < kSortWaves; w++) next[w][tid] = 0;
   // this digit in the tiles before, and in all of them
   uint32_t before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 32
   for (int t = 0; t < s.tiles; t++) {
     const uint32_t n = s.count[(int64_t)t * kDigits + tid];
     all += n;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(d
   const uint32_t key = s.key[end - 1];
   if (key >= (uint32_t)p.vocab) return;
   if (begin > 0 && s.key[begin - 1] == key) return;                             // it began in a chunk before
-  const int64_t last = (LowerBound(s.key, p.tokens, key + 1) - 1) / s.chunk;     // the chunk that the run ends in
+  const int64_t last = (LowerBoundOfWave(s.key, p.tokens, key + 1) - 1) / s.chunk;   // the chunk that the run ends in
   const int lane = threadIdx.x % kJoinLanes, k = threadIdx.x / kJoinLanes;
   const int64_t count = last - chunk, each = (count + kJoinParts - 1) / kJoinParts;
   const int64_t from = chunk + 1 + k * each, to = min(from + each, last + 1);
