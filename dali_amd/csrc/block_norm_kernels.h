@@ -13,6 +13,11 @@ namespace daliamd {
 // many waves as the row needs (a row of 1111 channels five, not eight), sums through LDS; RowPerWave says which rows have one wave.
 // Workgroups go through the rows with a stride; the backward pass keeps its sums over rows (three weights) in registers meanwhile and
 // leaves one partial sum per workgroup, which BlockNormWeightsKernel adds up in a fixed order.
+//
+// Memory bounds it.  32768 rows of 2048 channels bf16, residual in float, all parts: forward 196 us for 939 MB (4.8 TB/s), backward
+// 292 us for 1.48 GB (5.1 TB/s); a copy of 1 GiB runs at 5.1 TB/s.  Rows whose channels are no multiple of 4 (5003 rows of 1111
+// float16, norm and gate: forward 14.5 us, 2.3 TB/s; backward 25 us, 2.2 TB/s) are bound by the latency of few bytes in flight: every
+// load is still a whole one, but rows end between cache lines.
 constexpr int kNormV = 4, kWaves = 1024, kMaxWaves = 16;
 template <int TPR> constexpr int NormThreads() { return TPR == kWaves ? 1024 : 256; }
 

@@ -3,6 +3,11 @@
 
 namespace daliamd {
 
+// Memory bounds the lookup and the sums.  65536 tokens, frequent ones thousands of times, of a table of 48000 x 1024 bf16: lookup
+// 38 us for 134 MB written and 33 MB of the table read (4.4 TB/s); gradient 64 us for 134 MB read, rows of 2 KB in the order of their
+// ids, and 98 MB written (3.6 TB/s), 11 us to join runs, and 24 us for two sorting passes, whose four kernels each wait for a handful
+// of loads one after the other.  131072 tokens of 64000 x 2048: lookup 153 us (4.2 TB/s).  A copy of 1 GiB runs at 5.1 TB/s.
+
 // ---- lookup ------------------------------------------------------------------------------------------------------------
 // TPR threads per row, 8 channels per thread and step; kTokens rows per thread, whose loads are all in flight at once.
 constexpr int kEmbThreads = 256, kEmbV = 8;

@@ -16,12 +16,12 @@
 // The state in front of a tile is what the tile before leaves behind, which another workgroup has: a chain.  A workgroup says
 // what is known as soon as it is known - the product (A, S) of its tile, or the state behind it where that needs nothing from in
 // front (a sequence begins in the tile) - and then goes back along the chain, four tiles at a time, adding up products until it
-// meets a state.  Every 8th tile says no product, but the state behind it, once it has found the one in front: no tile
-// looks further back than that, and which numbers make up a state does not depend on who was first, so neither do its bits.  Tiles are given out by a counter in the order of the chain, so a
-// workgroup only ever waits for workgroups that have begun before it and wait for none behind them: every wait ends.  Each number
-// is said in one 64-bit word together with a mark that it is there, so a number and its mark cannot be seen apart and no fence is
-// needed (a release to the whole card would write back the L2 of an XCD); the words are cleared by a launch in front.
-// With whole sequences in each tile (dense, at most 256 steps) there is no chain.
+// meets a state.  Every 8th tile says no product, but the state behind it, once it has found the one in front: no tile looks
+// further back than that, and which numbers make up a state does not depend on who was first, so neither do its bits.  Tiles are
+// given out by a counter in the order of the chain, so a workgroup only ever waits for workgroups that have begun before it and
+// waits for none behind them: every wait ends.  Each number is said in one 64-bit word together with a mark that it is there, so
+// a number and its mark cannot be seen apart and no fence is needed (a release to the whole card would write back the L2 of an
+// XCD); the words are cleared by a launch in front.  With whole sequences in each tile (dense, at most 256 steps) there is no chain.
 //
 // 1 - f is computed and applied as such (h += (1 - f)(x - h)), and products of decays are held in 64 bits: with a gate of 0.9999
 // the rounding of f to 32 bits is an error of 3e-8 in each of ten thousand steps that still count, and with constant gates all
