@@ -374,6 +374,21 @@ __device__ __forceinline__ void LoadTile(RecTile<XT, GT, PER_CHANNEL> &t, const 
   if constexpr (!PER_CHANNEL) LoadSteps<GT, V>(t.g, p.a.decay, p.a.seq, first, stretch, limit, p.a.decay_row, p.a.decay_seq, own, p.decay_plain && full);
 }
 
+// The coefficients of a stretch's steps: kept, or computed again where they are used again.
+template <typename Decay, typename Tile, bool PER_CHANNEL, bool KEEP> struct RecCoefficients {
+  static constexpr int V = Tile::V;
+  float kept[KEEP ? kRecSteps : 1][V];
+  __device__ __forceinline__ float First(const Decay &decay, const Tile &t, int k, int j) {
+    const float c = decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
+    if constexpr (KEEP) kept[k][j] = c;
+    return c;
+  }
+  __device__ __forceinline__ float Get(const Decay &decay, const Tile &t, int k, int j) const {
+    if constexpr (KEEP) return kept[k][j];
+    else return decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
+  }
+};
+
 template <int V> __device__ __forceinline__ void LoadState(float (&h)[V], const float *state, int64_t s, int channels, const Channels<V> &own) {
 #pragma unroll
   for (int j = 0; j < V; j++) h[j] = state && j < own.end ? state[s * channels + own.base + j] : 0.0f;
@@ -400,15 +415,18 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
   }
 }
 
+constexpr bool kKeepForward = true;
+constexpr int kForwardWaves = 4, kBackwardWaves = 4;
+
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForward {
   static constexpr int V = RecV<XT>();
   typedef RecDecay<XT, GT, FORM, PER_CHANNEL> Decay;
   typedef RecTile<XT, GT, PER_CHANNEL> Tile;
 
-  // (A, S, R) of a thread's stretch; `c`: the steps' coefficients for the second time
-  template <bool EVENTS>
+  // (A, S, R) of a thread's stretch
+  template <bool EVENTS, typename Coefficients>
   __device__ static __forceinline__ bool Compose(const RecKernelArgs &p, const Decay &decay, const Tile &t, const RecEvents &e, int row,
-                                                 const Channels<V> &own, float (&c)[kRecSteps][V], double (&a)[V], float (&s)[V]) {
+                                                 const Channels<V> &own, Coefficients &c, double (&a)[V], float (&s)[V]) {
 #pragma unroll
     for (int j = 0; j < V; j++) a[j] = 1.0, s[j] = 0.0f;
 #pragma unroll
@@ -417,9 +435,9 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
       if (EVENTS && (e.first >> k & 1)) LoadState<V>(s, p.a.initial, e.first_of[k], p.a.channels, own);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        c[k][j] = decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
-        a[j] *= decay.Product(c[k][j], j);
-        s[j] = Decay::Step(c[k][j], t.x[k][j], s[j]);
+        const float ck = c.First(decay, t, k, j);
+        a[j] *= decay.Product(ck, j);
+        s[j] = Decay::Step(ck, t.x[k][j], s[j]);
       }
     }
     return EVENTS && e.first != 0;
@@ -431,12 +449,17 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = EventsOf(marks, lane.Stretch());
-    float c[kRecSteps][V], s[V], state[V];
+    RecCoefficients<Decay, Tile, PER_CHANNEL, kKeepForward> c;
+    float s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
+    if (!PER_CHANNEL && !kKeepForward) {
+#pragma unroll
+      for (int k = 0; k < kRecSteps; k++) t.g[PER_CHANNEL ? 0 : k].Repack();
+    }
     __syncthreads();
     const bool starts = place.sequence < 0 || place.row == place.begin;
     FindFront<false, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
@@ -454,13 +477,13 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
       if (EVENTS && row + k >= limit) break;
       if (EVENTS && !(e.live >> k & 1)) {
         const float zero[V] = {};
-        lane.own.Store(y + (int64_t)k * p.a.channels + offset, zero);
+        lane.own.Store(y + (int64_t)k * p.a.channels, zero, offset);
         continue;
       }
       if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
 #pragma unroll
-      for (int j = 0; j < V; j++) state[j] = Decay::Step(c[k][j], t.x[k][j], state[j]);
-      lane.own.Store(y + (int64_t)k * p.a.channels + offset, state);
+      for (int j = 0; j < V; j++) state[j] = Decay::Step(c.Get(decay, t, k, j), t.x[k][j], state[j]);
+      lane.own.Store(y + (int64_t)k * p.a.channels, state, offset);
       if (EVENTS && (e.last >> k & 1)) StoreState<V>(p.a.final_state, state, e.last_of[k], p.a.channels, lane.own);
     }
     if (!EVENTS && place.row + kRecTile == place.end && lane.Stretch() == kRecWaves * kRecPieces - 1)
@@ -469,7 +492,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 };
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
-__global__ __launch_bounds__(kRecThreads, 4) void RecurrenceForwardKernel(RecKernelArgs p) {
+__global__ __launch_bounds__(kRecThreads, kForwardWaves) void RecurrenceForwardKernel(RecKernelArgs p) {
   typedef RecForward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared;
@@ -493,9 +516,9 @@ __global__ __launch_bounds__(kRecThreads, 4) void RecurrenceForwardKernel(RecKer
 }
 
 // (A, S, R) of a thread's stretch against time; dy NULL: zeros
-template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool EVENTS>
+template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool EVENTS, typename Tile, typename Coefficients>
 __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDecay<XT, GT, FORM, PER_CHANNEL> &decay, const Group<XT, RecV<XT>()> (&dy)[kRecSteps],
-                                            const float (&c)[kRecSteps][RecV<XT>()], const RecEvents &e, int row, const Channels<RecV<XT>()> &own,
+                                            const Tile &t, const Coefficients &c, const RecEvents &e, int row, const Channels<RecV<XT>()> &own,
                                             double (&a)[RecV<XT>()], float (&s)[RecV<XT>()]) {
   constexpr int V = RecV<XT>();
 #pragma unroll
@@ -506,12 +529,30 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
     if (EVENTS && (e.last >> k & 1)) LoadState<V>(s, p.a.dfinal, e.last_of[k], p.a.channels, own);
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      a[j] *= decay.Product(c[k][j], j);
-      s[j] = RecDecay<XT, GT, FORM, PER_CHANNEL>::Back(c[k][j], s[j] + dy[k][j]);
+      const float ck = c.Get(decay, t, k, j);
+      a[j] *= decay.Product(ck, j);
+      s[j] = RecDecay<XT, GT, FORM, PER_CHANNEL>::Back(ck, s[j] + dy[k][j]);
     }
   }
   return EVENTS && e.last != 0;
 }
+
+// What the second half of the backward pass needs of each step, in LDS: a thread's own places.
+template <int V> struct RecSteps {
+  struct alignas(4 * V) Step { float v[V]; };
+  Step steps[kRecSteps][kRecThreads];
+  __device__ __forceinline__ void Put(int k, const float (&b)[V]) {
+    Step s;
+#pragma unroll
+    for (int j = 0; j < V; j++) s.v[j] = b[j];
+    steps[k][threadIdx.x] = s;
+  }
+  __device__ __forceinline__ void Get(int k, float (&b)[V]) const {
+    const Step s = steps[k][threadIdx.x];
+#pragma unroll
+    for (int j = 0; j < V; j++) b[j] = s.v[j];
+  }
+};
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackward {
   static constexpr int V = RecV<XT>();
@@ -519,40 +560,57 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
   typedef typename Forward::Decay Decay;
   typedef typename Forward::Tile Tile;
 
+  __device__ static __forceinline__ void Repack(Tile &t) {
+    if constexpr (!PER_CHANNEL) {
+#pragma unroll
+      for (int k = 0; k < kRecSteps; k++) t.g[k].Repack();
+    }
+  }
   template <bool EVENTS>
   __device__ static __forceinline__ void Process(const RecKernelArgs &p, const RecLane<XT> &lane, RecShared<RecChannels<XT>()> (&shared)[2], const Decay &decay,
                                                  Tile &t, Group<XT, V> (&dy)[kRecSteps], const RecPlace &place, const RecMarks &marks, int tile, int channel_tile,
-                                                 const float (&saved)[V], float (&sum)[V]) {
+                                                 const float (&saved)[V], float (&sum)[V], RecSteps<V> &before) {
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = EventsOf(marks, lane.Stretch());
-    float c[kRecSteps][V], s[V], state[V], back[V];
+    RecCoefficients<Decay, Tile, PER_CHANNEL, false> c;
+    float s[V], state[V], back[V];
     double a[V];
+    // the states first, from the one in front of the tile: x and what its scan needs are then done with
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
-    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
-    r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, c, e, row, lane.own, a, s);
+    {
+      const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
+#pragma unroll
+      for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
+      Repack(t);
+      __syncthreads();
+      // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
+      lane.template Start<false, EVENTS>(shared[0], front, saved, state);
+    }
+#pragma unroll
+    for (int k = 0; k < kRecSteps; k++) {
+      if (EVENTS && !(e.live >> k & 1)) continue;
+      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
+      float b[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float x = t.x[k][j], ck = c.Get(decay, t, k, j);
+        b[j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
+        state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-ck, b[j], state[j]) : Decay::Step(ck, x, state[j]);
+      }
+      before.Put(k, b);
+    }
+    Repack(t);
+    r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, t, c, e, row, lane.own, a, s);
     const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
 #pragma unroll
-    for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
+    for (int k = 0; k < kRecSteps; k++) dy[k].Repack();
+    Repack(t);
     __syncthreads();
     // the last row's sequence goes on behind the tile
     const int last_row = limit - 1 - place.row;
     const bool needs = EVENTS ? limit > place.row && marks.live[last_row] && marks.last[last_row] < 0 : place.row + kRecTile < place.end;
     FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
-    // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
-    lane.template Start<false, EVENTS>(shared[0], front, saved, state);
-    float before[kRecSteps][V];
-#pragma unroll
-    for (int k = 0; k < kRecSteps; k++) {
-      if (EVENTS && !(e.live >> k & 1)) continue;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        const float x = t.x[k][j];
-        before[k][j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
-        state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-c[k][j], before[k][j], state[j]) : Decay::Step(c[k][j], x, state[j]);
-      }
-    }
     __syncthreads();
     if (lane.Idle()) return;
     float in[V];
@@ -563,38 +621,40 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 #pragma unroll
     for (int k = kRecSteps - 1; k >= 0; k--) {
       if (EVENTS && row + k >= limit) continue;
-      float dx[V] = {}, dg[V] = {};
+      float dx[V] = {}, dg[V] = {}, b[V];
+      before.Get(k, b);
       const bool live = !EVENTS || (e.live >> k & 1);
       if (live) {
         if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, e.last_of[k], p.a.channels, lane.own);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          const float l = back[j] + dy[k][j];
+          const float l = back[j] + dy[k][j], ck = c.Get(decay, t, k, j);
           if (FORM == DALIAMD_RECURRENCE_GATE) {
-            dx[j] = c[k][j] * l;
-            dg[j] = Decay::Back(c[k][j], dx[j]) * before[k][j];   // (1 - f) L, then times f
+            dx[j] = ck * l;
+            dg[j] = Decay::Back(ck, dx[j]) * b[j];   // (1 - f) L, then times f
           } else {
             dx[j] = l;
-            dg[j] = l * before[k][j];
+            dg[j] = l * b[j];
           }
           if (PER_CHANNEL) sum[j] += dg[j];
-          back[j] = Decay::Back(c[k][j], l);
+          back[j] = Decay::Back(ck, l);
         }
         if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, e.first_of[k], p.a.channels, lane.own);
       }
       const int64_t at = (int64_t)(place.row + k) * p.a.channels;
-      lane.own.Store(static_cast<XT *>(p.a.dx) + at + offset, dx);
-      if (!PER_CHANNEL) lane.own.Store(static_cast<GT *>(p.a.ddecay) + at + offset, dg);
+      lane.own.Store(static_cast<XT *>(p.a.dx) + at, dx, offset);
+      if (!PER_CHANNEL) lane.own.Store(static_cast<GT *>(p.a.ddecay) + at, dg, offset);
     }
     if (!EVENTS && place.row == place.begin && lane.Stretch() == 0) StoreState<V>(p.a.dinitial, back, place.sequence, p.a.channels, lane.own);
   }
 };
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
-__global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKernelArgs p) {
+__global__ __launch_bounds__(kRecThreads, kBackwardWaves) void RecurrenceBackwardKernel(RecKernelArgs p) {
   typedef RecBackward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared[2];
+  __shared__ RecSteps<V> before;
   __shared__ int slot;
   int tile, channel_tile;
   TakeTile<true>(p, &slot, &tile, &channel_tile);
@@ -620,10 +680,10 @@ __global__ __launch_bounds__(kRecThreads, 2) void RecurrenceBackwardKernel(RecKe
   const typename Op::Decay decay(p.a, lane.own);
   place.Find(p);
   if (place.interior) {
-    Op::template Process<false>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum);
+    Op::template Process<false>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum, before);
   } else {
     Mark(p, place, marks);
-    Op::template Process<true>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum);
+    Op::template Process<true>(p, lane, shared, decay, t, dy, place, marks, tile, channel_tile, saved, sum, before);
   }
   PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.dfinal, p.a.dinitial);
   if (PER_CHANNEL) {

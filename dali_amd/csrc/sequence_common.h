@@ -107,9 +107,9 @@ template <int V, bool WHOLE = false> struct Channels {
     end = min(V, channels);
   }
   // (32 bits of bytes: a row that is the same in all lanes stays in scalar registers)
-  template <typename T> __device__ __forceinline__ T *At(T *row) const {
+  template <typename T> __device__ __forceinline__ T *At(T *row, uint32_t offset = 0) const {
     typedef typename std::conditional<std::is_const<T>::value, const char, char>::type Byte;
-    return reinterpret_cast<T *>(reinterpret_cast<Byte *>(row) + (uint32_t)base * (uint32_t)sizeof(T));
+    return reinterpret_cast<T *>(reinterpret_cast<Byte *>(row) + ((uint32_t)base + offset) * (uint32_t)sizeof(T));
   }
   template <typename T> __device__ __forceinline__ void Load(Group<T, V> &g, const T *row) const {
     if (narrow) {
@@ -137,15 +137,16 @@ template <int V, bool WHOLE = false> struct Channels {
       }
     }
   }
-  template <typename T> __device__ __forceinline__ void Store(T *row, const float *f) const {
+  // offset: elements that lanes are apart by already
+  template <typename T> __device__ __forceinline__ void Store(T *row, const float *f, uint32_t offset = 0) const {
     if constexpr (WHOLE) {
-      if (begin == 0) StoreWide<T, V>(At(row), f);
+      if (begin == 0) StoreWide<T, V>(At(row, offset), f);
     } else if (begin == 0 && end == V) {
-      StoreWide<T, V>(At(row), f);
+      StoreWide<T, V>(At(row, offset), f);
     } else {
 #pragma unroll
       for (int j = 0; j < V; j++)
-        if (j >= begin && j < end) At(row)[j] = FromFloat<T>(f[j]);
+        if (j >= begin && j < end) At(row, offset)[j] = FromFloat<T>(f[j]);
     }
   }
 };
