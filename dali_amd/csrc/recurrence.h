@@ -29,7 +29,18 @@
 //
 // The backward pass runs through the tiles from the last to the first.  It does not use y: the states are computed again in 32
 // bits from the one in front of each tile, which the forward pass saves (1/256 of the rows), in the same tile as the L_t: x, decay
-// and dy are read once, and with 16-bit types no h is a rounded one.
+// and dy are read once, and with 16-bit types no h is a rounded one.  The states come first; of them the second half needs h_{t-1}
+// (gates: h_{t-1} - x_t), which waits in LDS, 64 KB, because registers decide how many workgroups a compute unit holds; for the same
+// reason coefficients are computed again from the decays (4 times) rather than kept.
+//
+// Measured (bf16, 8 sequences of 4096 steps, 2048 channels; a copy of 1 GiB runs at 5138 GB/s on the same card): forward 110 us for
+// 403 MB, 3.7 TB/s; backward 196 us for 671 MB, 3.4 TB/s (225 us with everything in 204 registers and one workgroup per compute
+// unit).  What bounds it is how much is on its way at once: of the 10.6 us that a workgroup of the forward pass lives, its loads take
+// 2.4, the scan 3 and the chain 3.3, and there are two per compute unit; without the chain it takes 85 us.  Tried and slower: tiles of
+// 64 and of 512 rows; three workgroups per compute unit (80 registers); workgroups that stay and load the next tile meanwhile (they
+// hold a place in the chain that they do not work on); a chain that all waves listen to; two levels of groups; equal sequences step
+// by step (each tile's predecessor long done, but rows far apart in memory at a time).  Products of decays in 32 bits take the same
+// time: vector issue is not the bound.
 #ifndef DALI_AMD_CSRC_RECURRENCE_H_
 #define DALI_AMD_CSRC_RECURRENCE_H_
 
