@@ -75,6 +75,7 @@ daliamdResult_t daliamdBlockNormBackwardRun(daliamdStream_t stream, const daliam
                   "daliamdBlockNormBackwardRun: NULL gradient");
   DALIAMD_REQUIRE(workspace_bytes >= plan.backward_workspace_bytes && (workspace || !plan.backward_workspace_bytes),
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNormBackwardRun: the workspace is too small");
+  DALIAMD_REQUIRE((uintptr_t)workspace % 16 == 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdBlockNormBackwardRun: the workspace must start at a multiple of 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   const bool weights = a.post_weight || a.scale || a.pre_weight;
   float *partial = weights ? static_cast<float *>(workspace) : nullptr;

@@ -507,6 +507,7 @@ daliamdResult_t daliamdEmbeddingBackwardRun(daliamdStream_t stream, const daliam
                   "daliamdEmbeddingBackwardRun: NULL tensor");
   DALIAMD_REQUIRE(workspace_bytes >= plan.backward_workspace_bytes && (workspace || !plan.backward_workspace_bytes),
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdEmbeddingBackwardRun: the workspace is too small");
+  DALIAMD_REQUIRE((uintptr_t)workspace % 16 == 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdEmbeddingBackwardRun: the workspace must start at a multiple of 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   const daliamdEmbeddingArgs &a = *args;
   const EmbLayout l = LayOut(a, workspace);

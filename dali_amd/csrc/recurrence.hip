@@ -144,6 +144,7 @@ daliamdResult_t daliamdRecurrenceRun(daliamdStream_t stream, const daliamdRecurr
   DALIAMD_REQUIRE(q.rows == 0 || (args->x && args->decay && args->y), DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceRun: NULL tensor");
   DALIAMD_REQUIRE(workspace_bytes >= l.forward_bytes && (workspace || !l.forward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceRun: the workspace is too small");
+  DALIAMD_REQUIRE((uintptr_t)workspace % 16 == 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceRun: the workspace must start at a multiple of 16 bytes");
   if (!q.sequences) return DALIAMD_SUCCESS;
   hipStream_t s = (hipStream_t)stream;
   if (l.initial_copy) {
@@ -171,6 +172,7 @@ daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const dalia
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: NULL tensor");
   DALIAMD_REQUIRE(workspace_bytes >= l.backward_bytes && (workspace || !l.backward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceBackwardRun: the workspace is too small");
+  DALIAMD_REQUIRE((uintptr_t)workspace % 16 == 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: the workspace must start at a multiple of 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   l.k.few_steps = false;
   ClearChain(s, l);

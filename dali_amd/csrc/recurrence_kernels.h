@@ -621,10 +621,11 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 #pragma unroll
     for (int k = kRecSteps - 1; k >= 0; k--) {
       if (EVENTS && row + k >= limit) continue;
-      float dx[V] = {}, dg[V] = {}, b[V];
-      before.Get(k, b);
+      float dx[V] = {}, dg[V] = {};
       const bool live = !EVENTS || (e.live >> k & 1);
       if (live) {
+        float b[V];
+        before.Get(k, b);
         if (EVENTS && (e.last >> k & 1)) LoadState<V>(back, p.a.dfinal, e.last_of[k], p.a.channels, lane.own);
 #pragma unroll
         for (int j = 0; j < V; j++) {

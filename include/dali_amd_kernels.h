@@ -753,12 +753,13 @@ DALIAMD_API daliamdResult_t daliamdNormalizeRun(daliamdStream_t stream, const da
  * mel features, token ids).  Rows are the steps of all sequences, one behind the other, `channels` values each (adjacent
  * in memory).  The reference has no counterpart; types: FLOAT, FLOAT16, BFLOAT16, arithmetic in 32 bits or more.
  *
- * Unlike the per-sample kernels above these take ONE argument struct by value: a batch is one tensor, not a table of
- * buffers.  Setup checks the arguments and says how large the workspaces have to be (pure host code); Run checks them
- * again against what it is given, enqueues, and neither allocates nor waits.
+ * Unlike the per-sample kernels above these take ONE argument struct: a batch is one tensor, not a table of buffers.
+ * Setup checks the arguments and says how large the workspaces have to be (pure host code); Run checks them
+ * again against what it is given, enqueues, and neither allocates nor waits.  Workspaces start at a multiple of 16 bytes, as
+ * device allocations do, and belong to one call at a time.
  *
  * daliamdSequenceRows: which rows belong to which sequence.
- *   dense   offsets == NULL: `sequences` blocks of `steps` rows, sequence_rows == sequences * steps.  With `lengths`
+ *   dense   offsets == NULL: `sequences` blocks of `steps` rows, rows == sequences * steps.  With `lengths`
  *           (device, [sequences]) only the first lengths[s] steps of block s are rows of the sequence;
  *   packed  offsets (device, [sequences + 1], ascending): sequence s has the rows [offsets[s], offsets[s + 1]) of `rows`.
  * Both are read on the device: values outside [0, rows] (or [0, steps]) are clamped, no row outside the tensors is ever

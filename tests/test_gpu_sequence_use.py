@@ -161,6 +161,15 @@ def test_on_another_stream(op):
     same(got, want)
 
 
+@pytest.mark.skipif(MODEL or torch.cuda.device_count() < 2, reason="needs a second device")
+@pytest.mark.parametrize("op", list(STEPS))
+def test_on_a_device_that_is_not_the_current_one(op):
+    step, inputs = STEPS[op]
+    new = inputs(305)
+    same([t.cpu() for t in step(*[t.to("cuda:1") for t in new])], [t.cpu() for t in step(*new)])
+    assert torch.cuda.current_device() == 0
+
+
 @device_only
 def test_two_calls_at_once():
     """Workgroups of both chains share the compute units; neither waits for the other."""

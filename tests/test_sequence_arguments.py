@@ -148,6 +148,29 @@ def test_embedding_setup_checks(kw, code):
     assert lib.daliamdEmbeddingBackwardRun(None, C.byref(a), None, C.c_size_t(0)) == (code or 1)
 
 
+def test_workspaces_that_are_too_small_or_not_aligned_are_refused():
+    lib = capi.kernels()
+    one = 16            # (no address is looked at)
+    a = recurrence_args(rows=1000, steps=1000, sequences=1, x=one, decay=one, y=one, dx=one, ddecay=one, saved=one)
+    plan = capi.RecurrencePlan()
+    assert lib.daliamdRecurrenceSetup(C.byref(a), C.byref(plan)) == 0
+    b = capi.EmbeddingArgs(tokens=4, vocab=9, channels=16, dtype=capi.FLOAT, out_dtype=capi.FLOAT, index_dtype=capi.INT64, ids=one, dout=one, dtable=one)
+    plan_b = capi.EmbeddingPlan()
+    assert lib.daliamdEmbeddingSetup(C.byref(b), C.byref(plan_b)) == 0
+    n = capi.BlockNormArgs(rows=4, channels=16, dtype=capi.FLOAT, residual_dtype=capi.FLOAT, weight_dtype=capi.FLOAT, x=one, dx=one, post_weight=one,
+                           dpost_weight=one, rstd_post=one)
+    plan_n = capi.BlockNormPlan()
+    assert lib.daliamdBlockNormSetup(C.byref(n), C.byref(plan_n)) == 0
+    for run, args, size in (("daliamdRecurrenceRun", a, plan.forward_workspace_bytes), ("daliamdRecurrenceBackwardRun", a, plan.backward_workspace_bytes),
+                            ("daliamdEmbeddingBackwardRun", b, plan_b.backward_workspace_bytes),
+                            ("daliamdBlockNormBackwardRun", n, plan_n.backward_workspace_bytes)):
+        assert size > 0
+        for workspace, given, message in ((4096, size - 1, b"too small"), (None, size, b"too small"), (4096 + 8, size, b"multiple of 16")):
+            assert getattr(lib, run)(None, C.byref(args), workspace and C.c_void_p(workspace), C.c_size_t(given)) == 1
+            lib.daliamdGetLastErrorMessage.restype = C.c_char_p
+            assert message in lib.daliamdGetLastErrorMessage(), run
+
+
 def test_struct_sizes_match_the_c_header(tmp_path):
     import os
     import subprocess
