@@ -416,7 +416,13 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
 }
 
 constexpr bool kKeepForward = true;
-constexpr int kForwardWaves = 4, kBackwardWaves = 4;
+constexpr int kForwardWaves = 4;
+// Waves per SIMD that the backward pass' registers are to leave room for: two workgroups per compute unit.  16-bit rows with
+// decays of 32 bits do not fit (272 bytes spilled: 236 us against 142 for 8 x 4096 x 1024 with one): one.
+template <typename XT, typename GT, bool PER_CHANNEL> constexpr int BackwardWaves() { return !PER_CHANNEL && sizeof(GT) > sizeof(XT) ? 2 : 4; }
+// Where registers do not decide, the tile's product is said before its states are computed, and coefficients are kept: nothing else
+// covers the chain with one workgroup per compute unit (142 : 149 us), and float rows with decays per channel fit (113 : 117 us).
+template <typename XT, typename GT, bool PER_CHANNEL> constexpr bool BackwardChainFirst() { return PER_CHANNEL ? sizeof(XT) == 4 : sizeof(GT) > sizeof(XT); }
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForward {
   static constexpr int V = RecV<XT>();
@@ -573,44 +579,51 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = EventsOf(marks, lane.Stretch());
-    RecCoefficients<Decay, Tile, PER_CHANNEL, false> c;
+    constexpr bool kChainFirst = BackwardChainFirst<XT, GT, PER_CHANNEL>();
+    RecCoefficients<Decay, Tile, PER_CHANNEL, kChainFirst> c;
     float s[V], state[V], back[V];
     double a[V];
-    // the states first, from the one in front of the tile: x and what its scan needs are then done with
+    // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
+    auto states = [&](const RecFront<V> &front) {
+      lane.template Start<false, EVENTS>(shared[0], front, saved, state);
+#pragma unroll
+      for (int k = 0; k < kRecSteps; k++) {
+        if (EVENTS && !(e.live >> k & 1)) continue;
+        if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
+        float b[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float x = t.x[k][j], ck = c.Get(decay, t, k, j);
+          b[j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
+          state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-ck, b[j], state[j]) : Decay::Step(ck, x, state[j]);
+        }
+        before.Put(k, b);
+      }
+    };
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
-    {
-      const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
+    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
+    if constexpr (!kChainFirst) {   // x and what its scan needs are then done with
 #pragma unroll
       for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
       Repack(t);
       __syncthreads();
-      // h_{t-1}, or with gates h_{t-1} - x_t: what the decay's gradient takes
-      lane.template Start<false, EVENTS>(shared[0], front, saved, state);
+      states(front);
+      Repack(t);
     }
-#pragma unroll
-    for (int k = 0; k < kRecSteps; k++) {
-      if (EVENTS && !(e.live >> k & 1)) continue;
-      if (EVENTS && (e.first >> k & 1)) LoadState<V>(state, p.a.initial, e.first_of[k], p.a.channels, lane.own);
-      float b[V];
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        const float x = t.x[k][j], ck = c.Get(decay, t, k, j);
-        b[j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
-        state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-ck, b[j], state[j]) : Decay::Step(ck, x, state[j]);
-      }
-      before.Put(k, b);
-    }
-    Repack(t);
     r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, t, c, e, row, lane.own, a, s);
     const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
 #pragma unroll
-    for (int k = 0; k < kRecSteps; k++) dy[k].Repack();
-    Repack(t);
+    for (int k = 0; k < kRecSteps; k++) {
+      if (kChainFirst) t.x[k].Repack();
+      dy[k].Repack();
+    }
+    if (!kChainFirst) Repack(t);
     __syncthreads();
     // the last row's sequence goes on behind the tile
     const int last_row = limit - 1 - place.row;
     const bool needs = EVENTS ? limit > place.row && marks.live[last_row] && marks.last[last_row] < 0 : place.row + kRecTile < place.end;
     FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
+    if constexpr (kChainFirst) states(front);
     __syncthreads();
     if (lane.Idle()) return;
     float in[V];
@@ -651,7 +664,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 };
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
-__global__ __launch_bounds__(kRecThreads, kBackwardWaves) void RecurrenceBackwardKernel(RecKernelArgs p) {
+__global__ __launch_bounds__(kRecThreads, (BackwardWaves<XT, GT, PER_CHANNEL>())) void RecurrenceBackwardKernel(RecKernelArgs p) {
   typedef RecBackward<XT, GT, FORM, PER_CHANNEL> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared[2];
