@@ -31,7 +31,8 @@
 // bits from the one in front of each tile, which the forward pass saves (1/256 of the rows), in the same tile as the L_t: x, decay
 // and dy are read once, and with 16-bit types no h is a rounded one.  The states come first; of them the second half needs h_{t-1}
 // (gates: h_{t-1} - x_t), which waits in LDS, 64 KB, because registers decide how many workgroups a compute unit holds; for the same
-// reason coefficients are computed again from the decays (4 times) rather than kept.
+// reason coefficients are computed again from the decays (4 times) rather than kept.  (BackwardChainFirst names the types for which
+// registers do not decide, and the chain comes first.)
 //
 // Measured (bf16, 8 sequences of 4096 steps, 2048 channels; a copy of 1 GiB runs at 5138 GB/s on the same card): forward 110 us for
 // 403 MB, 3.7 TB/s; backward 196 us for 671 MB, 3.4 TB/s (225 us with everything in 204 registers and one workgroup per compute
