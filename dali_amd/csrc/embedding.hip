@@ -279,7 +279,8 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
   if (begin >= end) return;
   const uint32_t vocab = (uint32_t)p.vocab;
   const bool from_before = begin > 0 && s.key[begin - 1] == s.key[begin];
-  const bool goes_on = end < n && s.key[end] == s.key[end - 1];
+  // (not if these are tokens that take no part: the last real run ends in front of them)
+  const bool goes_on = end < n && s.key[end] == s.key[end - 1] && s.key[end] < vocab;
   constexpr int kAhead = 8;   // rows in flight
   for (int c = (int)threadIdx.x % s.tpr * kEmbV; c < p.channels; c += s.tpr * kEmbV) {
     const Channels<kEmbV, WHOLE> m(c, p.channels);
