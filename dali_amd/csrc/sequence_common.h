@@ -198,20 +198,24 @@ __device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int ro
 }
 
 // The logistic function f(g) = 1 / (1 + exp(-g)) in the instructions that the hardware has for it: 2^x and 1 / x, each good to the
-// last bit or two.  The product with log2(e) is off by 2^-24 of itself, which is |g| 2^-24 of the power; EXACT puts that back.
-template <bool EXACT> __device__ __forceinline__ float ExpOf(float g) {
+// last bit or two.  The product with log2(e) is off by 2^-24 of itself, which is |g| 2^-24 of the power; EXACT puts that back
+// where the power is neither 0 nor infinity: there g may be infinite, or its product with log2(e).
+__device__ __forceinline__ float PowerOf2(float v) {
 #if defined(__AMDGCN__)
+  return __builtin_amdgcn_exp2f(v);
+#else
+  return exp2f(v);
+#endif
+}
+template <bool EXACT> __device__ __forceinline__ float ExpOf(float g) {
   constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
   const float p = g * kLog2e;
-  float t = __builtin_amdgcn_exp2f(p);
+  float t = PowerOf2(p);
   if (EXACT) {
     const float more = t * (fmaf(g, kLog2e, -p) * kLn2);
-    t += t < __builtin_inff() ? more : 0.0f;
+    t += t > 0.0f && t < __builtin_inff() ? more : 0.0f;
   }
   return t;
-#else
-  return (float)exp((double)g);
-#endif
 }
 __device__ __forceinline__ float Reciprocal(float v) {
 #if defined(__AMDGCN__)

@@ -9,8 +9,9 @@ import pytest
 import torch
 
 from dali_amd import _capi as capi
+from dali_amd import sequence
 from tests import sequence_reference as R
-from tests.test_gpu_sequence import BF, F, HF
+from tests.test_gpu_sequence import BF, F, HF, decays, leaf, rand, run_recurrence
 
 MODEL = bool(os.environ.get("DALI_AMD_HIPEMU"))
 pytestmark = pytest.mark.gpu
@@ -54,3 +55,50 @@ def test_embedding_every_row_is_written_whatever_excluded_tokens_are_behind(coun
             got = embedding_gradient(ids.cuda(), dout, vocab, padding=-1 if behind == "outside" else 7).cpu()
             want = torch.zeros(vocab, channels).index_add_(0, ids[:real], host[:real])
             assert torch.equal(got, want), (place, run, (got != want).any(1).nonzero().flatten().tolist())
+
+
+# ------------------------------------------------------------------ gates at the ends of their type
+def ends(dtype):
+    return [float("-inf"), float("inf"), torch.finfo(dtype).min, torch.finfo(dtype).max]
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("dtype,gdtype", [(F, F), (BF, BF), (BF, F), (HF, HF), (HF, F)])
+@pytest.mark.parametrize("steps", [1, 3, 300])
+def test_recurrence_gates_at_the_ends_of_their_type(steps, dtype, gdtype, train):
+    """f is 0 at -infinity and at the lowest value, 1 at the other end: no value of a gate makes a NaN."""
+    x, g = rand(500, 2, steps, 24, dtype=dtype), decays(501, "gate", 2, steps, 24, dtype=gdtype)
+    pick = np.random.default_rng(502).integers(0, 8, g.shape)
+    for k, v in enumerate(ends(gdtype)):
+        g[torch.from_numpy(pick == k).cuda()] = v
+    run_recurrence(x, g, "gate", R.ranges(2 * steps, 2, steps), rand(503, 2, 24), train)
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+def test_recurrence_gates_per_channel_at_the_ends_of_their_type(dtype):
+    g = decays(504, "gate", 24, dtype=dtype)
+    g[:4] = torch.tensor(ends(dtype), dtype=dtype)
+    run_recurrence(rand(505, 2, 300, 24, dtype=dtype), g, "gate", R.ranges(600, 2, 300), rand(506, 2, 24), True)
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+@pytest.mark.parametrize("post", [False, True])
+def test_block_norm_gates_at_the_ends_of_their_type(post, dtype):
+    """g silu'(g) and silu(g) at the lowest and the largest value, the former with the norm in front as well (with the latter its sums
+    would not fit); at infinity the product is infinite."""
+    gate = rand(510, 5, 40, dtype=dtype)
+    gate[1, 3], gate[2] = torch.finfo(dtype).min, torch.finfo(dtype).min
+    if not post:
+        gate[3, ::2], gate[4, 7] = torch.finfo(dtype).max, torch.finfo(dtype).max
+    x, dh = (rand(511 + k, 5, 40, scale=0.2).clamp(-0.9, 0.9).to(dtype) for k in (0, 1))
+    w = rand(513, 40, dtype=dtype) if post else None
+    leaves = [leaf(x), leaf(gate)]
+    h, _ = sequence.block_norm(leaves[0], gate=leaves[1], post_weight=w)
+    dx, dgate = torch.autograd.grad(h, leaves, dh)
+    ref = R.block_norm(R.f64(x), R.f64(gate), post=R.f64(w), dh=R.f64(dh))
+    R.check("hidden", h, ref["h"], dtype, ref["h_slack"])
+    R.check("dx", dx, ref["dx"], dtype, ref["dx_slack"])
+    R.check("dgate", dgate, ref["dgate"], dtype, ref["dgate_slack"])
+    gate[4, 9] = float("inf")
+    h, _ = sequence.block_norm(x, gate=gate)
+    assert torch.isinf(h[4, 9]) and torch.signbit(h[4, 9]) == torch.signbit(x[4, 9]) and not torch.isnan(h).any()
