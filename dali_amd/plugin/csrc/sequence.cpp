@@ -3,9 +3,12 @@
 // 80 to 150 us of the host's time for a forward and a backward pass.
 //
 // The kernel library is not linked but bound at run time (bind()), so that the module has no HIP runtime of its own choosing.
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <optional>
 #include "dali_amd_kernels.h"
@@ -105,6 +108,24 @@ void CheckDevice(const char *name, const Tensor &t, const Tensor &x) {
 }
 void CheckDevice(const char *name, const Maybe &t, const Tensor &x) {
   if (t) CheckDevice(name, *t, x);
+}
+// What looks at a call through torch's operators sees the outputs' allocation and not the kernels that write them: a trace would
+// hold the former alone, a tangent would be lost.
+void CheckNotTraced(const char *what) {
+  const bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                      (c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                       c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+  TORCH_CHECK(!traced, what, " cannot be traced: its kernels are not torch operators");
+}
+void CheckNoTangent(const char *what, const Tensor &t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+void CheckNoTangent(const char *what, const Maybe &t) {
+  if (t) CheckNoTangent(what, *t);
+}
+template <typename... T> void CheckSeen(const char *what, const T &...inputs) {
+  CheckNotTraced(what);
+  (CheckNoTangent(what, inputs), ...);
 }
 
 // ---- plumbing ------------------------------------------------------------------------------------------------------------
@@ -209,6 +230,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
     const auto v = ctx->get_saved_variables();
     const Tensor &x = v[0], &decay = v[1], &initial = v[2], &offsets = v[3], &lengths = v[4], &saved = v[5];
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(6);
+    CheckSeen("linear_recurrence", grads[0], grads[1]);
     at::AutoDispatchBelowADInplaceOrView below;
     OnDevice on(x);
     daliamdRecurrenceArgs a = RecurrenceArgs(x, decay, initial, offsets, lengths, ctx->saved_data["form"].toInt());
@@ -237,6 +259,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
 
 std::tuple<Tensor, Tensor> Recurrence(const Tensor &x0, const Tensor &decay0, const std::string &form_name, const Maybe &initial_state, const Maybe &offsets,
                                       const Maybe &lengths, const Maybe &final_state) {
+  CheckSeen("linear_recurrence", x0, decay0, initial_state);
   TORCH_CHECK_VALUE(form_name == "decay" || form_name == "gate", "form must be \"decay\" or \"gate\", got \"", form_name, "\"");
   const int64_t form = form_name == "gate" ? DALIAMD_RECURRENCE_GATE : DALIAMD_RECURRENCE_DECAY;
   CheckValues("x", x0);
@@ -338,6 +361,7 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
     const NormTensors t = {v[0], v[1], v[2], v[3], v[4], v[5]};
     const Tensor &rstd = v[6];
     if (!grads[0].defined() && !(grads.size() > 1 && grads[1].defined())) return variable_list(7);
+    CheckSeen("block_norm", grads[0], grads.size() > 1 ? grads[1] : Tensor());
     at::AutoDispatchBelowADInplaceOrView below;
     OnDevice on(t.x);
     daliamdBlockNormArgs a = BlockNormArgs(t, ctx->saved_data["eps"].toDouble());
@@ -364,6 +388,7 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
 };
 
 std::tuple<Tensor, Maybe> BlockNorm(const Tensor &x, const Maybe &gate, const Maybe &residual, const Maybe &post, const Maybe &scale, const Maybe &pre, double eps) {
+  CheckSeen("block_norm", x, gate, residual, post, scale, pre);
   CheckValues("x", x);
   TORCH_CHECK_VALUE(x.dim() >= 1, "x must be [..., channels]");
   const int64_t channels = x.size(-1);
@@ -443,6 +468,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto v = ctx->get_saved_variables();
     const Tensor &table = v[0], &ids = v[1];
+    CheckSeen("embedding_lookup", grads[0]);
     at::AutoDispatchBelowADInplaceOrView below;
     OnDevice on(table);
     daliamdEmbeddingArgs a = EmbeddingArgs(ids, table, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
@@ -459,6 +485,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
 };
 
 Tensor Embedding(const Tensor &ids0, const Tensor &table0, double scale, std::optional<int64_t> padding_idx, std::optional<at::ScalarType> dtype) {
+  CheckSeen("embedding_lookup", table0);
   CheckValues("table", table0);
   TORCH_CHECK_VALUE(table0.dim() == 2 && table0.size(0) >= 1 && table0.size(1) >= 1 && table0.size(0) < ((int64_t)1 << 31) && table0.size(1) <= (1 << 24),
                     "table must be [vocab, channels], got the shape ", Shape(table0.sizes()));

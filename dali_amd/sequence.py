@@ -10,6 +10,9 @@ All arithmetic happens in libdali_amd_kernels.so (include/dali_amd_kernels.h); t
 the tensors' device and nothing waits; every call can be captured into a HIP graph.  A tensor that another stream is still
 writing, or that another stream goes on using, is the caller's to order, as with any torch operator.
 
+Gradients are backward ones, of first order.  Forward-mode derivatives, a second differentiation and tracing (torch.jit.trace, make_fx)
+are refused: they would not see the kernels.
+
 Results do not depend on the order in which the device runs things: the same inputs give the same bits."""
 import importlib.util
 import os

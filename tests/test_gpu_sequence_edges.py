@@ -7,6 +7,9 @@ import os
 import numpy as np
 import pytest
 import torch
+import torch._decomp.decompositions_for_jvp  # noqa: F401  (what make_dual would load where torch's factories are patched)
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from dali_amd import _capi as capi
 from dali_amd import sequence
@@ -102,3 +105,57 @@ def test_block_norm_gates_at_the_ends_of_their_type(post, dtype):
     gate[4, 9] = float("inf")
     h, _ = sequence.block_norm(x, gate=gate)
     assert torch.isinf(h[4, 9]) and torch.signbit(h[4, 9]) == torch.signbit(x[4, 9]) and not torch.isnan(h).any()
+
+
+# ------------------------------------------------------------------ what would not see the kernels
+def calls():
+    """name: (a function of tensors that have a derivative, the tensors)"""
+    ids = torch.tensor([3, 0, 3]).cuda()
+    x, g, w = rand(520, 2, 5, 8), rand(521, 2, 5, 8), rand(522, 8)
+    return {
+        "linear_recurrence": (lambda x, g, h: sequence.linear_recurrence(x, g, form="gate", initial_state=h)[0], [x, g, rand(523, 2, 8)]),
+        "block_norm": (lambda x, g, r, w1, s, w2: sequence.block_norm(x, gate=g, residual=r, post_weight=w1, scale=s, pre_weight=w2)[1],
+                       [x, g, rand(524, 2, 5, 8), w, rand(525, 8), rand(526, 8)]),
+        "embedding_lookup": (lambda table: sequence.embedding_lookup(ids, table), [rand(527, 6, 8)]),
+    }
+
+
+@pytest.mark.parametrize("op", ["linear_recurrence", "block_norm", "embedding_lookup"])
+def test_forward_mode_is_refused(op):
+    """A tangent would be lost without a word: its place in the result is not computed."""
+    f, tensors = calls()[op]
+    want = f(*tensors)
+    for k in range(len(tensors)):
+        for leaf_too in (False, True):
+            for grad in (False, True):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    args = [t.clone().requires_grad_(leaf_too) for t in tensors]
+                    args[k] = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+                    with pytest.raises(RuntimeError, match=f"{op} has no forward-mode derivative"):
+                        f(*args)
+    assert torch.equal(f(*tensors), want)
+    # ... and so for the gradient's gradients along a tangent
+    leaves = [leaf(t) for t in tensors]
+    out = f(*leaves)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match=f"{op} has no forward-mode derivative"):
+            torch.autograd.grad(out, leaves, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("op", ["linear_recurrence", "block_norm", "embedding_lookup"])
+@pytest.mark.parametrize("leaf_too", [False, True])
+def test_tracing_is_refused(op, leaf_too):
+    """A trace would hold the outputs' allocation and not the kernels."""
+    f, tensors = calls()[op]
+    want = f(*tensors)
+    args = tuple(t.clone().requires_grad_(leaf_too) for t in tensors)
+    with pytest.raises(RuntimeError, match=f"{op} cannot be traced"):
+        torch.jit.trace(f, args, check_trace=False)
+    for pre_dispatch in (False, True):
+        with pytest.raises(RuntimeError, match=f"{op} cannot be traced"):
+            make_fx(f, pre_dispatch=pre_dispatch)(*args)
+    assert torch.equal(f(*tensors), want)
+    leaves = [leaf(t) for t in tensors]
+    out = f(*leaves)
+    with pytest.raises(RuntimeError, match=f"{op} cannot be traced"):
+        make_fx(lambda d: torch.autograd.grad(out, leaves, d))(torch.ones_like(out))
