@@ -118,7 +118,8 @@ void CheckNotTraced(const char *what) {
   TORCH_CHECK(!traced, what, " cannot be traced: its kernels are not torch operators");
 }
 void CheckNoTangent(const char *what, const Tensor &t) {
-  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+  // (without autograd's data, which a tensor has that requires a gradient or has a tangent, there is none)
+  TORCH_CHECK(!t.defined() || !t.unsafeGetTensorImpl()->autograd_meta() || !t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
 }
 void CheckNoTangent(const char *what, const Maybe &t) {
   if (t) CheckNoTangent(what, *t);
