@@ -133,8 +133,10 @@ template <typename... T> void CheckSeen(const char *what, const T &...inputs) {
 void *Ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 float *FloatPtr(const Tensor &t) { return static_cast<float *>(Ptr(t)); }
 Tensor Get(const Maybe &t) { return t ? *t : Tensor(); }
+// t with its values in memory: a view that is negated in name only (of a conjugate's imaginary part) is copied
+Tensor Dense(const Tensor &t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
 // t with adjacent channels: itself if its last dimension is dense, else a copy
-Tensor Rows(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor Rows(const Tensor &t) { return !t.is_neg() && (t.stride(-1) == 1 || t.size(-1) == 1) ? t : Dense(t); }
 // t as [rows, channels]: in place where all leading dimensions are one, else a copy
 Tensor Flat(const Tensor &t) {
   const Tensor r = Rows(t);
@@ -245,7 +247,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
       else a.dy_seq = dy.stride(0), a.dy_row = dy.stride(1);
     }
     if (grads[1].defined()) {
-      dstate = grads[1].contiguous();
+      dstate = Dense(grads[1]);
       a.dfinal = FloatPtr(dstate);
     }
     a.saved = FloatPtr(saved);
@@ -293,7 +295,7 @@ std::tuple<Tensor, Tensor> Recurrence(const Tensor &x0, const Tensor &decay0, co
     TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, name, " must be float32, got ", TypeName(t->scalar_type()));
     CheckShape(name, *t, {sequences, channels});
   }
-  TORCH_CHECK_VALUE(!final_state || final_state->is_contiguous(), "final_state must be contiguous");
+  TORCH_CHECK_VALUE(!final_state || (final_state->is_contiguous() && !final_state->is_neg()), "final_state must be contiguous, and no view that is negated in name only");
   const bool tracked = Tracked({x0, decay0, Get(initial_state)});
   TORCH_CHECK_VALUE(!(tracked && final_state), "final_state cannot be given while gradients are recorded");
   CheckDevice("x", x0, x0);
@@ -302,8 +304,8 @@ std::tuple<Tensor, Tensor> Recurrence(const Tensor &x0, const Tensor &decay0, co
   CheckDevice("offsets", offsets, x0);
   CheckDevice("lengths", lengths, x0);
   CheckDevice("final_state", final_state, x0);
-  const Tensor x = Rows(x0), decay = Rows(decay0), initial = initial_state ? initial_state->contiguous() : Tensor();
-  const Tensor off = offsets ? offsets->contiguous() : Tensor(), len = lengths ? lengths->contiguous() : Tensor();
+  const Tensor x = Rows(x0), decay = Rows(decay0), initial = initial_state ? Dense(*initial_state) : Tensor();
+  const Tensor off = offsets ? Dense(*offsets) : Tensor(), len = lengths ? Dense(*lengths) : Tensor();
   if (tracked) {
     const variable_list out = RecurrenceFunction::apply(x, decay, AsMaybe(initial), AsMaybe(off), AsMaybe(len), form);
     return {out[0], out[1]};
@@ -420,8 +422,8 @@ std::tuple<Tensor, Maybe> BlockNorm(const Tensor &x, const Maybe &gate, const Ma
   CheckDevice("post_weight", post, x);
   CheckDevice("scale", scale, x);
   CheckDevice("pre_weight", pre, x);
-  NormTensors t = {Flat(x), gate ? Flat(*gate) : Tensor(), residual ? Flat(*residual) : Tensor(), post ? post->contiguous() : Tensor(),
-                   scale ? scale->contiguous() : Tensor(), pre ? pre->contiguous() : Tensor()};
+  NormTensors t = {Flat(x), gate ? Flat(*gate) : Tensor(), residual ? Flat(*residual) : Tensor(), post ? Dense(*post) : Tensor(),
+                   scale ? Dense(*scale) : Tensor(), pre ? Dense(*pre) : Tensor()};
   Tensor hidden, normed;
   if (Tracked({t.x, t.gate, t.residual, t.post, t.scale, t.pre})) {
     const variable_list out =
@@ -502,7 +504,7 @@ Tensor Embedding(const Tensor &ids0, const Tensor &table0, double scale, std::op
   }
   CheckDevice("table", table0, table0);
   CheckDevice("ids", ids0, table0);
-  const Tensor ids = ids0.contiguous(), table = Rows(table0);
+  const Tensor ids = Dense(ids0), table = Rows(table0);
   if (Tracked({table})) return EmbeddingFunction::apply(table, ids, scale, padding, type);
   return EmbeddingForward(ids, table, scale, padding, type);
 }

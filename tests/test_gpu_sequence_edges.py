@@ -159,3 +159,60 @@ def test_tracing_is_refused(op, leaf_too):
     out = f(*leaves)
     with pytest.raises(RuntimeError, match=f"{op} cannot be traced"):
         make_fx(lambda d: torch.autograd.grad(out, leaves, d))(torch.ones_like(out))
+
+
+# ------------------------------------------------------------------ negated in name only
+def negated(t):
+    """-t as torch holds the imaginary part of a conjugate: the memory of t and a mark."""
+    return torch._neg_view(t)
+
+
+def test_views_that_are_negated_in_name_only():
+    """Every tensor of a call, and the gradients that a backward pass is given."""
+    x, g, h0 = rand(530, 2, 9, 8), rand(531, 2, 9, 8), rand(532, 2, 8)
+    dy, dlast = rand(533, 2, 9, 8), rand(534, 2, 8)
+    lengths, offsets = torch.tensor([9, 4]).cuda(), torch.tensor([0, 5, 18]).cuda()
+
+    def recurrence(form, *t, **kw):
+        leaves = [leaf(v) for v in t[:3]]
+        y, state = sequence.linear_recurrence(leaves[0], leaves[1], form=form, initial_state=leaves[2], **kw)
+        return (y, state) + torch.autograd.grad((y, state), leaves, t[3:])
+
+    t = (x, g, h0, dy, dlast)
+    for form, kw in (("gate", {"lengths": lengths}), ("decay", {})):
+        want = recurrence(form, *t, **kw)
+        got = recurrence(form, *[negated(-v) for v in t], **{k: negated(-v) for k, v in kw.items()})
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    flat = [v.reshape(18, 8) for v in (x, g)]
+    want = sequence.linear_recurrence(*flat, offsets=offsets, form="gate")
+    got = sequence.linear_recurrence(*[negated(-v) for v in flat], offsets=negated(-offsets), form="gate")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    per_channel = sequence.linear_recurrence(x, g[0, 0], form="gate")[0]
+    assert torch.equal(sequence.linear_recurrence(x, negated(-g[0, 0]), form="gate")[0], per_channel)
+    # one channel: the imaginary part of a conjugate as a program gets it
+    z = torch.complex(rand(535, 3, 7, 1), rand(536, 3, 7, 1))
+    imaginary = z.conj().imag
+    assert imaginary.is_neg()
+    assert torch.equal(sequence.linear_recurrence(imaginary, x[0, :1, 0])[0], sequence.linear_recurrence(-z.imag.contiguous(), x[0, :1, 0])[0])
+
+    def norm(*t):
+        leaves = [leaf(v) for v in t[:6]]
+        out = sequence.block_norm(leaves[0], gate=leaves[1], residual=leaves[2], post_weight=leaves[3], scale=leaves[4], pre_weight=leaves[5])
+        return out + torch.autograd.grad(out, leaves, t[6:])
+
+    t = [rand(540 + k, 5, 24) for k in range(3)] + [rand(543 + k, 24) for k in range(3)] + [rand(546 + k, 5, 24) for k in range(2)]
+    assert all(torch.equal(a, b) for a, b in zip(norm(*[negated(-v) for v in t]), norm(*t)))
+
+    def embedding(ids, table, d):
+        table = leaf(table)
+        e = sequence.embedding_lookup(ids, table)
+        return e, torch.autograd.grad(e, table, d)[0]
+
+    t = (torch.tensor([1, 0, 3, 1]).cuda(), rand(550, 4, 24), rand(551, 4, 24))
+    assert all(torch.equal(a, b) for a, b in zip(embedding(*[negated(-v) for v in t]), embedding(*t)))
+
+
+def test_a_state_that_is_negated_in_name_only_is_not_written():
+    x, state = rand(552, 2, 3, 8), negated(torch.zeros(2, 8).cuda())
+    with pytest.raises(ValueError, match="final_state"):
+        sequence.linear_recurrence(x, x, final_state=state)
