@@ -23,9 +23,10 @@
 // a number and its mark cannot be seen apart and no fence is needed (a release to the whole card would write back the L2 of an
 // XCD); the words are cleared by a launch in front.  With whole sequences in each tile (dense, at most 256 steps) there is no chain.
 //
-// 1 - f is computed and applied as such (h += (1 - f)(x - h)), and products of decays are held in 64 bits: with a gate of 0.9999
-// the rounding of f to 32 bits is an error of 3e-8 in each of ten thousand steps that still count, and with constant gates all
-// of one sign.
+// Of a gate the smaller one of f and 1 - f is computed and applied as such - h + (1 - f)(x - h), or x + f (h - x) - and products of decays
+// are held in 64 bits.  With a gate of 0.9999 the rounding of f to 32 bits is an error of 3e-8 in each of ten thousand steps that still
+// count, and with constant gates all of one sign; with a gate of 1e-9 that of 1 - f is more than f, and a large state would not go
+// away but cancel.
 //
 // The backward pass runs through the tiles from the last to the first.  It does not use y: the states are computed again in 32
 // bits from the one in front of each tile, which the forward pass saves (1/256 of the rows), in the same tile as the L_t: x, decay

@@ -320,10 +320,16 @@ __device__ __forceinline__ RecEvents EventsOf(const RecMarks &marks, int stretch
   return e;
 }
 
-// The decay of a thread's channels, as the steps use it: `a` and, for gates, `k` = 1 - a.
-template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecDecay {
+// The decay of a thread's channels, as the steps use it.  A step works with one number, its coefficient: the decay, or of a gate
+// the smaller one of f and 1 - f, negative where that is f (`shut`).  So a gate that is nearly open takes 1 - f of the input, and one that is
+// nearly shut leaves f of the state, both exactly: h + (1 - f)(x - h) is x + f (h - x).
+// COMPARE: whether a gate is shut is found by comparison.  Otherwise its sign is spread over a register, which is no shorter but leaves
+// the scalar registers alone: the backward pass, which asks four times, spills (8 x 4096 x 2048 bf16, 197 : 205 us; ragged prompts
+// 144 : 166; the forward pass 129 : 127, with float gates 82 : 78).
+template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> struct RecDecay {
   static constexpr int V = RecV<XT>();
-  float k_fixed[PER_CHANNEL ? V : 1];
+  static constexpr bool kGate = FORM == DALIAMD_RECURRENCE_GATE;
+  float c_fixed[PER_CHANNEL ? V : 1];
   double a_fixed[PER_CHANNEL ? V : 1];
 
   __device__ __forceinline__ RecDecay(const daliamdRecurrenceArgs &p, const Channels<V> &own) {
@@ -331,32 +337,52 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecDecay 
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const double g = j < own.end ? (double)LoadElement(p.decay, own.base + j, p.decay_dtype) : 0.0;
-      if (FORM == DALIAMD_RECURRENCE_GATE) {
+      if (kGate) {
         const double t = exp(-fabs(g)), big = 1 / (1 + t);
         a_fixed[j] = g < 0 ? t * big : big;
-        k_fixed[j] = (float)(g < 0 ? big : t * big);
+        c_fixed[j] = copysignf((float)(t * big), (float)g);
       } else {
         a_fixed[j] = g;
-        k_fixed[j] = (float)g;
+        c_fixed[j] = (float)g;
       }
     }
   }
-  // the number that a step works with: 1 - f, or the decay
   __device__ __forceinline__ float Coefficient(const Group<GT, V> &g, int j) const {
-    if (PER_CHANNEL) return k_fixed[j];
-    if (FORM == DALIAMD_RECURRENCE_DECAY) return g[j];
-    return OneMinusLogistic<sizeof(GT) == 4>(g[j]);
+    if (PER_CHANNEL) return c_fixed[j];
+    if (!kGate) return g[j];
+    return SmallerOfLogistic<sizeof(GT) == 4>(g[j]);
+  }
+  // all bits set if f is the smaller one (-0 as well)
+  __device__ static __forceinline__ uint32_t Shut(float coefficient) {
+    uint32_t m = (uint32_t)(__builtin_bit_cast(int32_t, coefficient) >> 31);
+#if defined(__AMDGCN__)
+    if (!COMPARE) asm("" : "+v"(m));   // (the compiler would make a comparison of it)
+#endif
+    return m;
+  }
+  __device__ static __forceinline__ float PickOf(uint32_t shut, float then, float otherwise) {
+    return BitsToFloat((__builtin_bit_cast(uint32_t, then) & shut) | (__builtin_bit_cast(uint32_t, otherwise) & ~shut));
   }
   __device__ __forceinline__ double Product(float coefficient, int j) const {
     if (PER_CHANNEL) return a_fixed[j];
-    return FORM == DALIAMD_RECURRENCE_GATE ? 1.0 - (double)coefficient : (double)coefficient;
+    if (!kGate) return (double)coefficient;
+    const uint64_t one = (uint64_t)(0x3ff00000u & ~Shut(coefficient)) << 32;   // 1, or 0 if shut
+    return __builtin_bit_cast(double, one) - (double)coefficient;
   }
   __device__ static __forceinline__ float Step(float coefficient, float x, float h) {
-    return FORM == DALIAMD_RECURRENCE_GATE ? fmaf(coefficient, x - h, h) : fmaf(coefficient, h, x);
+    return kGate ? fmaf(coefficient, x - h, PickOf(Shut(coefficient), x, h)) : fmaf(coefficient, h, x);
   }
   // M = a L
   __device__ static __forceinline__ float Back(float coefficient, float l) {
-    return FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-coefficient, l, l) : coefficient * l;
+    return kGate ? fmaf(-coefficient, l, PickOf(Shut(coefficient), 0.0f, l)) : coefficient * l;
+  }
+  // of a gate: f L and (1 - f) L, which are s L and (1 - s) L with the smaller one s, and f (1 - f) L, which is s (1 - s) L either way
+  __device__ static __forceinline__ void Shares(float coefficient, float l, float *m, float *dx, float *both) {
+    const float s = fabsf(coefficient), p = s * l, q = fmaf(-s, l, l);
+    const uint32_t shut = Shut(coefficient);
+    *m = PickOf(shut, p, q);
+    *dx = PickOf(shut, q, p);
+    *both = s * q;
   }
 };
 
@@ -386,6 +412,18 @@ template <typename Decay, typename Tile, bool PER_CHANNEL, bool KEEP> struct Rec
   __device__ __forceinline__ float Get(const Decay &decay, const Tile &t, int k, int j) const {
     if constexpr (KEEP) return kept[k][j];
     else return decay.Coefficient(t.g[PER_CHANNEL ? 0 : k], j);
+  }
+  // Which of them are negative the compiler would keep as well, two scalar registers for each, which it then stores in lanes of
+  // vector registers and reads back; after this it looks again.
+  __device__ __forceinline__ void Forget() {
+#if defined(__AMDGCN__)
+    if constexpr (KEEP && !PER_CHANNEL) {
+#pragma unroll
+      for (int k = 0; k < kRecSteps; k++)
+#pragma unroll
+        for (int j = 0; j < V; j++) asm volatile("" : "+v"(kept[k][j]));
+    }
+#endif
   }
 };
 
@@ -424,9 +462,13 @@ template <typename XT, typename GT, bool PER_CHANNEL> constexpr int BackwardWave
 // covers the chain with one workgroup per compute unit (142 : 149 us), and float rows with decays per channel fit (113 : 117 us).
 template <typename XT, typename GT, bool PER_CHANNEL> constexpr bool BackwardChainFirst() { return PER_CHANNEL ? sizeof(XT) == 4 : sizeof(GT) > sizeof(XT); }
 
-template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForward {
+// The product of a stretch's gates is kept for the composition against time, not computed again; of decays and per channel it is one
+// multiplication a step, and keeping it costs registers that they do not have.
+template <int FORM, bool PER_CHANNEL> constexpr bool BackwardShared() { return FORM == DALIAMD_RECURRENCE_GATE && !PER_CHANNEL; }
+
+template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> struct RecForward {
   static constexpr int V = RecV<XT>();
-  typedef RecDecay<XT, GT, FORM, PER_CHANNEL> Decay;
+  typedef RecDecay<XT, GT, FORM, PER_CHANNEL, COMPARE> Decay;
   typedef RecTile<XT, GT, PER_CHANNEL> Tile;
 
   // (A, S, R) of a thread's stretch
@@ -460,6 +502,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
+    c.Forget();
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
     if (!PER_CHANNEL && !kKeepForward) {
@@ -499,7 +542,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecForwar
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL>
 __global__ __launch_bounds__(kRecThreads, kForwardWaves) void RecurrenceForwardKernel(RecKernelArgs p) {
-  typedef RecForward<XT, GT, FORM, PER_CHANNEL> Op;
+  typedef RecForward<XT, GT, FORM, PER_CHANNEL, true> Op;
   constexpr int V = RecV<XT>();
   __shared__ RecShared<RecChannels<XT>()> shared;
   __shared__ int slot;
@@ -521,14 +564,17 @@ __global__ __launch_bounds__(kRecThreads, kForwardWaves) void RecurrenceForwardK
   PassEmpty<V>(p, tile, lane.Stretch(), lane.own, p.a.initial, p.a.final_state);
 }
 
-// (A, S, R) of a thread's stretch against time; dy NULL: zeros
-template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool EVENTS, typename Tile, typename Coefficients>
-__device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDecay<XT, GT, FORM, PER_CHANNEL> &decay, const Group<XT, RecV<XT>()> (&dy)[kRecSteps],
+// (A, S, R) of a thread's stretch against time; dy NULL: zeros; SHARED: A is there, the product of the same decays
+template <typename XT, bool EVENTS, bool SHARED, typename Decay, typename Tile, typename Coefficients>
+__device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const Decay &decay, const Group<XT, RecV<XT>()> (&dy)[kRecSteps],
                                             const Tile &t, const Coefficients &c, const RecEvents &e, int row, const Channels<RecV<XT>()> &own,
                                             double (&a)[RecV<XT>()], float (&s)[RecV<XT>()]) {
   constexpr int V = RecV<XT>();
 #pragma unroll
-  for (int j = 0; j < V; j++) a[j] = 1.0, s[j] = 0.0f;
+  for (int j = 0; j < V; j++) {
+    s[j] = 0.0f;
+    if (!SHARED) a[j] = 1.0;
+  }
 #pragma unroll
   for (int k = kRecSteps - 1; k >= 0; k--) {
     if (EVENTS && !(e.live >> k & 1)) continue;
@@ -536,8 +582,8 @@ __device__ __forceinline__ bool ComposeBack(const RecKernelArgs &p, const RecDec
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const float ck = c.Get(decay, t, k, j);
-      a[j] *= decay.Product(ck, j);
-      s[j] = RecDecay<XT, GT, FORM, PER_CHANNEL>::Back(ck, s[j] + dy[k][j]);
+      if (!SHARED) a[j] *= decay.Product(ck, j);
+      s[j] = Decay::Back(ck, s[j] + dy[k][j]);
     }
   }
   return EVENTS && e.last != 0;
@@ -562,7 +608,7 @@ template <int V> struct RecSteps {
 
 template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackward {
   static constexpr int V = RecV<XT>();
-  typedef RecForward<XT, GT, FORM, PER_CHANNEL> Forward;
+  typedef RecForward<XT, GT, FORM, PER_CHANNEL, PER_CHANNEL> Forward;
   typedef typename Forward::Decay Decay;
   typedef typename Forward::Tile Tile;
 
@@ -579,7 +625,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = EventsOf(marks, lane.Stretch());
-    constexpr bool kChainFirst = BackwardChainFirst<XT, GT, PER_CHANNEL>();
+    constexpr bool kChainFirst = BackwardChainFirst<XT, GT, PER_CHANNEL>(), kShared = BackwardShared<FORM, PER_CHANNEL>();
     RecCoefficients<Decay, Tile, PER_CHANNEL, kChainFirst> c;
     float s[V], state[V], back[V];
     double a[V];
@@ -595,13 +641,17 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
         for (int j = 0; j < V; j++) {
           const float x = t.x[k][j], ck = c.Get(decay, t, k, j);
           b[j] = FORM == DALIAMD_RECURRENCE_GATE ? state[j] - x : state[j];
-          state[j] = FORM == DALIAMD_RECURRENCE_GATE ? fmaf(-ck, b[j], state[j]) : Decay::Step(ck, x, state[j]);
+          state[j] = Decay::kGate ? fmaf(-ck, b[j], Decay::PickOf(Decay::Shut(ck), x, state[j])) : Decay::Step(ck, x, state[j]);
         }
         before.Put(k, b);
       }
     };
     bool r = Forward::template Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
+    double product[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) product[j] = a[j];
     const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
+    c.Forget();
     if constexpr (!kChainFirst) {   // x and what its scan needs are then done with
 #pragma unroll
       for (int k = 0; k < kRecSteps; k++) t.x[k].Repack(), dy[k].Repack();
@@ -610,8 +660,13 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
       states(front);
       Repack(t);
     }
-    r = ComposeBack<XT, GT, FORM, PER_CHANNEL, EVENTS>(p, decay, dy, t, c, e, row, lane.own, a, s);
+    r = ComposeBack<XT, EVENTS, kShared>(p, decay, dy, t, c, e, row, lane.own, a, s);
+    if (kShared) {
+#pragma unroll
+      for (int j = 0; j < V; j++) a[j] = product[j];
+    }
     const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
+    c.Forget();
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
       if (kChainFirst) t.x[k].Repack();
@@ -623,7 +678,10 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     const int last_row = limit - 1 - place.row;
     const bool needs = EVENTS ? limit > place.row && marks.live[last_row] && marks.last[last_row] < 0 : place.row + kRecTile < place.end;
     FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
-    if constexpr (kChainFirst) states(front);
+    if constexpr (kChainFirst) {
+      states(front);
+      c.Forget();
+    }
     __syncthreads();
     if (lane.Idle()) return;
     float in[V];
@@ -644,14 +702,15 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
         for (int j = 0; j < V; j++) {
           const float l = back[j] + dy[k][j], ck = c.Get(decay, t, k, j);
           if (FORM == DALIAMD_RECURRENCE_GATE) {
-            dx[j] = ck * l;
-            dg[j] = Decay::Back(ck, dx[j]) * b[j];   // (1 - f) L, then times f
+            float both;
+            Decay::Shares(ck, l, &back[j], &dx[j], &both);
+            dg[j] = both * b[j];
           } else {
             dx[j] = l;
             dg[j] = l * b[j];
+            back[j] = Decay::Back(ck, l);
           }
           if (PER_CHANNEL) sum[j] += dg[j];
-          back[j] = Decay::Back(ck, l);
         }
         if (EVENTS && (e.first >> k & 1)) StoreState<V>(p.a.dinitial, back, e.first_of[k], p.a.channels, lane.own);
       }
@@ -735,7 +794,8 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArg
   const int channel = (int)(id - s * groups) * V, n = min(p.a.channels - channel, V);
   Channels<V> own(channel, p.a.channels);
   if (n < V) own.base = channel, own.begin = 0, own.end = n, own.narrow = true;
-  const RecDecay<XT, GT, FORM, PER_CHANNEL> decay(p.a, own);
+  typedef RecDecay<XT, GT, FORM, PER_CHANNEL, true> Decay;
+  const Decay decay(p.a, own);
   int begin, end;
   SequenceRange(p.a.seq, (int)s, &begin, &end);
   const int steps = (int)p.a.seq.steps, length = end - begin;
@@ -751,7 +811,7 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArg
       own.Load(x, px + (own.narrow ? own.base : 0));
       if (!PER_CHANNEL) own.Load(g, pg + (own.narrow ? own.base : 0));
 #pragma unroll
-      for (int j = 0; j < V; j++) h[j] = RecDecay<XT, GT, FORM, PER_CHANNEL>::Step(decay.Coefficient(g, j), x[j], h[j]);
+      for (int j = 0; j < V; j++) h[j] = Decay::Step(decay.Coefficient(g, j), x[j], h[j]);
       own.Store(y, h);
     } else {
       const float zero[V] = {};

@@ -230,8 +230,10 @@ __device__ __forceinline__ void LogisticPair(float g, float *f, float *k) {
   *f = g < 0 ? small : big;
   *k = g < 0 ? big : small;
 }
-// 1 - f alone
-template <bool EXACT> __device__ __forceinline__ float OneMinusLogistic(float g) { return Reciprocal(1.0f + ExpOf<EXACT>(g)); }
+// The smaller one of f and 1 - f to its last bits, negative where that is f: of the other, which is near 1, it is all that matters.
+template <bool EXACT> __device__ __forceinline__ float SmallerOfLogistic(float g) {
+  return copysignf(Reciprocal(1.0f + ExpOf<EXACT>(fabsf(g))), g);
+}
 // g f(g)
 __device__ __forceinline__ float Silu(float g) { return g * Reciprocal(1.0f + ExpOf<true>(-g)); }
 

@@ -216,3 +216,81 @@ def test_a_state_that_is_negated_in_name_only_is_not_written():
     x, state = rand(552, 2, 3, 8), negated(torch.zeros(2, 8).cuda())
     with pytest.raises(ValueError, match="final_state"):
         sequence.linear_recurrence(x, x, final_state=state)
+
+
+# ------------------------------------------------------------------ gates of all sizes, element by element
+def elementwise(x, g, spans, initial, dy, dlast, per_step):
+    """The gate form in 64 bits with a bound for each element by itself.  H and L are the same sums of absolute values: what a state or a
+    gradient is made of.  A step's arithmetic is off by per_step 2^-24 of what it adds up, and passes on f of the error it is given; the
+    pieces that a sequence is cut into are joined by 16 further roundings, each of such a sum."""
+    rows, c = x.shape
+    one = g.ndim == 1
+    f, k = R.logistic(g)
+    at = (lambda t: f) if one else (lambda t: f[t])
+    kt = (lambda t: k) if one else (lambda t: k[t])
+    out = R.recurrence(x, g, "gate", spans, initial, dy, dlast)
+    e = {n: np.zeros((rows, c)) for n in ("y", "dx", "dg")}
+    e["state"], e["dinitial"] = np.zeros((len(spans), c)), np.zeros((len(spans), c))
+    u, join = per_step * R.U, 16 * R.U
+    for s, (b, end) in enumerate(spans):
+        h = np.zeros(c) if initial is None else np.abs(initial[s])
+        err, before = np.zeros(c), []
+        for t in range(b, end):
+            before.append((h, err + join * h))
+            grown = at(t) * h + kt(t) * np.abs(x[t])
+            h, err = grown, at(t) * err + u * grown
+            e["y"][t] = err + join * h
+        e["state"][s] = err + join * h
+        m, err = np.abs(dlast[s]), np.zeros(c)
+        for t in range(end - 1, b - 1, -1):
+            l = m + np.abs(dy[t])   # noqa: E741
+            err = err + u * l
+            seen = err + join * l
+            hb, eb = before[t - b]
+            e["dx"][t] = kt(t) * (seen + u * l)
+            reach = hb + np.abs(x[t])
+            e["dg"][t] = at(t) * kt(t) * (seen * reach + l * (eb + u * reach))
+            m, err = at(t) * l, at(t) * (err + u * l)
+        e["dinitial"][s] = err + join * m
+    if one:   # a sum over the rows in 32 bits
+        terms = np.zeros((rows, c))
+        for b, end in spans:
+            m = np.abs(dlast[spans.index((b, end))])
+            for t in range(end - 1, b - 1, -1):
+                l = m + np.abs(dy[t])   # noqa: E741
+                terms[t] = f * k * l * np.abs(np.abs(x[t]) + (np.abs(out["y"][t - 1]) if t > b else np.abs(initial[spans.index((b, end))])))
+                m = f * l
+        e["dg"] = e["dg"].sum(0) + (32 + rows / 256) * R.U * terms.sum(0)
+    return out, e
+
+
+@pytest.mark.parametrize("dtype,gdtype", [(F, F), (BF, BF), (BF, F), (HF, HF), (F, "per channel")])
+@pytest.mark.parametrize("low,high", [(-40, -4), (-40, 40), (3, 12), (-2, 2)])
+@pytest.mark.parametrize("batch,steps", [(2, 300), (3, 3), (1, 1100)])
+def test_recurrence_gates_of_all_sizes(batch, steps, low, high, dtype, gdtype):
+    """A gate that is nearly shut leaves f of the state in front, as exactly as one that is nearly open leaves 1 - f of the input: x is
+    large at some steps and small at others, and each result is compared with what it is made of, not with the largest one."""
+    c, rows = 24, batch * steps
+    rng = np.random.default_rng(560)
+    one = gdtype == "per channel"
+    gdtype = F if one else gdtype
+    spread = 2 if dtype == HF else 5       # (float16 ends at 65504)
+    wide = lambda *shape: torch.from_numpy(rng.normal(size=shape) * 10.0 ** rng.uniform(-spread, spread, shape))  # noqa: E731
+    x = wide(batch, steps, c).clamp(-1e4, 1e4).to(dtype).cuda()
+    g = torch.from_numpy(rng.uniform(low, high, (c,) if one else (batch, steps, c))).to(gdtype).cuda()
+    h0, dy, dlast = wide(batch, c).float().cuda(), rand(561, batch, steps, c, dtype=dtype), rand(562, batch, c)
+    leaves = [leaf(t) for t in (x, g, h0)]
+    y, state = sequence.linear_recurrence(leaves[0], leaves[1], form="gate", initial_state=leaves[2])
+    dx, dg, dinitial = torch.autograd.grad((y, state), leaves, (dy, dlast))
+    flat = lambda t: R.f64(t).reshape(rows, c)  # noqa: E731
+    # 12: the logistic function (exp with two, 1 + t, its reciprocal, their product), the step, a product of two; 16-bit gates leave out
+    # the rounding of g log2(e), which is |g| 2^-24 of the power
+    per_step = 12 + (0 if gdtype == F else max(abs(low), abs(high)))
+    ref, e = elementwise(flat(x), R.f64(g) if one else flat(g), R.ranges(rows, batch, steps), R.f64(h0), flat(dy), R.f64(dlast), per_step)
+    # (2^-126: a power below the smallest normal number may be taken for 0; times what it multiplies, at most 1e8)
+    for name, got, t in (("y", y, dtype), ("state", state, F), ("dx", dx, dtype), ("dg", dg, gdtype), ("dinitial", dinitial, F)):
+        R.check(name, got.reshape(ref[name].shape), ref[name], t, e[name] + 2.0 ** -99)
+    # and without gradients, where a thread goes through a few steps by itself
+    z, last = sequence.linear_recurrence(x, g, form="gate", initial_state=h0)
+    R.check("y", z.reshape(rows, c), ref["y"], dtype, e["y"] + 2.0 ** -99)
+    R.check("state", last, ref["state"], F, e["state"] + 2.0 ** -99)
