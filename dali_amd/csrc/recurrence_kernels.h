@@ -45,6 +45,11 @@ template <int CH> struct RecShared {
   float front[CH];              // the state in front of the tile
 };
 
+// A product of decays, kept finite: of more than 1 in size, hundreds of them pass the 64 bits' range, and infinity times a state of 0
+// (or a decay of 0) is NaN.  Any other state is infinite in 32 bits long before.  (Those of one stretch are within the range.)
+// GATES: none is more than 1.
+template <bool GATES> __device__ __forceinline__ double Bounded(double a) { return GATES ? a : fmin(fmax(a, -1e300), 1e300); }
+
 // A stretch's place in its wave's scan: what is in front of it inside the wave.
 template <int V> struct RecFront {
   double a[V];
@@ -68,7 +73,7 @@ template <typename XT> struct RecLane {
 
   // Scan over the stretches of a wave, in the order of time or (REV) against it; a, s, r: of this thread's stretch.  The wave's
   // own product goes to `shared`.  MAY_RESET false: no r is set.
-  template <bool REV, bool MAY_RESET>
+  template <bool REV, bool MAY_RESET, bool GATES>
   __device__ __forceinline__ RecFront<V> ScanWave(RecShared<CH> &shared, double (&a)[V], float (&s)[V], bool r) const {
     const int order = REV ? kRecPieces - 1 - piece : piece;
     bool any = r;
@@ -82,7 +87,7 @@ template <typename XT> struct RecLane {
         const float s1 = REV ? __shfl_down(s[j], d * kRecLanes, 64) : __shfl_up(s[j], d * kRecLanes, 64);
         if (have && !(MAY_RESET && any)) {
           s[j] = (float)fma(a[j], (double)s1, (double)s[j]);
-          a[j] *= a1;
+          a[j] = Bounded<GATES>(a[j] * a1);
         }
       }
       if (MAY_RESET && have) any |= before;
@@ -137,7 +142,7 @@ __device__ __forceinline__ float Value(uint64_t word) { return BitsToFloat((uint
 
 // For one channel of the workgroup's tile (`place`: its place among all tiles' channels): finds the state in front of the tile and says what is behind it.  a, s, r: of the
 // whole tile; `known`: nothing in front counts but `state`.  Returns the state in front.
-template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int place, double a, float s, bool r, bool known, float state) {
+template <bool REV, bool GATES> __device__ __forceinline__ float Chain(const RecKernelArgs &p, int tile, int64_t width, int place, double a, float s, bool r, bool known, float state) {
   uint64_t *mine = p.words + ((int64_t)tile * width + place) * kRecWords;
   const bool joint = (REV ? p.tiles - 1 - tile : tile) % kRecGroup == kRecGroup - 1;
   if (r || known) {
@@ -174,7 +179,7 @@ template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &
         go = false;
       } else if (Said(w[k][1]) && Said(w[k][2]) && Said(w[k][3])) {
         ps = (float)fma(pa, (double)Value(w[k][1]), (double)ps);
-        pa *= __builtin_bit_cast(double, (uint64_t)(uint32_t)w[k][2] << 32 | (uint32_t)w[k][3]);
+        pa = Bounded<GATES>(pa * __builtin_bit_cast(double, (uint64_t)(uint32_t)w[k][2] << 32 | (uint32_t)w[k][3]));
         moved++;
       } else {
         go = false;
@@ -190,7 +195,7 @@ template <bool REV> __device__ __forceinline__ float Chain(const RecKernelArgs &
 
 // The state in front of the tile into shared.front: by the first threads, one per channel.  initial: of `sequence` where that
 // begins with the tile (REV: ends with it); `needs`: the row in front belongs to the same sequence.
-template <bool REV, typename XT>
+template <bool REV, bool GATES, typename XT>
 __device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecChannels<XT>()> &shared, int tile, int channel_tile, bool needs,
                                           const float *initial, int sequence) {
   constexpr int CH = RecChannels<XT>();
@@ -208,11 +213,11 @@ __device__ __forceinline__ void FindFront(const RecKernelArgs &p, RecShared<RecC
     const float ws = shared.s[w][threadIdx.x];
     const bool forget = shared.r[w] != 0;
     s = forget ? ws : (float)fma(wa, (double)s, (double)ws);
-    a *= wa;
+    a = Bounded<GATES>(a * wa);
     r |= forget;
   }
   const float state = initial && sequence >= 0 && channel < p.a.channels ? initial[(int64_t)sequence * p.a.channels + channel] : 0.0f;
-  shared.front[threadIdx.x] = p.chained ? Chain<REV>(p, tile, (int64_t)p.channel_tiles * CH, channel_tile * CH + (int)threadIdx.x, a, s, r, !needs, state) : state;
+  shared.front[threadIdx.x] = p.chained ? Chain<REV, GATES>(p, tile, (int64_t)p.channel_tiles * CH, channel_tile * CH + (int)threadIdx.x, a, s, r, !needs, state) : state;
 }
 
 // the workgroup's tile: in the order of the chain
@@ -501,7 +506,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> st
     float s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
-    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared, a, s, r);
+    const RecFront<V> front = lane.template ScanWave<false, EVENTS, Decay::kGate>(shared, a, s, r);
     c.Forget();
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
@@ -511,7 +516,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> st
     }
     __syncthreads();
     const bool starts = place.sequence < 0 || place.row == place.begin;
-    FindFront<false, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
+    FindFront<false, Decay::kGate, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);
     __syncthreads();
     if (lane.Idle()) return;
     float in[V];
@@ -650,7 +655,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     double product[V];
 #pragma unroll
     for (int j = 0; j < V; j++) product[j] = a[j];
-    const RecFront<V> front = lane.template ScanWave<false, EVENTS>(shared[0], a, s, r);
+    const RecFront<V> front = lane.template ScanWave<false, EVENTS, Decay::kGate>(shared[0], a, s, r);
     c.Forget();
     if constexpr (!kChainFirst) {   // x and what its scan needs are then done with
 #pragma unroll
@@ -665,7 +670,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
 #pragma unroll
       for (int j = 0; j < V; j++) a[j] = product[j];
     }
-    const RecFront<V> behind = lane.template ScanWave<true, EVENTS>(shared[1], a, s, r);
+    const RecFront<V> behind = lane.template ScanWave<true, EVENTS, Decay::kGate>(shared[1], a, s, r);
     c.Forget();
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) {
@@ -677,7 +682,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecBackwa
     // the last row's sequence goes on behind the tile
     const int last_row = limit - 1 - place.row;
     const bool needs = EVENTS ? limit > place.row && marks.live[last_row] && marks.last[last_row] < 0 : place.row + kRecTile < place.end;
-    FindFront<true, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
+    FindFront<true, Decay::kGate, XT>(p, shared[1], tile, channel_tile, needs, EVENTS ? nullptr : p.a.dfinal, place.sequence);
     if constexpr (kChainFirst) {
       states(front);
       c.Forget();

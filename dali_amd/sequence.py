@@ -53,7 +53,9 @@ def linear_recurrence(x, decay, *, form="decay", initial_state=None, offsets=Non
     x              [batch, steps, channels], or [rows, channels] with `offsets`: float32, float16 or bfloat16.  Adjacent
                    channels have to be adjacent in memory (a copy is made otherwise), rows may be any distance apart, as in
                    a slice of a wider projection.
-    decay          of x's shape, or [channels]: the same at every step (exponential smoothing); x's type or float32.
+    decay          of x's shape, or [channels]: the same at every step (exponential smoothing); x's type or float32.  Decays of
+                   more than 1 in size are computed as well, but pieces of a sequence are composed: a state that stays small
+                   only because what such decays make of its past is taken away again by x loses its digits.
     initial_state  h_0, float32 [sequences, channels]; zeros if None.  To go on with a sequence pass the state of the call
                    before: one step at a time gives what one call over all steps gives, up to rounding.
     offsets        int32 or int64 [sequences + 1], ascending, on the device: sequence s has the rows offsets[s] up to

@@ -294,3 +294,28 @@ def test_recurrence_gates_of_all_sizes(batch, steps, low, high, dtype, gdtype):
     z, last = sequence.linear_recurrence(x, g, form="gate", initial_state=h0)
     R.check("y", z.reshape(rows, c), ref["y"], dtype, e["y"] + 2.0 ** -99)
     R.check("state", last, ref["state"], F, e["state"] + 2.0 ** -99)
+
+
+# ------------------------------------------------------------------ decays of more than 1
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("decay", [100.0, -3e38])
+@pytest.mark.parametrize("steps", [7, 512, 1800])
+def test_recurrence_large_decays_of_a_state_that_is_zero(steps, decay, one):
+    """A state of 0 stays 0 under any decay, however large the product of many of them; in both directions of time."""
+    x, g = torch.zeros(2, steps, 24).cuda(), torch.full((24,) if one else (2, steps, 24), decay).cuda()
+    x[:, -1 if one else -2] = rand(570, 2, 24)
+    if not one:
+        g[0, steps // 3, ::2], g[1, 3, ::3] = 0.0, 0.0     # (a product of infinity and 0 is none either)
+        g[:, -1] = 0.5
+    leaves = [leaf(x), leaf(g)]
+    y, state = sequence.linear_recurrence(*leaves)
+    dy = torch.zeros_like(y)
+    dy[:, 0] = rand(571, 2, 24)
+    dx, dg = torch.autograd.grad((y, state), leaves, (dy, torch.zeros_like(state)))
+    ref = R.recurrence(R.f64(x).reshape(-1, 24), R.f64(g) if one else R.f64(g).reshape(-1, 24), "decay", R.ranges(2 * steps, 2, steps), None,
+                       R.f64(dy).reshape(-1, 24), np.zeros((2, 24)))
+    for name, got in (("y", y), ("state", state), ("dx", dx), ("dg", dg)):
+        want = ref[name]
+        assert np.isfinite(want).all()
+        # a product or two of numbers that are not 0, and nothing added to them
+        R.check(name, got.reshape(want.shape), want, F, 4 * R.U * np.abs(want))
