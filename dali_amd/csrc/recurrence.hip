@@ -101,8 +101,10 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   const uint8_t *initial = reinterpret_cast<const uint8_t *>(a.initial), *final_state = reinterpret_cast<const uint8_t *>(a.final_state);
   k.few_steps = FewSteps(a);
   l.forward_bytes = used;
-  // tiles read initial states while others write final ones
-  if (initial && final_state && !k.few_steps && initial < final_state + states && final_state < initial + states) {
+  // Initial states are read while others' final ones are written; only where a thread has all of a state, and writes it where it read it,
+  // that is no matter.
+  const bool overlap = initial && final_state && initial < final_state + states && final_state < initial + states;
+  if (overlap && !(k.few_steps && initial == final_state)) {
     const size_t before = used;
     l.initial_copy = reinterpret_cast<float *>(take(states));
     l.forward_bytes = used;

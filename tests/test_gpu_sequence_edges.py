@@ -319,3 +319,20 @@ def test_recurrence_large_decays_of_a_state_that_is_zero(steps, decay, one):
         assert np.isfinite(want).all()
         # a product or two of numbers that are not 0, and nothing added to them
         R.check(name, got.reshape(want.shape), want, F, 4 * R.U * np.abs(want))
+
+
+# ------------------------------------------------------------------ states that share memory
+@pytest.mark.parametrize("shift", [-1, 0, 1, 3])
+@pytest.mark.parametrize("steps", [1, 4, 5, 300])
+def test_recurrence_states_that_overlap(steps, shift):
+    """The final states in the memory of the initial ones, or some rows off it: what is read is what was there before the call."""
+    n, c = 40, 72
+    x, g = rand(580, n, steps, c, dtype=BF), decays(581, "gate", n, steps, c, dtype=BF)
+    memory = rand(582, n + 4, c)
+    start = max(-shift, 0)
+    initial = memory[start:start + n].clone()
+    want, last = sequence.linear_recurrence(x, g, form="gate", initial_state=initial)
+    rest = memory.clone()
+    rest[start + shift:start + shift + n] = last
+    y, state = sequence.linear_recurrence(x, g, form="gate", initial_state=memory[start:start + n], final_state=memory[start + shift:start + shift + n])
+    assert torch.equal(y, want) and torch.equal(state, last) and torch.equal(memory, rest)
