@@ -57,16 +57,16 @@ static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
   return DALIAMD_SUCCESS;
 }
 
-// Tiles and workspaces: a function of sizes and types alone, so that the backward pass finds what the forward pass saved.
+// Tiles and workspaces: a function of sizes, types and of whether the states share memory, so that the backward pass finds what the
+// forward pass saved, and Setup names what Run takes.
 struct RecLayout {
   RecKernelArgs k;
   float *initial_copy;
   size_t chain_bytes, saved_bytes, forward_bytes, backward_bytes;
 };
-// a few steps per sequence and nothing to save: one thread goes through a sequence's steps
-static bool FewSteps(const daliamdRecurrenceArgs &a) {
-  return !a.seq.offsets && a.seq.steps > 0 && a.seq.steps <= kRecFewSteps && !a.saved;
-}
+// A few steps per sequence: one thread goes through a sequence's steps.  There is nothing to save then: each tile has whole sequences,
+// several of them, so nothing in front of it is the state of one that it has rows of.
+static bool FewSteps(const daliamdRecurrenceArgs &a) { return !a.seq.offsets && a.seq.steps > 0 && a.seq.steps <= kRecFewSteps; }
 static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   RecLayout l = {};
   RecKernelArgs &k = l.k;
@@ -84,7 +84,8 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   k.x_plain = plain(a.x_row, a.x_seq, e);
   k.decay_plain = plain(a.decay_row, a.decay_seq, d);
   k.dy_plain = plain(a.dy_row, a.dy_seq, e);
-  l.saved_bytes = sizeof(float) * (size_t)k.tiles * a.channels;
+  k.few_steps = FewSteps(a);
+  l.saved_bytes = k.few_steps ? 0 : sizeof(float) * (size_t)k.tiles * a.channels;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   size_t used = 0;
   auto take = [&](size_t bytes) {
@@ -99,7 +100,6 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   }
   const size_t states = sizeof(float) * (size_t)q.sequences * a.channels;
   const uint8_t *initial = reinterpret_cast<const uint8_t *>(a.initial), *final_state = reinterpret_cast<const uint8_t *>(a.final_state);
-  k.few_steps = FewSteps(a);
   l.forward_bytes = used;
   // Initial states are read while others' final ones are written; only where a thread has all of a state, and writes it where it read it,
   // that is no matter.
@@ -170,13 +170,14 @@ daliamdResult_t daliamdRecurrenceBackwardRun(daliamdStream_t stream, const dalia
   if (daliamdResult_t r = CheckRecurrence(args)) return r;
   const daliamdSequenceRows &q = args->seq;
   RecLayout l = LayOut(*args, workspace);
-  DALIAMD_REQUIRE((args->ddecay || (q.rows == 0 && !args->per_channel)) && (q.rows == 0 || (args->x && args->decay && args->dx && args->saved)),
+  DALIAMD_REQUIRE((args->ddecay || (q.rows == 0 && !args->per_channel)) && (q.rows == 0 || (args->x && args->decay && args->dx && (args->saved || !l.saved_bytes))),
                   DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: NULL tensor");
   DALIAMD_REQUIRE(workspace_bytes >= l.backward_bytes && (workspace || !l.backward_bytes), DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrenceBackwardRun: the workspace is too small");
   DALIAMD_REQUIRE((uintptr_t)workspace % 16 == 0, DALIAMD_ERROR_INVALID_ARGUMENT, "daliamdRecurrenceBackwardRun: the workspace must start at a multiple of 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   l.k.few_steps = false;
+  if (!l.saved_bytes) l.k.a.saved = nullptr;
   ClearChain(s, l);
   if (args->dtype == DALIAMD_FLOAT) LaunchRecurrenceBackward<float>(s, l.k);
   else if (args->dtype == DALIAMD_FLOAT16) LaunchRecurrenceBackward<F16>(s, l.k);

@@ -782,14 +782,15 @@ enum { DALIAMD_SEQUENCE_MAX_ROWS = 0x7fff0000, DALIAMD_RECURRENCE_MAX_CHANNELS =
  * decay: [rows][channels] in x's type or FLOAT, or [channels] with per_channel (same for every step).
  * Backward: from dy and dfinal (NULL: zero) the gradients of x, decay (per_channel: summed over all rows) and initial.
  * `saved` is written by a forward pass that a backward pass follows (states at the starts of the kernels' row tiles;
- * plan.saved_bytes) and read by the latter with the same x, decay and initial. */
+ * plan.saved_bytes, none for dense sequences of a few steps) and read by the latter with the same x, decay and initial.
+ * Of the tensors Setup looks at initial and final_state alone: states that share memory may have to be copied first. */
 typedef enum { DALIAMD_RECURRENCE_DECAY = 0, DALIAMD_RECURRENCE_GATE = 1 } daliamdRecurrenceForm_t;
 typedef struct {
   daliamdSequenceRows seq;
   const void *x, *decay;
   const float *initial;           /* [sequences][channels] or NULL                                      */
   void *y;                        /* dtype, dense [rows][channels]                                      */
-  float *final_state;             /* [sequences][channels] or NULL; may be the buffer `initial`         */
+  float *final_state;             /* [sequences][channels] or NULL; may be the buffer `initial`, or overlap it */
   float *saved;                   /* plan.saved_bytes or NULL (no backward pass follows)                */
   const void *dy;                 /* backward from here on: dtype                                       */
   const float *dfinal;            /* [sequences][channels] or NULL                                      */

@@ -336,3 +336,25 @@ def test_recurrence_states_that_overlap(steps, shift):
     rest[start + shift:start + shift + n] = last
     y, state = sequence.linear_recurrence(x, g, form="gate", initial_state=memory[start:start + n], final_state=memory[start + shift:start + shift + n])
     assert torch.equal(y, want) and torch.equal(state, last) and torch.equal(memory, rest)
+
+
+@pytest.mark.parametrize("steps", [1, 4, 5, 300])
+def test_recurrence_workspace_does_not_depend_on_what_setup_names(steps):
+    """C entries: the sizes that Setup gives without the tensors suffice for every Run over the same states."""
+    n, c, lib = 6, 40, capi.kernels()
+    x, g, state = rand(583, n, steps, c), decays(584, "gate", n, steps, c), rand(585, n, c)
+    before = state.clone()
+    a, plan = capi.RecurrenceArgs(), capi.RecurrencePlan()
+    a.seq.rows, a.seq.steps, a.seq.sequences = n * steps, steps, n
+    a.x_row, a.x_seq, a.decay_row, a.decay_seq = c, steps * c, c, steps * c
+    a.channels, a.dtype, a.decay_dtype, a.form = c, capi.FLOAT, capi.FLOAT, capi.RECURRENCE_GATE
+    a.initial = a.final_state = state.data_ptr()
+    capi.check(lib.daliamdRecurrenceSetup(C.byref(a), C.byref(plan)))
+    y, ws = torch.empty_like(x), torch.empty(max(plan.forward_workspace_bytes, 16), dtype=torch.uint8).cuda()
+    saved = torch.empty(max(plan.saved_bytes, 16), dtype=torch.uint8).cuda()
+    a.x, a.decay, a.y, a.saved = x.data_ptr(), g.data_ptr(), y.data_ptr(), saved.data_ptr()
+    capi.check(lib.daliamdRecurrenceRun(C.c_void_p(torch.cuda.current_stream().cuda_stream), C.byref(a), C.c_void_p(ws.data_ptr()),
+                                        C.c_size_t(plan.forward_workspace_bytes)))
+    torch.cuda.synchronize()
+    want, last = sequence.linear_recurrence(x, g, form="gate", initial_state=before)
+    assert torch.equal(y, want) and torch.equal(state, last)
