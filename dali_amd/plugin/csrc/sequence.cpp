@@ -441,17 +441,18 @@ std::tuple<Tensor, Maybe> BlockNorm(const Tensor &x, const Maybe &gate, const Ma
 }
 
 // ---- embedding lookup ----------------------------------------------------------------------------------------------------
-daliamdEmbeddingArgs EmbeddingArgs(const Tensor &ids, const Tensor &table, double scale, int64_t padding, at::ScalarType out) {
+daliamdEmbeddingArgs EmbeddingArgs(const Tensor &ids, c10::IntArrayRef table, at::ScalarType dtype, double scale, int64_t padding, at::ScalarType out) {
   daliamdEmbeddingArgs a = {};
   a.ids = Ptr(ids), a.index_dtype = DType(ids.scalar_type()), a.tokens = ids.numel();
-  a.table = Ptr(table), a.table_row = table.stride(0), a.vocab = table.size(0), a.channels = (int32_t)table.size(1);
-  a.dtype = DType(table.scalar_type()), a.out_dtype = DType(out);
+  a.vocab = table[0], a.channels = (int32_t)table[1];
+  a.dtype = DType(dtype), a.out_dtype = DType(out);
   a.padding = padding, a.scale = (float)scale;
   return a;
 }
 Tensor EmbeddingForward(const Tensor &ids, const Tensor &table, double scale, int64_t padding, at::ScalarType type) {
   OnDevice on(table);
-  daliamdEmbeddingArgs a = EmbeddingArgs(ids, table, scale, padding, type);
+  daliamdEmbeddingArgs a = EmbeddingArgs(ids, table.sizes(), table.scalar_type(), scale, padding, type);
+  a.table = Ptr(table), a.table_row = table.stride(0);
   std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
   shape.push_back(table.size(1));
   Tensor out = at::empty(shape, table.options().dtype(type));
@@ -462,26 +463,31 @@ Tensor EmbeddingForward(const Tensor &ids, const Tensor &table, double scale, in
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &table, const Tensor &ids, double scale, int64_t padding, at::ScalarType type) {
-    ctx->save_for_backward({table, ids});
+    // The gradient takes the table's size, type and device, not its values, which may change before the backward pass.
+    ctx->save_for_backward({ids});
+    ctx->saved_data["table"] = table;
+    ctx->saved_data["sizes"] = table.sizes();
+    ctx->saved_data["dtype"] = (int64_t)table.scalar_type();
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
     ctx->saved_data["type"] = (int64_t)type;
     return EmbeddingForward(ids, table, scale, padding, type);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    const auto v = ctx->get_saved_variables();
-    const Tensor &table = v[0], &ids = v[1];
+    const Tensor ids = ctx->get_saved_variables()[0], table = ctx->saved_data["table"].toTensor();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
     CheckSeen("embedding_lookup", grads[0]);
     at::AutoDispatchBelowADInplaceOrView below;
-    OnDevice on(table);
-    daliamdEmbeddingArgs a = EmbeddingArgs(ids, table, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
+    OnDevice on(ids);
+    daliamdEmbeddingArgs a = EmbeddingArgs(ids, sizes, dtype, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
                                            (at::ScalarType)ctx->saved_data["type"].toInt());
     daliamdEmbeddingPlan plan;
     Check(lib.EmbeddingSetup(&a, &plan));
     const Tensor dout = Flat(grads[0]);
-    Tensor dtable = EmptyLike(table);
+    Tensor dtable = at::empty(sizes, ids.options().dtype(dtype));
     a.dout = Ptr(dout), a.dout_row = dout.stride(0), a.dtable = Ptr(dtable);
-    const Tensor ws = Workspace(plan.backward_workspace_bytes, table);
+    const Tensor ws = Workspace(plan.backward_workspace_bytes, ids);
     Check(lib.EmbeddingBackwardRun(on.stream, &a, Ptr(ws), plan.backward_workspace_bytes));
     return Once({dtable, Tensor(), Tensor(), Tensor(), Tensor()}, {table}, grads, "embedding_lookup");
   }

@@ -358,3 +358,21 @@ def test_recurrence_workspace_does_not_depend_on_what_setup_names(steps):
     torch.cuda.synchronize()
     want, last = sequence.linear_recurrence(x, g, form="gate", initial_state=before)
     assert torch.equal(y, want) and torch.equal(state, last)
+
+
+# ------------------------------------------------------------------ embedding: a table that changes before the backward pass
+def test_embedding_table_changed_before_the_backward_pass():
+    """The gradient does not depend on the table's values: an optimizer may have stepped, as with torch's own lookup."""
+    ids, d = torch.tensor([3, 1, 3, 0]).cuda(), rand(590, 4, 24, dtype=BF)
+    table = leaf(rand(591, 5, 24, dtype=BF))
+    want, = torch.autograd.grad(sequence.embedding_lookup(ids, table, scale=2.0, padding_idx=1), table, d)
+    e = sequence.embedding_lookup(ids, table, scale=2.0, padding_idx=1)
+    with torch.no_grad():
+        table += 1
+    got, = torch.autograd.grad(e, table, d)
+    assert got.dtype == BF and torch.equal(got, want)
+    # the ids are read: to change them is an error
+    e = sequence.embedding_lookup(ids, table)
+    ids += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(e, table, d)
