@@ -463,11 +463,9 @@ Tensor EmbeddingForward(const Tensor &ids, const Tensor &table, double scale, in
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &table, const Tensor &ids, double scale, int64_t padding, at::ScalarType type) {
-    // The gradient takes the table's size, type and device, not its values, which may change before the backward pass.
+    // The gradient takes the table's size and type, not its values, which may change before the backward pass.
     ctx->save_for_backward({ids});
     ctx->saved_data["table"] = table;
-    ctx->saved_data["sizes"] = table.sizes();
-    ctx->saved_data["dtype"] = (int64_t)table.scalar_type();
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
     ctx->saved_data["type"] = (int64_t)type;
@@ -475,17 +473,16 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor ids = ctx->get_saved_variables()[0], table = ctx->saved_data["table"].toTensor();
-    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
-    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
     CheckSeen("embedding_lookup", grads[0]);
     at::AutoDispatchBelowADInplaceOrView below;
     OnDevice on(ids);
-    daliamdEmbeddingArgs a = EmbeddingArgs(ids, sizes, dtype, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
+    const Tensor dout = Flat(grads[0]);
+    const std::array<int64_t, 2> sizes = {table.size(0), dout.size(1)};
+    daliamdEmbeddingArgs a = EmbeddingArgs(ids, sizes, table.scalar_type(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
                                            (at::ScalarType)ctx->saved_data["type"].toInt());
     daliamdEmbeddingPlan plan;
     Check(lib.EmbeddingSetup(&a, &plan));
-    const Tensor dout = Flat(grads[0]);
-    Tensor dtable = at::empty(sizes, ids.options().dtype(dtype));
+    Tensor dtable = at::empty(sizes, ids.options().dtype(table.scalar_type()));
     a.dout = Ptr(dout), a.dout_row = dout.stride(0), a.dtable = Ptr(dtable);
     const Tensor ws = Workspace(plan.backward_workspace_bytes, ids);
     Check(lib.EmbeddingBackwardRun(on.stream, &a, Ptr(ws), plan.backward_workspace_bytes));
