@@ -1,4 +1,5 @@
 // Embedding lookup with a scale, and its gradient: the tokens' gradients summed per row of the table.
+#include <algorithm>
 #include "sequence_common.h"
 
 namespace daliamd {
@@ -222,6 +223,7 @@ struct EmbSums {
   const uint32_t *key, *index;
   float *part;                  // [chunks][2][part_row]: of the run that came from the chunk before, of the one that goes on behind
   int chunk, chunks, chunk_groups, tpr, part_row;
+  int64_t first;                // of a launch: the first row that it may fill with zeros, or the first chunk whose run it may join
 };
 
 // the first place whose key is not below `key`
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
   if ((int)blockIdx.x >= s.chunk_groups) {   // rows without a token
     __shared__ uint8_t none[kFillRows];
     __shared__ int bound[2];
-    const int64_t row = (int64_t)((int)blockIdx.x - s.chunk_groups) * kFillRows;
+    const int64_t row = s.first + (int64_t)((int)blockIdx.x - s.chunk_groups) * kFillRows;
     const int tid = threadIdx.x;
     if (tid < 128) {
       const int at = (int)LowerBoundOfWave(s.key, n, (uint32_t)(row + (tid >> 6) * kFillRows));
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(kEmbThreads) void EmbeddingBackwardKernel(daliamdEm
 constexpr int kJoinLanes = 64, kJoinParts = 4, kJoinColumns = kJoinLanes * 4;
 __global__ __launch_bounds__(kJoinLanes * kJoinParts) void EmbeddingJoinKernel(daliamdEmbeddingArgs p, EmbSums s) {
   __shared__ float4 part[kJoinParts][kJoinLanes];
-  const int64_t chunk = blockIdx.x, begin = chunk * s.chunk, end = begin + s.chunk;
+  const int64_t chunk = s.first + blockIdx.x, begin = chunk * s.chunk, end = begin + s.chunk;
   if (end >= p.tokens || s.key[end] != s.key[end - 1]) return;                  // nothing goes on behind this chunk
   const uint32_t key = s.key[end - 1];
   if (key >= (uint32_t)p.vocab) return;
@@ -425,11 +427,21 @@ static EmbLayout LayOut(const daliamdEmbeddingArgs &a, void *workspace) {
 }
 
 template <typename TT, typename OT> struct EmbLaunch {
-  static void Forward(hipStream_t s, const daliamdEmbeddingArgs &a) {
+  // (a second launch only for more than 2^26 tokens)
+  static void Forward(hipStream_t s, const daliamdEmbeddingArgs &all) {
     int tpr = 8;
-    while (tpr < kEmbThreads && tpr * kEmbV < a.channels) tpr *= 2;
-    const int64_t per_group = kEmbThreads / tpr;
+    while (tpr < kEmbThreads && tpr * kEmbV < all.channels) tpr *= 2;
+    const int64_t per_group = kEmbThreads / tpr, most = 4 * MaxWorkgroups(kEmbThreads) * per_group;
     KernelTimer timer("EmbeddingKernel", s);
+    for (int64_t first = 0; first < all.tokens; first += most) {
+      daliamdEmbeddingArgs a = all;
+      a.tokens = std::min(most, all.tokens - first);
+      a.ids = static_cast<const char *>(all.ids) + first * (all.index_dtype == DALIAMD_INT64 ? 8 : 4);
+      a.out = static_cast<OT *>(all.out) + first * all.channels;
+      ForwardPart(s, a, tpr, per_group);
+    }
+  }
+  static void ForwardPart(hipStream_t s, const daliamdEmbeddingArgs &a, int tpr, int64_t per_group) {
     // four rows per thread where that still leaves workgroups for every compute unit
     if (a.tokens >= 4 * per_group * 1024) ForwardOf<4>(s, a, tpr, (a.tokens + 4 * per_group - 1) / (4 * per_group));
     else ForwardOf<1>(s, a, tpr, (a.tokens + per_group - 1) / per_group);
@@ -446,11 +458,16 @@ template <typename TT, typename OT> struct EmbLaunch {
     }
   }
   static void Backward(hipStream_t s, const daliamdEmbeddingArgs &a, const EmbSums &sums) {
-    const int64_t fill = (a.vocab + kFillRows - 1) / kFillRows;
-    const dim3 grid((unsigned)(sums.chunk_groups + fill)), block(kEmbThreads);
     KernelTimer timer("EmbeddingBackwardKernel", s);
-    if (a.channels % kEmbV == 0) hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, true>), grid, block, 0, s, a, sums);
-    else hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, false>), grid, block, 0, s, a, sums);
+    EmbSums part = sums;
+    do {   // (a second launch only for more than 2^29 rows)
+      const int64_t rows = (a.vocab - part.first + kFillRows - 1) / kFillRows, fill = std::min(rows, MaxWorkgroups(kEmbThreads) - part.chunk_groups);
+      const dim3 grid((unsigned)(part.chunk_groups + fill)), block(kEmbThreads);
+      if (a.channels % kEmbV == 0) hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, true>), grid, block, 0, s, a, part);
+      else hipLaunchKernelGGL((EmbeddingBackwardKernel<TT, OT, false>), grid, block, 0, s, a, part);
+      part.first += fill * kFillRows;
+      part.chunk_groups = 0;
+    } while (part.first < a.vocab);
   }
 };
 template <typename F> static void WithTypes(const daliamdEmbeddingArgs &a, F f) {
@@ -475,7 +492,9 @@ static daliamdResult_t CheckEmbedding(const daliamdEmbeddingArgs *args, daliamdE
                   "daliamdEmbedding: table and output must be FLOAT, FLOAT16 or BFLOAT16");
   DALIAMD_REQUIRE(a.index_dtype == DALIAMD_INT32 || a.index_dtype == DALIAMD_INT64, DALIAMD_ERROR_UNSUPPORTED,
                   "daliamdEmbedding: ids must be INT32 or INT64");
-  plan->backward_workspace_bytes = LayOut(a, nullptr).bytes;
+  const EmbLayout l = LayOut(a, nullptr);
+  DALIAMD_REQUIRE(l.sums.chunk_groups < MaxWorkgroups(kEmbThreads), DALIAMD_ERROR_OUT_OF_RANGE, "daliamdEmbedding: more tokens and channels than one launch may have");
+  plan->backward_workspace_bytes = l.bytes;
   return DALIAMD_SUCCESS;
 }
 
@@ -527,8 +546,13 @@ daliamdResult_t daliamdEmbeddingBackwardRun(daliamdStream_t stream, const daliam
   if (sums.chunks > 1) {
     KernelTimer timer("EmbeddingJoinKernel", s);
     const int tiles = (a.channels + kJoinColumns - 1) / kJoinColumns;
-    hipLaunchKernelGGL(EmbeddingJoinKernel, dim3((unsigned)sums.chunks - 1, (unsigned)(tiles < 65535 ? tiles : 65535)),
-                       dim3(kJoinLanes * kJoinParts), 0, s, a, sums);
+    EmbSums part = sums;
+    while (part.first < sums.chunks - 1) {   // (a second launch only for more than 2^29 tokens)
+      const int64_t groups = std::min<int64_t>(sums.chunks - 1 - part.first, MaxWorkgroups(kJoinLanes * kJoinParts));
+      hipLaunchKernelGGL(EmbeddingJoinKernel, dim3((unsigned)groups, (unsigned)(tiles < 65535 ? tiles : 65535)), dim3(kJoinLanes * kJoinParts), 0, s, a,
+                         part);
+      part.first += groups;
+    }
   }
   DALIAMD_HIP_CHECK(hipGetLastError());
   return DALIAMD_SUCCESS;

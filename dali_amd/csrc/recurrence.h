@@ -46,6 +46,7 @@
 #ifndef DALI_AMD_CSRC_RECURRENCE_H_
 #define DALI_AMD_CSRC_RECURRENCE_H_
 
+#include <algorithm>
 #include "sequence_common.h"
 
 namespace daliamd {
@@ -61,7 +62,8 @@ struct RecKernelArgs {
   daliamdRecurrenceArgs a;
   int tile_rows;                      // kRecTile, or a little less: whole sequences
   int tiles, channel_tiles;
-  bool few_steps;                     // a thread goes through a sequence's steps
+  bool few_steps;                     // a thread goes through a sequence's steps ...
+  int first_sequence, sequences;      // ... of these
   bool chained;                       // a tile may need the state behind the one before
   bool x_plain, decay_plain, dy_plain; // rows one distance apart, those of a tile within 32 bits
   uint32_t *ticket;                   // the chain: cleared before each launch, with the words behind it

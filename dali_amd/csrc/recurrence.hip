@@ -54,6 +54,9 @@ static daliamdResult_t CheckRecurrence(const daliamdRecurrenceArgs *args) {
                   "daliamdRecurrence: decay must have x's type or be FLOAT");
   DALIAMD_REQUIRE(a.form == DALIAMD_RECURRENCE_DECAY || a.form == DALIAMD_RECURRENCE_GATE, DALIAMD_ERROR_INVALID_ARGUMENT,
                   "daliamdRecurrence: unknown form %d", a.form);
+  const int channels = kRecLanes * (kRecBytes / ElementSize(a.dtype));
+  DALIAMD_REQUIRE((a.seq.rows / kRecTile + 1) * ((a.channels + channels - 1) / channels) <= MaxWorkgroups(kRecThreads), DALIAMD_ERROR_OUT_OF_RANGE,
+                  "daliamdRecurrence: more rows and channels than one launch may have");
   return DALIAMD_SUCCESS;
 }
 
@@ -74,8 +77,10 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   const daliamdSequenceRows &q = a.seq;
   const int e = ElementSize(a.dtype), d = ElementSize(a.decay_dtype), ch = kRecLanes * (kRecBytes / e);
   k.channel_tiles = (a.channels + ch - 1) / ch;
-  const bool whole = !q.offsets && q.steps > 0 && q.steps <= kRecTile;   // whole sequences in each tile
+  // whole sequences in each tile, unless that makes more tiles (of 129 rows instead of 256) than a launch may have
+  bool whole = !q.offsets && q.steps > 0 && q.steps <= kRecTile;
   k.tile_rows = whole ? kRecTile / (int)q.steps * (int)q.steps : kRecTile;
+  if ((q.rows / k.tile_rows + 1) * k.channel_tiles > MaxWorkgroups(kRecThreads)) whole = false, k.tile_rows = kRecTile;
   k.tiles = (int)std::max<int64_t>(1, (q.rows + k.tile_rows - 1) / k.tile_rows);
   k.chained = !whole && k.tiles > 1;
   auto plain = [&](int64_t row, int64_t seq, int elem) {
@@ -84,7 +89,7 @@ static RecLayout LayOut(const daliamdRecurrenceArgs &a, void *workspace) {
   k.x_plain = plain(a.x_row, a.x_seq, e);
   k.decay_plain = plain(a.decay_row, a.decay_seq, d);
   k.dy_plain = plain(a.dy_row, a.dy_seq, e);
-  k.few_steps = FewSteps(a);
+  k.few_steps = whole && FewSteps(a);
   l.saved_bytes = k.few_steps ? 0 : sizeof(float) * (size_t)k.tiles * a.channels;
   uint8_t *at = static_cast<uint8_t *>(workspace);
   size_t used = 0;

@@ -793,14 +793,15 @@ __global__ __launch_bounds__(kRecThreads) void RecurrenceStepKernel(RecKernelArg
   constexpr int V = RecV<XT>();
   const int groups = (p.a.channels + V - 1) / V;
   const int64_t id = (int64_t)blockIdx.x * kRecThreads + threadIdx.x;
-  const int64_t s = (uint32_t)id / (uint32_t)groups;
-  if (s >= p.a.seq.sequences) return;
+  int64_t s = (uint32_t)id / (uint32_t)groups;
+  if (s >= p.sequences) return;
   // (a state may be written over the one it is read from: threads have no channels in common)
   const int channel = (int)(id - s * groups) * V, n = min(p.a.channels - channel, V);
   Channels<V> own(channel, p.a.channels);
   if (n < V) own.base = channel, own.begin = 0, own.end = n, own.narrow = true;
   typedef RecDecay<XT, GT, FORM, PER_CHANNEL, true> Decay;
   const Decay decay(p.a, own);
+  s += p.first_sequence;
   int begin, end;
   SequenceRange(p.a.seq, (int)s, &begin, &end);
   const int steps = (int)p.a.seq.steps, length = end - begin;
@@ -830,10 +831,18 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL> struct RecLaunch
   static void Forward(hipStream_t s, const RecKernelArgs &p) {
     const daliamdSequenceRows &q = p.a.seq;
     if (p.few_steps) {
-      constexpr int V = RecV<XT>();
-      const int64_t threads = (int64_t)q.sequences * ((p.a.channels + V - 1) / V);
+      const int64_t groups = (p.a.channels + RecV<XT>() - 1) / RecV<XT>();
+      const int most = (int)std::min<int64_t>(q.sequences, MaxWorkgroups(kRecThreads) * kRecThreads / groups);
       KernelTimer timer("RecurrenceStepKernel", s);
-      hipLaunchKernelGGL((RecurrenceStepKernel<XT, GT, FORM, PER_CHANNEL>), dim3((unsigned)((threads + kRecThreads - 1) / kRecThreads)), dim3(kRecThreads), 0, s, p);
+      for (int first = 0, n; first < q.sequences; first += n) {   // (a second launch only for more than 2^32 threads)
+        n = std::min(most, q.sequences - first);
+        RecKernelArgs part = p;
+        part.first_sequence = first;
+        part.sequences = n;
+        const int64_t threads = n * groups;
+        hipLaunchKernelGGL((RecurrenceStepKernel<XT, GT, FORM, PER_CHANNEL>), dim3((unsigned)((threads + kRecThreads - 1) / kRecThreads)), dim3(kRecThreads), 0, s,
+                           part);
+      }
       return;
     }
     const dim3 grid((unsigned)p.tiles * p.channel_tiles);

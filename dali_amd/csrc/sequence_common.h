@@ -161,6 +161,9 @@ __device__ __forceinline__ void StoreElement(void *p, int64_t i, int dtype, floa
   else static_cast<Bf16 *>(p)[i] = FromFloat<Bf16>(v);
 }
 
+// workgroups of `threads` that one launch may have: its threads are counted in 32 bits
+inline int64_t MaxWorkgroups(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
+
 inline bool IsSequenceType(int dtype) { return dtype == DALIAMD_FLOAT || dtype == DALIAMD_FLOAT16 || dtype == DALIAMD_BFLOAT16; }
 inline int ElementSize(int dtype) { return dtype == DALIAMD_FLOAT ? 4 : 2; }
 

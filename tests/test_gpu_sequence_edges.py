@@ -376,3 +376,87 @@ def test_embedding_table_changed_before_the_backward_pass():
     ids += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(e, table, d)
+
+
+# ------------------------------------------------------------------ more threads than one launch may have (2^32)
+def enough_memory(gigabytes):
+    if MODEL or torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
+        pytest.skip("not enough memory on the device")
+    torch.cuda.empty_cache()
+
+
+def test_embedding_of_as_many_tokens_as_there_may_be():
+    """2^31 - 1 tokens of one channel: the lookup, and the join of 2^26 chunks of 32 sorted tokens.  Counts are exact in 32 bits."""
+    enough_memory(90)
+    count, vocab = 2 ** 31 - 1, 300
+    ids = torch.empty(count, dtype=torch.int32, device="cuda").random_(0, vocab)
+    table = leaf(torch.arange(vocab).to(F).view(-1, 1).cuda())
+    e = sequence.embedding_lookup(ids, table, dtype=HF)
+    for first in range(0, count, 2 ** 28):
+        assert torch.equal(e[first:first + 2 ** 28, 0], ids[first:first + 2 ** 28].to(HF))
+    counts = torch.zeros(vocab, dtype=torch.int64, device="cuda")
+    for first in range(0, count, 2 ** 28):
+        counts += torch.bincount(ids[first:first + 2 ** 28], minlength=vocab)
+    assert int(counts.max()) < 2 ** 24
+    got, = torch.autograd.grad(e, table, torch.ones_like(e))
+    assert torch.equal(got[:, 0].long(), counts)
+
+
+def test_embedding_of_a_table_of_more_rows_than_one_launch_fills():
+    enough_memory(40)
+    vocab = 2 ** 30 + 1000
+    table = torch.empty(vocab, 2, dtype=HF, device="cuda").fill_(1).requires_grad_(True)
+    rows = torch.tensor([0, 63, 64, 2 ** 29, 2 ** 30 - 64, 2 ** 30 - 1, 2 ** 30, vocab - 1]).cuda()
+    ids = rows.repeat(700)
+    got, = torch.autograd.grad(sequence.embedding_lookup(ids, table), table, torch.ones(ids.numel(), 2, dtype=HF, device="cuda"))
+    assert (got[rows] == 700).all()
+    got[rows] = 0
+    assert not got.any()
+
+
+def test_recurrence_of_more_sequences_than_one_launch_steps_through():
+    """One step of 1.45e9 sequences of 5 channels: a thread has two channels, so three threads each."""
+    enough_memory(130)
+    n = 1_450_000_000
+    x = torch.empty(n, 1, 5, device="cuda").fill_(0.25)
+    x[-1] = 3.0
+    x[::1_000_003] = -1.0
+    g = torch.tensor([0.0, 1.0, -1.0, 0.5, 2.0]).cuda()
+    y, state = sequence.linear_recurrence(x, g)
+    assert torch.equal(y, x) and torch.equal(state, x[:, 0])
+
+
+def test_recurrence_of_more_short_sequences_than_tiles_of_their_own():
+    """8 400 000 sequences of 129 steps, of which a tile of 256 rows would have one: sums of -1, 0 and 1 with changing sign, exact in
+    every type; in both directions of time."""
+    enough_memory(60)
+    n, steps = 8_400_000, 129
+    x, dy = (torch.empty(n, steps, 1, dtype=BF, device="cuda") for _ in range(2))
+    for t in (x, dy):
+        t.random_(-1, 2)
+    a = torch.tensor([-1.0], device="cuda")
+    xs = leaf(x)
+    y, state = sequence.linear_recurrence(xs, a)
+    dx, = torch.autograd.grad(y, xs, dy)
+    sign = (1 - 2 * (torch.arange(steps, device="cuda") % 2)).to(torch.int32).view(1, steps)
+    for first in range(0, n, 2 ** 20):
+        part = slice(first, first + 2 ** 20)
+        v = x[part, :, 0].to(torch.int32) * sign
+        want = torch.cumsum(v, 1).to(torch.int32) * sign
+        assert torch.equal(y[part, :, 0].to(torch.int32), want) and torch.equal(state[part, 0].to(torch.int32), want[:, -1])
+        d = (dy[part, :, 0].to(torch.int32) * sign).flip(1)
+        assert torch.equal(dx[part, :, 0].to(torch.int32), (torch.cumsum(d, 1).to(torch.int32)).flip(1) * sign)
+
+
+def test_more_rows_and_channels_than_one_launch_may_have_are_refused():
+    lib, plan = capi.kernels(), capi.RecurrencePlan()
+    a = capi.RecurrenceArgs()
+    a.seq.rows = a.seq.steps = 0x7fff0000
+    a.seq.sequences, a.channels, a.dtype, a.decay_dtype = 1, 32, capi.FLOAT, capi.FLOAT
+    assert lib.daliamdRecurrenceSetup(C.byref(a), C.byref(plan)) == 0
+    a.channels = 33
+    assert lib.daliamdRecurrenceSetup(C.byref(a), C.byref(plan)) == 3
+    b, plan_b = capi.EmbeddingArgs(tokens=2 ** 31 - 1, vocab=9, channels=1024, dtype=capi.FLOAT, out_dtype=capi.FLOAT, index_dtype=capi.INT64), capi.EmbeddingPlan()
+    assert lib.daliamdEmbeddingSetup(C.byref(b), C.byref(plan_b)) == 3
+    b.channels = 64
+    assert lib.daliamdEmbeddingSetup(C.byref(b), C.byref(plan_b)) == 0
