@@ -4,21 +4,22 @@
 
 namespace daliamd {
 
-// per-channel gradients: the tiles' sums, in a fixed order
+// Per-channel gradients: the tiles' sums, in a fixed order and in 64 bits, since there are as many as there are rows by the hundred and
+// their errors would be of the size of all rows' sum.
 constexpr int kRecSumColumns = 16, kRecSumParts = 16;
 __global__ __launch_bounds__(kRecSumColumns * kRecSumParts) void RecurrenceChannelSumKernel(RecKernelArgs p) {
-  __shared__ float part[kRecSumParts][kRecSumColumns];
+  __shared__ double part[kRecSumParts][kRecSumColumns];
   const int column = threadIdx.x % kRecSumColumns, k = threadIdx.x / kRecSumColumns, c = blockIdx.x * kRecSumColumns + column;
-  float sum = 0;
+  double sum = 0;
   if (c < p.a.channels) {
 #pragma unroll 8
-    for (int n = k; n < p.tiles; n += kRecSumParts) sum += p.partial[(int64_t)n * p.a.channels + c];
+    for (int n = k; n < p.tiles; n += kRecSumParts) sum += (double)p.partial[(int64_t)n * p.a.channels + c];
   }
   part[k][column] = sum;
   __syncthreads();
   if (k == 0 && c < p.a.channels) {
     for (int n = 1; n < kRecSumParts; n++) sum += part[n][column];
-    StoreElement(p.a.ddecay, c, p.a.decay_dtype, sum);
+    StoreElement(p.a.ddecay, c, p.a.decay_dtype, (float)sum);
   }
 }
 

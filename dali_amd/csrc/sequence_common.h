@@ -233,7 +233,8 @@ __device__ __forceinline__ void LogisticPair(float g, float *f, float *k) {
   *f = g < 0 ? small : big;
   *k = g < 0 ? big : small;
 }
-// The smaller one of f and 1 - f to its last bits, negative where that is f: of the other, which is near 1, it is all that matters.
+// The smaller one of f and 1 - f, negative where that is f: of the other, which is near 1, it is all that matters.  To its last bits if EXACT;
+// without, it is off by |g| 2^-24 of itself, a 2^-16th (bf16; f16: 2^-13th) of what the half step that g was rounded by makes of it.
 template <bool EXACT> __device__ __forceinline__ float SmallerOfLogistic(float g) {
   return copysignf(Reciprocal(1.0f + ExpOf<EXACT>(fabsf(g))), g);
 }

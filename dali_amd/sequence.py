@@ -67,7 +67,12 @@ def linear_recurrence(x, decay, *, form="decay", initial_state=None, offsets=Non
     final_state    a float32 tensor [sequences, channels] that receives the state and is returned as such; it may be
                    `initial_state` itself, which is then updated in place.  Not while gradients are recorded.
 
-    Gradients with respect to x, decay and initial_state; the state may be differentiated as well."""
+    Gradients with respect to x, decay and initial_state; the state may be differentiated as well.
+
+    States and gradients are held in 32 bits, products of decays in 64; the gradient of a decay per channel is a sum in 32 bits over
+    256 rows and in 64 bits over these sums.  A gate is taken to the last bits of 32 if `decay` is float32.  Of 16-bit types the
+    logistic function leaves out the rounding of its argument, |decay| 2^-24 relative, far below what such a decay is rounded to
+    itself; this holds for the state in 32 bits as well."""
     return (_module or _ops()).linear_recurrence(x, decay, form, initial_state, offsets, lengths, final_state)
 
 

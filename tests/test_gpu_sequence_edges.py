@@ -448,6 +448,21 @@ def test_recurrence_of_more_short_sequences_than_tiles_of_their_own():
         assert torch.equal(dx[part, :, 0].to(torch.int32), (torch.cumsum(d, 1).to(torch.int32)).flip(1) * sign)
 
 
+def test_recurrence_gradient_per_channel_is_a_sum_over_many_rows():
+    """2^28 rows, of which 256 at a time are added up in 32 bits (at most 8 + 2 + 8 roundings), those sums in 64, and the result is rounded
+    once.  With a decay of 0 a state is the input itself, and a term of the sum one product."""
+    enough_memory(30)
+    torch.manual_seed(2)
+    x, dy = (torch.empty(2 ** 13, 2 ** 15, 4, device="cuda").uniform_(0, 1) for _ in range(2))
+    a = leaf(torch.zeros(4).cuda())
+    y, _ = sequence.linear_recurrence(x, a)
+    got, = torch.autograd.grad(y, a, dy)
+    want = torch.zeros(4, dtype=torch.float64, device="cuda")
+    for s in range(0, 2 ** 13, 32):
+        want += (x[s:s + 32, :-1].double() * dy[s:s + 32, 1:].double()).sum((0, 1))
+    assert ((got.double() - want).abs() <= 20 * R.U * want).all(), (got.double() / want - 1).abs() / R.U
+
+
 def test_more_rows_and_channels_than_one_launch_may_have_are_refused():
     lib, plan = capi.kernels(), capi.RecurrencePlan()
     a = capi.RecurrenceArgs()
