@@ -305,7 +305,7 @@ __device__ __forceinline__ void Mark(const RecKernelArgs &p, const RecPlace &pla
     }
   } else if (tid < kRecTile) {
     int begin = 0, end = 0;
-    const int s = row < place.limit ? FindSequence(q, row, &begin, &end) : -1;
+    const int s = row < place.limit ? FindDenseSequence(q, row, &begin, &end) : -1;
     marks.live[tid] = s >= 0;
     marks.first[tid] = s >= 0 && row == begin ? s : -1;
     marks.last[tid] = s >= 0 && row == end - 1 ? s : -1;
@@ -458,7 +458,6 @@ template <int V> __device__ __forceinline__ void PassEmpty(const RecKernelArgs &
   }
 }
 
-constexpr bool kKeepForward = true;
 constexpr int kForwardWaves = 4;
 // Waves per SIMD that the backward pass' registers are to leave room for: two workgroups per compute unit.  16-bit rows with
 // decays of 32 bits do not fit (272 bytes spilled: 236 us against 142 for 8 x 4096 x 1024 with one): one.
@@ -502,7 +501,7 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> st
     const int row = place.row + lane.Stretch() * kRecSteps, limit = place.limit;
     RecEvents e = {};
     if (EVENTS) e = EventsOf(marks, lane.Stretch());
-    RecCoefficients<Decay, Tile, PER_CHANNEL, kKeepForward> c;
+    RecCoefficients<Decay, Tile, PER_CHANNEL, true> c;
     float s[V], state[V];
     double a[V];
     const bool r = Compose<EVENTS>(p, decay, t, e, row, lane.own, c, a, s);
@@ -510,10 +509,6 @@ template <typename XT, typename GT, int FORM, bool PER_CHANNEL, bool COMPARE> st
     c.Forget();
 #pragma unroll
     for (int k = 0; k < kRecSteps; k++) t.x[k].Repack();
-    if (!PER_CHANNEL && !kKeepForward) {
-#pragma unroll
-      for (int k = 0; k < kRecSteps; k++) t.g[PER_CHANNEL ? 0 : k].Repack();
-    }
     __syncthreads();
     const bool starts = place.sequence < 0 || place.row == place.begin;
     FindFront<false, Decay::kGate, XT>(p, shared, tile, channel_tile, !starts, starts && !EVENTS ? p.a.initial : nullptr, place.sequence);

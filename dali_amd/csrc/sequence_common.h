@@ -119,11 +119,7 @@ template <int V, bool WHOLE = false> struct Channels {
       LoadWide(g, At(row));
     }
   }
-  // ... with zeros in the places of others
-  template <typename T> __device__ __forceinline__ void LoadOwn(Group<T, V> &g, const T *row) const {
-    Load(g, row);
-    Mask(g);
-  }
+  // zeros in the places of others
   template <typename T> __device__ __forceinline__ void Mask(Group<T, V> &g) const {
 #pragma unroll
     for (int k = 0; k < Group<T, V>::kWords; k++) {
@@ -183,21 +179,11 @@ __device__ __forceinline__ void SequenceRange(const daliamdSequenceRows &q, int 
   }
 }
 
-// the sequence that `row` belongs to, or -1: with ascending offsets the last one that begins at or before it
-__device__ __forceinline__ int FindSequence(const daliamdSequenceRows &q, int row, int *begin, int *end) {
-  int s;
-  if (q.offsets) {
-    int lo = 0, hi = q.sequences - 1;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo + 1) / 2;
-      if (LoadIndex(q.offsets, mid, q.index_dtype) <= row) lo = mid; else hi = mid - 1;
-    }
-    s = lo;
-  } else {
-    s = (uint32_t)row / (uint32_t)q.steps;
-  }
+// dense: the sequence that `row` belongs to, or -1 if it is padding
+__device__ __forceinline__ int FindDenseSequence(const daliamdSequenceRows &q, int row, int *begin, int *end) {
+  const int s = (uint32_t)row / (uint32_t)q.steps;
   SequenceRange(q, s, begin, end);
-  return *begin <= row && row < *end ? s : -1;
+  return row < *end ? s : -1;
 }
 
 // The logistic function f(g) = 1 / (1 + exp(-g)) in the instructions that the hardware has for it: 2^x and 1 / x, each good to the
