@@ -379,13 +379,19 @@ def test_embedding_table_changed_before_the_backward_pass():
 
 
 # ------------------------------------------------------------------ more threads than one launch may have (2^32)
-def enough_memory(gigabytes):
-    if MODEL or torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
-        pytest.skip("not enough memory on the device")
-    torch.cuda.empty_cache()
+@pytest.fixture
+def enough_memory():
+    def need(gigabytes):
+        if MODEL or torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
+            pytest.skip("not enough memory on the device")
+    if not MODEL:
+        torch.cuda.empty_cache()
+    yield need
+    if not MODEL:
+        torch.cuda.empty_cache()
 
 
-def test_embedding_of_as_many_tokens_as_there_may_be():
+def test_embedding_of_as_many_tokens_as_there_may_be(enough_memory):
     """2^31 - 1 tokens of one channel: the lookup, and the join of 2^26 chunks of 32 sorted tokens.  Counts are exact in 32 bits."""
     enough_memory(90)
     count, vocab = 2 ** 31 - 1, 300
@@ -402,7 +408,7 @@ def test_embedding_of_as_many_tokens_as_there_may_be():
     assert torch.equal(got[:, 0].long(), counts)
 
 
-def test_embedding_of_a_table_of_more_rows_than_one_launch_fills():
+def test_embedding_of_a_table_of_more_rows_than_one_launch_fills(enough_memory):
     enough_memory(40)
     vocab = 2 ** 30 + 1000
     table = torch.empty(vocab, 2, dtype=HF, device="cuda").fill_(1).requires_grad_(True)
@@ -414,7 +420,7 @@ def test_embedding_of_a_table_of_more_rows_than_one_launch_fills():
     assert not got.any()
 
 
-def test_recurrence_of_more_sequences_than_one_launch_steps_through():
+def test_recurrence_of_more_sequences_than_one_launch_steps_through(enough_memory):
     """One step of 1.45e9 sequences of 5 channels: a thread has two channels, so three threads each."""
     enough_memory(130)
     n = 1_450_000_000
@@ -426,7 +432,7 @@ def test_recurrence_of_more_sequences_than_one_launch_steps_through():
     assert torch.equal(y, x) and torch.equal(state, x[:, 0])
 
 
-def test_recurrence_of_more_short_sequences_than_tiles_of_their_own():
+def test_recurrence_of_more_short_sequences_than_tiles_of_their_own(enough_memory):
     """8 400 000 sequences of 129 steps, of which a tile of 256 rows would have one: sums of -1, 0 and 1 with changing sign, exact in
     every type; in both directions of time."""
     enough_memory(60)
@@ -448,7 +454,7 @@ def test_recurrence_of_more_short_sequences_than_tiles_of_their_own():
         assert torch.equal(dx[part, :, 0].to(torch.int32), (torch.cumsum(d, 1).to(torch.int32)).flip(1) * sign)
 
 
-def test_recurrence_gradient_per_channel_is_a_sum_over_many_rows():
+def test_recurrence_gradient_per_channel_is_a_sum_over_many_rows(enough_memory):
     """2^28 rows, of which 256 at a time are added up in 32 bits (at most 8 + 2 + 8 roundings), those sums in 64, and the result is rounded
     once.  With a decay of 0 a state is the input itself, and a term of the sum one product."""
     enough_memory(30)
