@@ -35,14 +35,15 @@
 // reason coefficients are computed again from the decays (4 times) rather than kept.  (BackwardChainFirst names the types for which
 // registers do not decide, and the chain comes first.)
 //
-// Measured (bf16, 8 sequences of 4096 steps, 2048 channels; a copy of 1 GiB runs at 5138 GB/s on the same card): forward 110 us for
-// 403 MB, 3.7 TB/s; backward 196 us for 671 MB, 3.4 TB/s (225 us with everything in 204 registers and one workgroup per compute
-// unit).  What bounds it is how much is on its way at once: of the 10.6 us that a workgroup of the forward pass lives, its loads take
-// 2.4, the scan 3 and the chain 3.3, and there are two per compute unit; without the chain it takes 85 us.  Tried and slower: tiles of
-// 64 and of 512 rows; three workgroups per compute unit (80 registers); workgroups that stay and load the next tile meanwhile (they
-// hold a place in the chain that they do not work on); a chain that all waves listen to; two levels of groups; equal sequences step
-// by step (each tile's predecessor long done, but rows far apart in memory at a time).  Products of decays in 32 bits take the same
-// time: vector issue is not the bound.
+// Measured (gates, bf16, 8 sequences of 4096 steps, 2048 channels; a copy of 1 GiB runs at 5138 GB/s on the same card): forward 118 us
+// for 403 MB, 3.4 TB/s; backward 209 us for 671 MB, 3.2 TB/s (with everything in 204 registers and one workgroup per compute unit it
+// was 12 % slower).  Decays instead of gates take 7 and 16 % less.  What bounds it is how much is on its way at once, and vector issue
+// adds to that.  Holding a gate by the smaller one of f and 1 - f is a quarter more vector instructions than by 1 - f alone, and 5 % of
+// the time; without that, a workgroup of the forward pass lived for 10.6 us, of which its loads took 2.4, the scan 3 and the chain 3.3,
+// with two per compute unit, and without the chain the pass took 85 us for 110.  Tried and slower: tiles of 64 and of 512 rows; three workgroups
+// per compute unit (80 registers); workgroups that stay and load the next tile meanwhile (they hold a place in the chain that they do
+// not work on); a chain that all waves listen to; two levels of groups; equal sequences step by step (each tile's predecessor long
+// done, but rows far apart in memory at a time); the composition against time in the pass of the other one (256 bytes spilled).
 #ifndef DALI_AMD_CSRC_RECURRENCE_H_
 #define DALI_AMD_CSRC_RECURRENCE_H_
 

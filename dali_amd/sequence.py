@@ -58,21 +58,23 @@ def linear_recurrence(x, decay, *, form="decay", initial_state=None, offsets=Non
                    only because what such decays make of its past is taken away again by x loses its digits.
     initial_state  h_0, float32 [sequences, channels]; zeros if None.  To go on with a sequence pass the state of the call
                    before: one step at a time gives what one call over all steps gives, up to rounding.
-    offsets        int32 or int64 [sequences + 1], ascending, on the device: sequence s has the rows offsets[s] up to
-                   offsets[s + 1].  Sequences may be empty: their state is h_0.
+    offsets        int32 or int64 [sequences + 1], on the device: sequence s has the rows offsets[s] up to offsets[s + 1].
+                   Sequences may be empty: their state is h_0.  They have to ascend, or the results are undefined.
     lengths        int32 or int64 [batch], on the device: only the first lengths[b] steps of x[b] are its sequence.
                    Rows of no sequence (padding, rows in front of the first offset and behind the last) give zeros in y and
                    in the gradients, whatever they hold.  The device reads offsets and lengths: values out of range are
                    clamped, not reported.
     final_state    a float32 tensor [sequences, channels] that receives the state and is returned as such; it may be
-                   `initial_state` itself, which is then updated in place.  Not while gradients are recorded.
+                   `initial_state` itself, which is then updated in place, or overlap it, but no other input.  Not while
+                   gradients are recorded.
 
     Gradients with respect to x, decay and initial_state; the state may be differentiated as well.
 
     States and gradients are held in 32 bits, products of decays in 64; the gradient of a decay per channel is a sum in 32 bits over
     256 rows and in 64 bits over these sums.  A gate is taken to the last bits of 32 if `decay` is float32.  Of 16-bit types the
     logistic function leaves out the rounding of its argument, |decay| 2^-24 relative, far below what such a decay is rounded to
-    itself; this holds for the state in 32 bits as well."""
+    itself; this holds for the state in 32 bits as well.  An infinite x or state makes its channel infinite or NaN up to the end of its
+    sequence, and no other."""
     return (_module or _ops()).linear_recurrence(x, decay, form, initial_state, offsets, lengths, final_state)
 
 
@@ -85,7 +87,7 @@ def block_norm(x, *, gate=None, residual=None, post_weight=None, scale=None, pre
       normed = hidden rstd(hidden) pre_weight   norm before the next block (without pre_weight: None)
 
     rstd(z) = 1 / sqrt(mean(z^2) + eps) over the channels, silu(g) = g / (1 + exp(-g)).  block_norm(x, pre_weight=w)[1] is
-    the plain root mean square norm.
+    the plain root mean square norm.  Sums of squares are held in 32 bits: a row whose sum passes 3.4e38 is normalised to zeros.
 
     x, gate, residual  [..., channels] of one shape, up to 16384 channels: float32, float16 or bfloat16; gate has x's type, the
                        residual x's or float32.  Adjacent channels have to be adjacent in memory, rows may be any distance
@@ -98,7 +100,7 @@ def block_norm(x, *, gate=None, residual=None, post_weight=None, scale=None, pre
 
 
 def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, dtype=None):
-    """scale * table[ids], rounded once: [*ids.shape, channels].
+    """scale * table[ids], in 32 bits (so is scale) and rounded once: [*ids.shape, channels].
 
     ids          int32 or int64, any shape.  The device reads them: an id outside the table gives a row of zeros and takes no
                  part in the gradient; it is not reported.
@@ -106,6 +108,7 @@ def embedding_lookup(ids, table, *, scale=1.0, padding_idx=None, dtype=None):
     padding_idx  a row of the table whose gradient stays zero (0 <= padding_idx < vocab, or negative: from the end).
     dtype        type of the result (default: the table's).
 
-    The gradient of the table is dense: for each row, scale times the sum of its tokens' gradients, in 32 bits and in the
-    order of the tokens, rounded once."""
+    The gradient of the table is dense: for each row, scale times the sum of its tokens' gradients, in 32 bits, in an order that
+    the ids alone decide (pieces of up to 32 tokens in their order, then the pieces), rounded once.  It does not depend on the table's values,
+    which may change before the backward pass."""
     return (_module or _ops()).embedding_lookup(ids, table, scale, padding_idx, dtype)

@@ -763,7 +763,7 @@ DALIAMD_API daliamdResult_t daliamdNormalizeRun(daliamdStream_t stream, const da
  *           (device, [sequences]) only the first lengths[s] steps of block s are rows of the sequence;
  *   packed  offsets (device, [sequences + 1], ascending): sequence s has the rows [offsets[s], offsets[s + 1]) of `rows`.
  * Both are read on the device: values outside [0, rows] (or [0, steps]) are clamped, no row outside the tensors is ever
- * touched.  Rows of no sequence get zeros in the outputs (gradients too); their inputs are not used.
+ * touched (offsets that do not ascend leave results of the sequences concerned undefined).  Rows of no sequence get zeros in the outputs (gradients too); their inputs are not used.
  * -------------------------------------------------------------------------------------------- */
 typedef struct {
   const void *offsets, *lengths;  /* device, index_dtype; at most one of the two                        */
@@ -838,8 +838,9 @@ DALIAMD_API daliamdResult_t daliamdBlockNormBackwardRun(daliamdStream_t stream, 
                                                         size_t workspace_bytes);
 
 /* out_i = scale * table[ids_i] (zeros for an id outside [0, vocab)), rounded once.
- * Backward: dtable_v = scale * sum over { i : ids_i = v } of dout_i, added up in the order of i, for every row v of the
- * table (zeros where no token is v, and for v == padding); the tokens are sorted in the workspace. */
+ * Backward: dtable_v = scale * sum over { i : ids_i = v } of dout_i for every row v of the table (zeros where no token is v, and
+ * for v == padding).  The tokens are sorted in the workspace, equal ids in the order of i, and added up in 32 bits in an order that
+ * depends on the ids alone: runs inside pieces of 8 to 32 sorted tokens, then the pieces of a run in four stretches, then these. */
 typedef struct {
   const void *ids;                /* device, [tokens], index_dtype                                      */
   const void *table;              /* [vocab][channels], rows table_row elements apart                   */
