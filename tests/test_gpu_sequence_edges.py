@@ -296,6 +296,25 @@ def test_recurrence_gates_of_all_sizes(batch, steps, low, high, dtype, gdtype):
     R.check("state", last, ref["state"], F, e["state"] + 2.0 ** -99)
 
 
+@pytest.mark.parametrize("dtype,gdtype", [(F, F), (BF, BF), (HF, F)])
+@pytest.mark.parametrize("low,high", [(-40, -4), (-40, 40)])
+def test_recurrence_gates_of_all_sizes_packed(low, high, dtype, gdtype):
+    """Sequences that begin and end inside the pieces, none, one and many steps long."""
+    c, lens = 40, [5, 0, 300, 1, 257, 40, 0, 3]
+    rows, rng = sum(lens), np.random.default_rng(565)
+    ends = np.cumsum([0] + lens)
+    x = torch.from_numpy(rng.normal(size=(rows, c)) * 10.0 ** rng.uniform(-2, 2, (rows, c))).to(dtype).cuda()
+    g = torch.from_numpy(rng.uniform(low, high, (rows, c))).to(gdtype).cuda()
+    h0, dy, dlast = rand(566, len(lens), c, scale=100.0), rand(567, rows, c, dtype=dtype), rand(568, len(lens), c)
+    leaves = [leaf(t) for t in (x, g, h0)]
+    y, state = sequence.linear_recurrence(leaves[0], leaves[1], form="gate", initial_state=leaves[2], offsets=torch.from_numpy(ends).cuda())
+    dx, dg, dinitial = torch.autograd.grad((y, state), leaves, (dy, dlast))
+    per_step = 12 + (0 if gdtype == F else max(abs(low), abs(high)))
+    ref, e = elementwise(R.f64(x), R.f64(g), list(zip(ends[:-1], ends[1:])), R.f64(h0), R.f64(dy), R.f64(dlast), per_step)
+    for name, got, t in (("y", y, dtype), ("state", state, F), ("dx", dx, dtype), ("dg", dg, gdtype), ("dinitial", dinitial, F)):
+        R.check(name, got, ref[name], t, e[name] + 2.0 ** -99)
+
+
 # ------------------------------------------------------------------ decays of more than 1
 @pytest.mark.parametrize("one", [False, True])
 @pytest.mark.parametrize("decay", [100.0, -3e38])
